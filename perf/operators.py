@@ -168,6 +168,9 @@ def prepare(case, seed):
         st["pages"] = order
         st["pool"] = _q8_pages(g, n_pages, hkv, page, d)
         st["q_out"] = torch.empty(n, hq, d, dtype=torch.float16, device="cuda")
+        if own:   # the view of its pool that a program keeps
+            from helm_amd.kernels import attention as ka
+            st["view"] = ka.Q8PoolView.of_pool(*st["pool"])
         return st
     if kind == "attn":
         hkv, d, page = case["hkv"], case["d"], case["page"]
@@ -177,8 +180,9 @@ def prepare(case, seed):
         st["q"] = _normal(g, case["b"], case["hq"], d)
         st["pool"] = _q8_pages(g, case["b"] * cols, hkv, page, d)
         st["page_table"], st["seq_lens"] = order.view(case["b"], cols), n
-        if own:   # the split workspace that a decode loop keeps
+        if own:   # the view of its pool and the split workspace that a decode loop keeps
             from helm_amd.kernels import attention as ka
+            st["view"] = ka.Q8PoolView.of_pool(*st["pool"])
             st["workspace"] = ka.AttnWorkspace(st["q"].device)
         return st
     m, v = case["m"], case["v"]
@@ -217,15 +221,14 @@ def _run_own(st):
     if kind == "int4":
         return int4_linear(st["x"], st["weight"], st["bias"])
     if kind == "append":
-        pool = ka.Q8PoolView.of_pool(*st["pool"])
         q = fused.qk_norm_rope_append_q8(st["qkv"], st["q_norm"], st["k_norm"], EPS, st["positions"], st["inv_freq"],
-                                         st["q_out"], pool, st["slots"], st["offsets"], case["hq"], case["hkv"],
-                                         case["d"], case["page"])
-        held = ka.dequantize_pages(pool, st["pages"])
+                                         st["q_out"], st["view"], st["slots"], st["offsets"], case["hq"],
+                                         case["hkv"], case["d"], case["page"])
+        held = ka.dequantize_pages(st["view"], st["pages"])
         return q, held.k, held.v
     if kind == "attn":
-        return ka.paged_decode_attention_q8(st["q"], ka.Q8PoolView.of_pool(*st["pool"]), st["page_table"],
-                                            st["seq_lens"], case["page"], workspace=st["workspace"])
+        return ka.paged_decode_attention_q8(st["q"], st["view"], st["page_table"], st["seq_lens"], case["page"],
+                                            workspace=st["workspace"])
     return fused.sample(st["logits"], st["u"], st["temperature"], st["top_k"], st["top_p"], st["min_p"],
                         workspace=st["workspace"])
 
