@@ -61,6 +61,15 @@ _SIGNATURES = {
     "helm_silu_mul": [_vp, _vp, _vp, _i64, _vp],
     "helm_fp16_gemv_rmsnorm": [_vp, _i64, _vp, _f32, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp],
     "helm_argmax_f16": [_vp, _i64, _i32, _i32, _vp, _vp],
+    "helm_int4_linear": [_vp, _i64, _vp, _vp, _i32, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _i64, _vp],
+    "helm_kv_append_q8": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp],
+    "helm_qk_norm_rope_append_q8": [_vp, _i64, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _i32,
+                                    _i32, _i32, _i32, _i32, _vp],
+    "helm_dequantize_pages": [_vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp],
+    "helm_paged_decode_attn_q8": [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32,
+                                  _i32, _i32, _i32, _i32, _i32, _f32, _vp],
+    "helm_sample": [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _f32, _i32, _f32, _f32, _vp, _vp,
+                    _i64, _vp],
     "helm_argmax_f16_ws": [_vp, _i64, _i32, _i32, _vp, _vp, _i64, _vp],
 }
 _OTHER = {
@@ -69,6 +78,8 @@ _OTHER = {
     "helm_paged_attn_workspace_floats": ([_i32, _i32, _i32, _i32], _i64),
     "helm_paged_attn_max_split_pages": ([], _i32),
     "helm_paged_attn_noalloc_max_floats": ([], _i64),
+    "helm_int4_linear_workspace_bytes": ([_i32, _i32, _i32], _i64),
+    "helm_sample_workspace_bytes": ([_i32, _i32], _i64),
     "helm_argmax_workspace_bytes": ([_i32], _i64),
     "helm_prefill_attn_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32], _i64),
     "helm_int8_gemv_workspace_bytes": ([_i32, _i32, _i32], _i64),
@@ -141,6 +152,16 @@ def call(name: str, *args) -> None:
         check(rc)
 
 
+def call_on(device: torch.device, name: str, *args) -> None:
+    """`call` with `device` as the current GPU: a launch belongs to the GPU of its
+    stream, whichever one is current in the caller's program."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
+
+
 def version() -> str:
     return lib().helm_version().decode()
 
@@ -168,6 +189,12 @@ def require_cuda(*tensors: Optional[torch.Tensor], what: str = "helm_amd") -> No
         if t is not None and not t.is_cuda:
             raise RuntimeError(f"{what}: tensors must be on the GPU (got {t.device}); "
                                "this library has no CPU path")
+
+
+def require_same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"{what}: tensors must be on one GPU (got {first.device} and {t.device})")
 
 
 def workspace_floats(B: int, Hq: int, D: int, total_splits: int) -> int:

@@ -73,6 +73,9 @@ bool launch_xreg_fp16(const void* x, int64_t ldx, const void* norm_w, float eps,
                       int64_t ldw, const void* bias, void* y, int64_t ldy, int M, int N, int K,
                       hipStream_t stream);
 
+// Checks of a pool of 8-bit pages (kv_q8.hip): 0, or the error code with its message set.
+int check_q8_pool(const helm_kv_pool_q8* pool, int Hkv, int D, int P, const char* fn);
+
 }  // namespace helm
 
 // ---------------------------------------------------------------------------

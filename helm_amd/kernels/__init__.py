@@ -13,6 +13,9 @@ patch_cpu_linears(module, verbose)     patch_linears(module, verbose, exclude) (
                                        weights kept, FP16Linear = _AVXLinear)
 HELM_DISABLE_AVX (env) :80             HELM_DISABLE_GEMV (env): fp16_linear decode calls
                                        take the fp32 F.linear branch (ablation)
+(none)                                 int4_linear(input, weight, bias), Int4Weight,
+                                       Int4Linear, patch_int4_linears (4-bit weights,
+                                       a scale per group of inputs)
 is_available() :91-94                  is_available()
 load_error() :97-100                   load_error()
 =====================================  =============================================
@@ -27,6 +30,7 @@ from __future__ import annotations
 
 import functools
 import os
+from dataclasses import dataclass
 from typing import Iterable, Optional, Tuple
 
 import torch
@@ -37,6 +41,7 @@ from .._native import is_available, load_error
 
 __all__ = [
     "int8_linear", "fp16_linear", "quantize_per_channel", "dequantize",
+    "quantize_int4", "Int4Weight", "int4_linear", "Int4Linear", "patch_int4_linears",
     "Int8Linear", "patch_linears", "FP16Linear", "patch_fp16_linears", "patch_cpu_linears",
     "is_available", "load_error", "GEMV_MAX_TOKENS",
 ]
@@ -257,6 +262,194 @@ def patch_linears(module: nn.Module, verbose: bool = False,
             count += patch_linears(child, verbose=verbose, exclude=exclude)
     if verbose and count:
         print(f"[helm_amd.kernels] patched {count} nn.Linear -> Int8Linear under "
+              f"{module.__class__.__name__}")
+    return count
+
+
+def quantize_int4(weight: torch.Tensor, group_size: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Symmetric 4-bit quantisation of a [N, K] weight in groups of `group_size` inputs:
+    codes int8 [N, K] and scales fp16 [N, K / group_size],
+
+    scale[n, g] = fp16(max_{k in g} |W[n, k]| / 7)
+    c[n, k]     = clamp(round_half_even(W[n, k] / scale[n, g]), -8, 7)   (0 if the scale is 0)
+    """
+    if weight.dim() != 2 or group_size not in (32, 64, 128) or weight.shape[1] % group_size:
+        raise ValueError(f"quantize_int4: expected a 2-D weight whose inputs are a multiple of the group size "
+                         f"(32, 64 or 128), got {tuple(weight.shape)} and {group_size}")
+    N, K = weight.shape
+    w = weight.detach().float().view(N, K // group_size, group_size)
+    scale = (w.abs().amax(-1) / 7.0).to(torch.float16)
+    s32 = scale.float()[..., None]
+    c = torch.round(w / torch.where(s32 > 0, s32, torch.ones_like(s32))).clamp_(-8, 7)
+    c = torch.where(s32 > 0, c, torch.zeros_like(c))
+    return c.to(torch.int8).view(N, K), scale.contiguous()
+
+
+@dataclass
+class Int4Weight:
+    """4-bit weights in the layout the kernels read (helm_int4_linear): `qweight` int32
+    [ceil(N/16), ceil(K/128), 64, 4], `scale` fp16 [ceil(N/16), ceil(K/128),
+    128/group_size, 16]; made once by `pack`, from codes or a weight."""
+    qweight: torch.Tensor
+    scale: torch.Tensor
+    out_features: int
+    in_features: int
+    group_size: int
+
+    @staticmethod
+    def pack(codes: torch.Tensor, scale: torch.Tensor) -> "Int4Weight":
+        """codes int8 [N, K] in [-8, 7] and fp16 scales [N, K / group_size] (group_size
+        32, 64 or 128: the quotient), on any device; the packed weight stays there."""
+        if codes.dim() != 2 or codes.dtype != torch.int8 or scale.dim() != 2 or scale.dtype != torch.float16:
+            raise RuntimeError("Int4Weight: codes must be int8 [N, K] and scale fp16 [N, K / group_size]")
+        N, K = codes.shape
+        if N == 0 or K == 0 or scale.shape[0] != N or scale.shape[1] == 0 or K % scale.shape[1]:
+            raise RuntimeError(f"Int4Weight: scale {tuple(scale.shape)} does not fit codes {tuple(codes.shape)}")
+        gs = K // scale.shape[1]
+        if gs not in (32, 64, 128):
+            raise RuntimeError(f"Int4Weight: group size must be 32, 64 or 128 (got {gs})")
+        if bool(((codes < -8) | (codes > 7)).any()):
+            raise RuntimeError("Int4Weight: codes must be in [-8, 7]")
+        nt, kt = -(-N // 16), -(-K // 128)
+        u = torch.full((nt * 16, kt * 128), 8, dtype=torch.uint8, device=codes.device)
+        u[:N, :K] = (codes + 8).to(torch.uint8)
+        # [tile, row, tile, word, lane group, pair, odd] -> [tile, tile, lane group, row, word, pair, odd]
+        u = u.view(nt, 16, kt, 4, 4, 4, 2).permute(0, 2, 4, 1, 3, 5, 6)
+        # nibble 4p of the low half: input 2p, of the high half: input 2p + 1
+        b = torch.empty(nt, kt, 4, 16, 4, 4, dtype=torch.uint8, device=codes.device)
+        for odd in (0, 1):
+            b[..., 2 * odd] = u[..., 0, odd] | (u[..., 1, odd] << 4)
+            b[..., 2 * odd + 1] = u[..., 2, odd] | (u[..., 3, odd] << 4)
+        s = torch.zeros(nt * 16, kt * 128 // gs, dtype=torch.float16, device=scale.device)
+        s[:N, :K // gs] = scale
+        s = s.view(nt, 16, kt, 128 // gs).permute(0, 2, 3, 1).contiguous()
+        return Int4Weight(b.view(torch.int32).view(nt, kt, 64, 4), s, N, K, gs)
+
+    @staticmethod
+    def from_weight(weight: torch.Tensor, group_size: int = 128) -> "Int4Weight":
+        return Int4Weight.pack(*quantize_int4(weight, group_size))
+
+    def unpack(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(codes int8 [N, K], scale fp16 [N, K / group_size]) as given to `pack`."""
+        nt, kt = self.qweight.shape[:2]
+        b = self.qweight.contiguous().view(torch.uint8).view(nt, kt, 4, 16, 4, 4)
+        u = torch.empty(nt, kt, 4, 16, 4, 4, 2, dtype=torch.uint8, device=b.device)
+        for odd in (0, 1):
+            u[..., 0, odd], u[..., 1, odd] = b[..., 2 * odd] & 15, b[..., 2 * odd] >> 4
+            u[..., 2, odd], u[..., 3, odd] = b[..., 2 * odd + 1] & 15, b[..., 2 * odd + 1] >> 4
+        c = u.permute(0, 3, 1, 4, 2, 5, 6).reshape(nt * 16, kt * 128).to(torch.int8) - 8
+        s = self.scale.permute(0, 3, 1, 2).reshape(nt * 16, -1)
+        return (c[:self.out_features, :self.in_features].contiguous(),
+                s[:self.out_features, :self.in_features // self.group_size].contiguous())
+
+    def dequantize(self) -> torch.Tensor:
+        """fp32 [N, K] weight."""
+        c, s = self.unpack()
+        return c.float() * s.float().repeat_interleave(self.group_size, 1)
+
+    def to(self, device) -> "Int4Weight":
+        return Int4Weight(self.qweight.to(device), self.scale.to(device), self.out_features, self.in_features,
+                          self.group_size)
+
+
+@functools.lru_cache(maxsize=4096)
+def int4_workspace_bytes(M: int, N: int, K: int) -> int:
+    """Workspace helm_int4_linear needs at this shape (0: none): fp32 partial sums of
+    inputs split over workgroups."""
+    return int(_native.lib().helm_int4_linear_workspace_bytes(int(M), int(N), int(K)))
+
+
+def int4_linear(input: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y = fp16(input @ W.T + bias) with 4-bit weights W = codes * scale (one scale per
+    output and group of inputs) on the GPU, fp32 accumulate.
+
+    input [..., K] fp16, weight an Int4Weight of [N, K], bias [N] fp16 or None.  Decode
+    (<= 16 tokens) scales each group's sum in fp32; above, the weights enter the product
+    as fp16(code * scale)."""
+    q, s = weight.qweight, weight.scale
+    _native.require_cuda(input, q, s, bias, what="int4_linear")
+    if input.dtype != torch.float16:
+        raise RuntimeError(f"int4_linear: input must be fp16 (got {input.dtype})")
+    N, K, gs = weight.out_features, weight.in_features, weight.group_size
+    nt, kt = -(-N // 16), -(-K // 128)
+    if (q.dtype != torch.int32 or q.shape != (nt, kt, 64, 4) or not q.is_contiguous()
+            or s.dtype != torch.float16 or s.shape != (nt, kt, 128 // gs, 16) or not s.is_contiguous()):
+        raise RuntimeError("int4_linear: weight must be laid out by Int4Weight.pack")
+    if bias is not None and (bias.dtype != torch.float16 or bias.shape != (N,) or not bias.is_contiguous()):
+        raise RuntimeError("int4_linear: bias must be fp16 [N], contiguous")
+    _native.require_same_device("int4_linear", input, q, s, bias, out)
+    x2 = _flatten(input, K, "int4_linear")
+    M = x2.shape[0]
+    if M > 1 and x2.stride(0) < K or x2.data_ptr() % 16:   # rows that overlap (an expanded input), or lie askew
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        out = torch.empty((*input.shape[:-1], N), dtype=torch.float16, device=input.device)
+    elif out.dtype != torch.float16 or out.shape != (*input.shape[:-1], N) or not out.is_contiguous():
+        raise RuntimeError("int4_linear: out must be a contiguous fp16 tensor [..., N]")
+    if M == 0:
+        return out
+    need = int4_workspace_bytes(M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=input.device) if need else None
+    _native.call_on(input.device, "helm_int4_linear", x2.data_ptr(), x2.stride(0) if M > 1 else K, q.data_ptr(),
+                    s.data_ptr(), gs, _native.ptr(bias), out.data_ptr(), N, M, N, K, _native.ptr(ws), need,
+                    _native.stream_ptr(input.device))
+    return out
+
+
+class Int4Linear(nn.Module):
+    """4-bit weight-only replacement for nn.Linear (beside Int8Linear): buffers
+    ``qweight`` and ``scale`` as Int4Weight lays them out, optional ``bias`` fp16 [out].
+    ``weight`` returns the dequantised fp16 weight (computed on access)."""
+
+    def __init__(self, weight: Int4Weight, bias: Optional[torch.Tensor] = None):
+        super().__init__()
+        self.in_features = weight.in_features
+        self.out_features = weight.out_features
+        self.group_size = weight.group_size
+        self.register_buffer("qweight", weight.qweight)
+        self.register_buffer("scale", weight.scale)
+        self.register_buffer("bias", bias)
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, group_size: int = 128) -> "Int4Linear":
+        b = linear.bias.detach().to(torch.float16) if linear.bias is not None else None
+        return cls(Int4Weight.from_weight(linear.weight, group_size), b)
+
+    @property
+    def packed(self) -> Int4Weight:
+        return Int4Weight(self.qweight, self.scale, self.out_features, self.in_features, self.group_size)
+
+    @property
+    def weight(self) -> torch.Tensor:
+        return self.packed.dequantize().to(torch.float16)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return int4_linear(x, self.packed, self.bias)
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, "
+                f"group_size={self.group_size}, bias={self.bias is not None}, int4=True")
+
+
+def patch_int4_linears(module: nn.Module, group_size: int = 128, verbose: bool = False,
+                       exclude: Iterable[str] = ()) -> int:
+    """patch_linears with 4-bit weights: replace every nn.Linear under `module` with an
+    Int4Linear; returns the number replaced.  Children whose attribute name is in
+    `exclude`, and those whose inputs are no multiple of the group size, are left."""
+    exclude = set(exclude)
+    count = 0
+    for name, child in list(module.named_children()):
+        if name in exclude:
+            continue
+        if isinstance(child, nn.Linear):
+            if child.in_features % group_size == 0:
+                setattr(module, name, Int4Linear.from_linear(child, group_size))
+                count += 1
+        else:
+            count += patch_int4_linears(child, group_size, verbose=verbose, exclude=exclude)
+    if verbose and count:
+        print(f"[helm_amd.kernels] patched {count} nn.Linear -> Int4Linear under "
               f"{module.__class__.__name__}")
     return count
 

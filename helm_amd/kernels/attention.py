@@ -1,7 +1,8 @@
 """Paged GQA decode attention and KV page writes on the GPU (functional layer).
 
 Thin typed wrappers over helm_paged_decode_attn / helm_paged_attn_reduce /
-helm_kv_append / helm_stage_pages_h2d.
+helm_kv_append / helm_stage_pages_h2d, and the same over pages held in 8 bits
+(Q8PoolView: paged_decode_attention_q8, kv_append_q8, dequantize_pages).
 
 KV layout.  A page of the reference is a pair of (1, Hkv, P, D) tensors
 (helm/runtime/kv_allocator.py:26-28).  Here every page is a slot of a pool: K is
@@ -365,6 +366,193 @@ def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, pool: PoolView, slots: t
     _native.call("helm_kv_append", k_new.data_ptr(), v_new.data_ptr(), pool.c_ref(),
                  slots.data_ptr(), offsets.data_ptr(), B, Hkv, n_tok, D, page_size,
                  _native.stream_ptr(k_new.device))
+
+
+# ── pages held in 8 bits ─────────────────────────────────────────────────────
+
+Q8_STEP_TOKENS = 64       # tokens of one wave step of the 8-bit decode attention
+
+
+class KvPoolQ8Struct(ctypes.Structure):
+    """helm_kv_pool_q8 (include/helm_mi355x.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("slot_stride", ctypes.c_int64), ("scale_slot_stride", ctypes.c_int64),
+                ("num_slots", ctypes.c_int64)]
+
+
+class Q8PoolView:
+    """Pages of int8 codes with one fp16 scale per token and kv head: the element of
+    (slot, head, token, dim) stands for code * scale.  One scale per token, so writing a
+    token leaves its page's other tokens as they are.  Logical shapes as in PoolView
+    (a slot of `k` / `v` is a [Hkv, P, D] page, V stored token-contiguous per dim);
+    `k_scale` / `v_scale` are [slots, Hkv, P].  `alloc_q8_pool` makes one."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        if (any(t.dim() != 4 or t.dtype != torch.int8 for t in (k, v)) or k.shape != v.shape
+                or any(t.dim() != 3 or t.dtype != torch.float16 or t.shape != k.shape[:3]
+                       for t in (k_scale, v_scale))):
+            raise RuntimeError("Q8PoolView: k and v must be int8 [slots, Hkv, P, D], k_scale and v_scale fp16 "
+                               "[slots, Hkv, P]")
+        slots, hkv, p, d = k.shape
+        if 0 in (slots, hkv):
+            raise RuntimeError("Q8PoolView: an empty pool")
+        if d not in (64, 128) or p not in (16, 32, 64):
+            raise RuntimeError(f"Q8PoolView: head_dim must be 64 or 128 and the page size 16, 32 or 64 (got {d}, {p})")
+        ss = k.stride(0) if slots > 1 else hkv * p * d
+        sss = k_scale.stride(0) if slots > 1 else hkv * p
+
+        def strided(t, *inner):
+            return all(n == 1 or s == w for n, s, w in zip(t.shape, t.stride(), inner))
+        if not strided(k, ss, p * d, d, 1):
+            raise RuntimeError("Q8PoolView: K pages must be token rows of D contiguous codes")
+        if not strided(v, ss, p * d, 1, p):
+            raise RuntimeError("Q8PoolView: V pages must be stored [Hkv, D, P], with K's slot stride "
+                               "(alloc_q8_pool allocates both)")
+        if not (strided(k_scale, sss, p, 1) and strided(v_scale, sss, p, 1)):
+            raise RuntimeError("Q8PoolView: scales must be [slots, Hkv, P] with contiguous pages and one slot stride")
+        if slots > 1 and (ss < hkv * p * d or sss < hkv * p):
+            raise RuntimeError("Q8PoolView: slots overlap")
+        _native.require_same_device("Q8PoolView", k, v, k_scale, v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_slots, self.num_kv_heads, self.page_size, self.head_dim = slots, hkv, p, d
+        self._struct = KvPoolQ8Struct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ss, sss,
+                                      slots)
+        self._ref = ctypes.byref(self._struct)
+
+    @staticmethod
+    def of_pool(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> "Q8PoolView":
+        return Q8PoolView(k, v, k_scale, v_scale)
+
+    def c_ref(self):
+        """A pointer to the helm_kv_pool_q8 (kept alive by this view)."""
+        return self._ref
+
+    def _check_page_size(self, page_size: Optional[int], what: str) -> int:
+        if page_size is not None and page_size != self.page_size:
+            raise RuntimeError(f"{what}: the pool's pages hold {self.page_size} tokens, not {page_size}")
+        return self.page_size
+
+
+def alloc_q8_pool(num_slots: int, num_kv_heads: int, page_size: int, head_dim: int, device=None) -> Q8PoolView:
+    """A zero-filled pool of `num_slots` 8-bit pages."""
+    k = torch.zeros(num_slots, num_kv_heads, page_size, head_dim, dtype=torch.int8, device=device)
+    v = alloc_v((num_slots, num_kv_heads, page_size, head_dim), dtype=torch.int8, device=device, zero=True)
+    s = torch.zeros(2, num_slots, num_kv_heads, page_size, dtype=torch.float16, device=device)
+    return Q8PoolView(k, v, s[0], s[1])
+
+
+@functools.lru_cache(maxsize=4096)
+def choose_q8_splits(batch: int, num_kv_heads: int, max_pages: int, page_size: int = 16) -> int:
+    """Split count of paged_decode_attention_q8: workgroups for the GPU's 256 CUs, each
+    split at least one 64-token step for each of its four waves."""
+    tokens = max(1, int(max_pages)) * page_size
+    n = max(1, min(256 // max(1, batch * num_kv_heads), tokens // (4 * Q8_STEP_TOKENS)))
+    while -(-(-(-tokens // Q8_STEP_TOKENS)) // n) * (Q8_STEP_TOKENS // page_size) > MAX_SPLIT_PAGES:
+        n += 1
+    return n
+
+
+def paged_decode_attention_q8(q: torch.Tensor, pool: Q8PoolView, page_table: torch.Tensor,
+                              seq_lens: torch.Tensor, page_size: Optional[int] = None,
+                              scale: Optional[float] = None, num_splits: Optional[int] = None,
+                              workspace: Optional[AttnWorkspace] = None,
+                              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_decode_attention over 8-bit pages: out[b, h] = softmax(scale q[b,h] K_b^T) V_b,
+    K and V the values that codes and scales stand for.
+
+    q [B, Hq, D] fp16; page_table [B, max_pages] int32 slots; seq_lens [B] int32.
+    Returns out [B, Hq, D] fp16 (zeros for an empty item)."""
+    what = "paged_decode_attention_q8"
+    _native.require_cuda(q, pool.k, page_table, seq_lens, out, what=what)
+    _native.require_same_device(what, q, pool.k, page_table, seq_lens, out)
+    if q.dtype != torch.float16 or q.dim() != 3 or q.stride(-1) != 1:
+        raise RuntimeError(f"{what}: q must be fp16 [B, Hq, D] with unit stride on D")
+    B, Hq, D = q.shape
+    P = pool._check_page_size(page_size, what)
+    if D != pool.head_dim:
+        raise RuntimeError(f"{what}: q has head_dim {D}, the pool {pool.head_dim}")
+    if (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B
+            or page_table.stride(1) != 1 and page_table.shape[1] > 1):
+        raise RuntimeError(f"{what}: page_table must be int32 [B, max_pages], row-major")
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,) or not seq_lens.is_contiguous():
+        raise RuntimeError(f"{what}: seq_lens must be int32 [B], contiguous")
+    if out is None:
+        out = torch.empty(B, Hq, D, dtype=torch.float16, device=q.device)
+    elif out.dtype != torch.float16 or out.shape != (B, Hq, D) or not out.is_contiguous():
+        raise RuntimeError(f"{what}: out must be fp16 [B, Hq, D], contiguous")
+    if B == 0:
+        return out
+    max_pages = page_table.shape[1]
+    if max_pages == 0:
+        return out.zero_()
+    if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if num_splits is None:
+        num_splits = choose_q8_splits(B, pool.num_kv_heads, max_pages, P)
+    part_o = part_ml = None
+    if num_splits > 1:
+        ws = workspace if workspace is not None else AttnWorkspace(q.device)
+        part_o, part_ml = ws.get(B, Hq, D, num_splits)
+    pts = page_table.stride(0) if B > 1 else max_pages
+    _native.call_on(q.device, "helm_paged_decode_attn_q8", q.data_ptr(), q.stride(0), q.stride(1), pool.c_ref(),
+                    page_table.data_ptr(), pts, seq_lens.data_ptr(), _native.ptr(part_o), _native.ptr(part_ml),
+                    out.data_ptr(), B, Hq, pool.num_kv_heads, D, P, max_pages, num_splits, float(scale),
+                    _native.stream_ptr(q.device))
+    return out
+
+
+def _check_places(what: str, slots: torch.Tensor, offsets: torch.Tensor, n: int) -> None:
+    for name, t in (("slots", slots), ("offsets", offsets)):
+        if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+            raise RuntimeError(f"{what}: {name} must be int32 [{n}], contiguous")
+
+
+def kv_append_q8(k_new: torch.Tensor, v_new: torch.Tensor, pool: Q8PoolView, slots: torch.Tensor,
+                 offsets: torch.Tensor, page_size: Optional[int] = None) -> None:
+    """Quantise k_new/v_new [B, Hkv, n_tok, D] fp16 into (slots[b], offsets[b] + t) of an
+    8-bit pool: scale = fp16(max |x| / 127) per token and head, code = x / scale rounded to
+    nearest even.  Tokens whose slot is outside the pool or whose offset is outside the page
+    are skipped; of two tokens for one place, one is kept (which one is not defined)."""
+    what = "kv_append_q8"
+    _native.require_cuda(k_new, v_new, pool.k, slots, offsets, what=what)
+    _native.require_same_device(what, k_new, v_new, pool.k, slots, offsets)
+    P = pool._check_page_size(page_size, what)
+    if k_new.dtype != torch.float16 or v_new.dtype != torch.float16 or k_new.dim() != 4 or k_new.shape != v_new.shape:
+        raise RuntimeError(f"{what}: k_new and v_new must be fp16 [B, Hkv, n_tok, D]")
+    B, Hkv, n_tok, D = k_new.shape
+    if (Hkv, D) != (pool.num_kv_heads, pool.head_dim):
+        raise RuntimeError(f"{what}: {Hkv} heads of {D} do not fit the pool's {pool.num_kv_heads} of {pool.head_dim}")
+    _check_places(what, slots, offsets, B)
+    if k_new.numel() == 0:
+        return
+    k_new = k_new.contiguous()
+    v_new = v_new.contiguous()
+    _native.call_on(k_new.device, "helm_kv_append_q8", k_new.data_ptr(), v_new.data_ptr(), pool.c_ref(),
+                    slots.data_ptr(), offsets.data_ptr(), B, Hkv, n_tok, D, P, _native.stream_ptr(k_new.device))
+
+
+def dequantize_pages(pool: Q8PoolView, pages: torch.Tensor) -> PoolView:
+    """fp16 copies of pages `pages` (int32 slots) of an 8-bit pool, as a PoolView whose
+    slot i is page i: each value fp16(code * scale), zeros for a slot outside the pool.
+    `prefill_attention` over it (page table arange(n)) attends a prompt that continues
+    8-bit pages."""
+    what = "dequantize_pages"
+    _native.require_cuda(pool.k, pages, what=what)
+    _native.require_same_device(what, pool.k, pages)
+    if pages.dtype != torch.int32 or pages.dim() != 1 or not pages.is_contiguous():
+        raise RuntimeError(f"{what}: pages must be a contiguous int32 vector")
+    n = pages.numel()
+    shape = (n, pool.num_kv_heads, pool.page_size, pool.head_dim)
+    k = torch.empty(shape, dtype=torch.float16, device=pages.device)
+    v = alloc_v(shape, device=pages.device)
+    if n:
+        _native.call_on(pages.device, "helm_dequantize_pages", pool.c_ref(), pages.data_ptr(), n, k.data_ptr(),
+                        v.data_ptr(), pool.num_kv_heads, pool.head_dim, pool.page_size,
+                        _native.stream_ptr(pages.device))
+    return PoolView.of_pool(k, v)
 
 
 def stage_pages_h2d(host_pool: torch.Tensor, dev_staging: torch.Tensor, host_slots,

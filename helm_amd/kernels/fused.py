@@ -8,7 +8,7 @@ projection, and q/k-norm + RoPE + the paged KV write into one kernel.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
@@ -140,6 +140,50 @@ def qk_norm_rope_append(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: tor
     return q_out
 
 
+def qk_norm_rope_append_q8(qkv: torch.Tensor, q_norm_w: Optional[torch.Tensor],
+                           k_norm_w: Optional[torch.Tensor], eps: float, positions: torch.Tensor,
+                           inv_freq: torch.Tensor, q_out: Optional[torch.Tensor], pool, slots: torch.Tensor,
+                           offsets: torch.Tensor, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                           page_size: Optional[int] = None) -> torch.Tensor:
+    """qk_norm_rope_append into an 8-bit pool (an attention.Q8PoolView): q/k RMSNorm (when
+    the norm weights are given) + RoPE of the fused qkv [B, (Hq+2Hkv)*D] in fp32, the angle
+    in 64 bits; the rotated q rounded to fp16 once into q_out [B, Hq, D], k and v quantised
+    into (slots[b], offsets[b]) with a scale per token and head, as kv_append_q8 does."""
+    what = "qk_norm_rope_append_q8"
+    _native.require_cuda(qkv, q_norm_w, k_norm_w, positions, inv_freq, q_out, pool.k, slots, offsets, what=what)
+    _native.require_same_device(what, qkv, q_norm_w, k_norm_w, positions, inv_freq, q_out, pool.k, slots, offsets)
+    _check_fp16(qkv, q_norm_w, k_norm_w, q_out)
+    Hq, Hkv, D = num_q_heads, num_kv_heads, head_dim
+    if qkv.dim() != 2 or qkv.shape[1] != (Hq + 2 * Hkv) * D or qkv.stride(1) != 1:
+        raise RuntimeError(f"{what}: qkv must be [B, (Hq + 2 Hkv) * D] with unit stride")
+    if (Hkv, D) != (pool.num_kv_heads, pool.head_dim):
+        raise RuntimeError(f"{what}: {Hkv} heads of {D} do not fit the pool's {pool.num_kv_heads} of {pool.head_dim}")
+    P = pool._check_page_size(page_size, what)
+    B = qkv.shape[0]
+    for name, t, n, dtype in (("positions", positions, B, torch.int32), ("slots", slots, B, torch.int32),
+                              ("offsets", offsets, B, torch.int32), ("inv_freq", inv_freq, D // 2, torch.float32)):
+        if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
+            raise RuntimeError(f"{what}: {name} must be {dtype} [{n}], contiguous")
+    if (q_norm_w is None) != (k_norm_w is None):
+        raise RuntimeError(f"{what}: give both q / k norm weights or neither")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.shape != (D,) or not w.is_contiguous()):
+            raise RuntimeError(f"{what}: norm weights must be [D], contiguous")
+    if q_out is None:
+        q_out = torch.empty(B, Hq, D, dtype=torch.float16, device=qkv.device)
+    elif q_out.shape != (B, Hq, D) or not q_out.is_contiguous():
+        raise RuntimeError(f"{what}: q_out must be [B, Hq, D], contiguous")
+    if B == 0:
+        return q_out
+    if B > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1]) or qkv.data_ptr() % 16:
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    _native.call_on(qkv.device, "helm_qk_norm_rope_append_q8", qkv.data_ptr(),
+                    qkv.stride(0) if B > 1 else qkv.shape[1], _native.ptr(q_norm_w), _native.ptr(k_norm_w),
+                    float(eps), positions.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(), pool.c_ref(),
+                    slots.data_ptr(), offsets.data_ptr(), B, Hq, Hkv, D, P, _native.stream_ptr(qkv.device))
+    return q_out
+
+
 def fp16_gemv_rmsnorm(x: torch.Tensor, norm_weight: torch.Tensor, eps: float,
                       weight: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = fp16(weight . rmsnorm(x)) for <= 16 tokens (final norm + lm_head)."""
@@ -199,4 +243,68 @@ def argmax(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     _native.require_cuda(workspace, what="argmax")
     _native.call("helm_argmax_f16_ws", x2.data_ptr(), x2.stride(0), M, N, out.data_ptr(),
                  workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream)
+    return out
+
+
+def sample_workspace(M: int, N: int, device) -> torch.Tensor:
+    """Workspace of helm_sample for M rows of N logits (reusable across calls on one
+    stream; calls that overlap, or two graphs that may replay at once, need one each)."""
+    return torch.empty(int(_native.lib().helm_sample_workspace_bytes(int(M), int(N))), dtype=torch.uint8,
+                       device=device)
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torch.Tensor] = 1.0,
+           top_k: Union[int, torch.Tensor] = 0, top_p: Union[float, torch.Tensor] = 1.0,
+           min_p: Union[float, torch.Tensor] = 0.0, out: Optional[torch.Tensor] = None,
+           workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A token drawn from each row of fp16 logits [..., N], int64 [...], from the random
+    numbers u [...] (fp32 in [0, 1)), beside `argmax` (helm_sample):
+
+    weights exp((x - max) / temperature); of these the top_k largest (0: all; equal logits
+    by index), of these the shortest prefix, by weight, that holds a share top_p, of these
+    the ones of at least min_p times the largest; then, in index order, the token at which
+    the summed weight passes u times the sum of all.  temperature 0 is `argmax`.  Each
+    setting is a number, or a tensor with one per row (fp32, top_k int32).  NaN logits are
+    never drawn; a row with no logit above -inf gives 0.  `workspace` from
+    sample_workspace, allocated here when not given."""
+    what = "sample"
+    tensors = [x for x in (temperature, top_k, top_p, min_p) if torch.is_tensor(x)]
+    _native.require_cuda(logits, u, out, workspace, *tensors, what=what)
+    _native.require_same_device(what, logits, u, out, workspace, *tensors)
+    _check_fp16(logits)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise RuntimeError("sample: logits must be [..., N] with N >= 1")
+    N = logits.shape[-1]
+    x2 = logits.reshape(-1, N)
+    M = x2.shape[0]
+    if x2.stride(-1) != 1 and N > 1 or M > 1 and x2.stride(0) < N:
+        x2 = x2.contiguous()
+
+    def rows(x, dtype, name):
+        if x.dtype != dtype or x.numel() != M or not x.is_contiguous():
+            raise RuntimeError(f"sample: {name} must be {dtype} with one number per row ({M}), contiguous")
+        return x.data_ptr()
+
+    def setting(x, dtype, name):
+        return (rows(x, dtype, name), 0) if torch.is_tensor(x) else (None, x)
+    up = rows(u, torch.float32, "u")
+    tp, t = setting(temperature, torch.float32, "temperature")
+    kp, k = setting(top_k, torch.int32, "top_k")
+    pp, p = setting(top_p, torch.float32, "top_p")
+    lp, lo = setting(min_p, torch.float32, "min_p")
+    if not (t >= 0.0 and k >= 0 and p >= 0.0 and lo >= 0.0):
+        raise RuntimeError("sample: temperature, top_k, top_p and min_p must not be negative")
+    if out is None:
+        out = torch.empty(logits.shape[:-1], dtype=torch.int64, device=logits.device)
+    elif out.dtype != torch.int64 or out.numel() != M or not out.is_contiguous():
+        raise RuntimeError("sample: out must be int64 with one token per row, contiguous")
+    if M == 0:
+        return out
+    if workspace is None:
+        workspace = sample_workspace(M, N, logits.device)
+    elif not workspace.is_contiguous():
+        raise RuntimeError("sample: workspace must be contiguous")
+    _native.call_on(logits.device, "helm_sample", x2.data_ptr(), x2.stride(0) if M > 1 else N, M, N, up, tp, kp, pp,
+                    lp, float(t), min(int(k), 2**31 - 1), float(p), float(lo), out.data_ptr(), workspace.data_ptr(),
+                    workspace.numel() * workspace.element_size(), _native.stream_ptr(logits.device))
     return out

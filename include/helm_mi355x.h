@@ -132,6 +132,31 @@ int helm_int8_gemm_ws(const void* x, int64_t ldx, const int8_t* q, int64_t ldq,
                       void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Linear: 4-bit weights, one scale per group of inputs                     */
+/*   y[m,n] = fp16( sum_g s[n,g] sum_{k in g} c[n,k] x[m,k]  (+ bias[n]) )  */
+/* ------------------------------------------------------------------------ */
+
+/* Any M >= 1: a matrix-core GEMV for 1-16 tokens, a tiled product above (whose weights
+ * are fp16(c * s); the GEMV applies s in fp32).  c in [-8, 7], group_size 32, 64 or 128.
+ *   x       [M, K] fp16, row stride ldx        y [M, N] fp16, row stride ldy
+ *   qweight the codes in tiles of 16 outputs x 128 inputs, NT = ceil(N / 16) by
+ *           KT = ceil(K / 128) of them: 32-bit word t (0..3) of lane l (0..63) of tile
+ *           (nt, kt), at ((nt * KT + kt) * 64 + l) * 4 + t, holds output 16 nt + l % 16,
+ *           inputs k0 = 128 kt + 32 t + 8 (l / 16) .. + 7, the codes plus 8: of input
+ *           k0 + 2p at bit 4p, of input k0 + 2p + 1 at bit 16 + 4p.  Outputs past N and
+ *           inputs past K hold code 0 (nibble 8).
+ *   scale   fp16 [NT][KT][128 / group_size][16], 0 past N and K
+ *   bias    [N] fp16 or NULL
+ * Requirements: K % group_size == 0, ldx % 8 == 0, x, qweight and scale 16-byte aligned;
+ * workspace (16-byte aligned, contents on entry do not matter) of at least
+ * helm_int4_linear_workspace_bytes (0: may be NULL).  Beside helm_int8_gemv_ws and
+ * helm_int8_gemm_ws, the counterparts of fp16_gemv.cpp:105-157. */
+int64_t helm_int4_linear_workspace_bytes(int M, int N, int K);
+int helm_int4_linear(const void* x, int64_t ldx, const void* qweight, const void* scale,
+                     int group_size, const void* bias, void* y, int64_t ldy, int M, int N, int K,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Paged GQA decode attention                                               */
 /* ------------------------------------------------------------------------ */
 /* KV storage.  One pool (or one contiguous per-layer buffer) of fp16 pages:
@@ -353,6 +378,69 @@ int helm_stage_pages_h2d(const void* host_pool, void* dev_staging,
                          size_t page_bytes, void* copy_stream, void* done_event);
 
 /* ------------------------------------------------------------------------ */
+/* KV pages held in 8 bits                                                  */
+/* ------------------------------------------------------------------------ */
+/* A pool of pages of int8 codes with one fp16 scale per token and kv head; element
+ * (slot s, kv head h, token t, dim d) stands for code * scale:
+ *   K code  at k[s*slot_stride + (h*P + t)*D + d]      K scale at k_scale[s*scale_slot_stride + h*P + t]
+ *   V code  at v[s*slot_stride + (h*D + d)*P + t]      V scale at v_scale[same]
+ * (V token-contiguous per dim, as in helm_kv_pool).  Strides in elements: slot_stride >=
+ * Hkv*P*D and a multiple of 16, scale_slot_stride >= Hkv*P and a multiple of 8; all four
+ * pointers 16-byte aligned; D 64 or 128, P 16, 32 or 64.  Slots and page-table entries
+ * outside [0, num_slots) are never dereferenced.  One scale per token: writing a token
+ * leaves every other token's bits as they are. */
+typedef struct helm_kv_pool_q8 {
+  void* k;
+  void* v;
+  void* k_scale;
+  void* v_scale;
+  int64_t slot_stride, scale_slot_stride;
+  int64_t num_slots;
+} helm_kv_pool_q8;
+
+/* helm_kv_append into 8-bit pages: scale = fp16(max |x| / 127) over the D values of a token
+ * and head, code = x / scale rounded to nearest even, in [-127, 127] (0 where the scale
+ * rounds to 0; values that are not finite give a scale that is not).  k_new / v_new
+ * [B, Hkv, n_tok, D] fp16 contiguous, token t of item b to (slots[b], offsets[b] + t);
+ * slots outside [0, num_slots) and offsets outside [0, P) are skipped.  Replaces the same
+ * copies as helm_kv_append (helm/runtime/kv_cache.py:103-107). */
+int helm_kv_append_q8(const void* k_new, const void* v_new, const helm_kv_pool_q8* pool,
+                      const int32_t* slots, const int32_t* offsets,
+                      int B, int Hkv, int n_tok, int D, int P, void* stream);
+
+/* helm_qk_norm_rope_append into 8-bit pages: per-head RMSNorm of q and k (q_norm_w /
+ * k_norm_w [D], both null for models without), RoPE at positions[b] (rotate_half; the
+ * angle positions[b] * inv_freq[i] in 64 bits, so far positions keep theirs), q rounded
+ * to fp16 once into q_out [B, Hq, D], k and v quantised as by helm_kv_append_q8 (k from
+ * fp32) into page slot slots[b] at offset offsets[b].  qkv [B, (Hq + 2*Hkv) * D] fp16,
+ * row stride qkv_stride_b (a multiple of 8; rows 16-byte aligned).  Follows
+ * helm/runtime/kv_offload.py:244-249 and kv_cache.py:103-107. */
+int helm_qk_norm_rope_append_q8(const void* qkv, int64_t qkv_stride_b, const void* q_norm_w,
+                                const void* k_norm_w, float eps, const int32_t* positions,
+                                const float* inv_freq, void* q_out, const helm_kv_pool_q8* pool,
+                                const int32_t* slots, const int32_t* offsets,
+                                int B, int Hq, int Hkv, int D, int P, void* stream);
+
+/* Pages pages[0 .. n) of an 8-bit pool as fp16 pages 0 .. n-1: k_out [n, Hkv, P, D] and
+ * v_out [n, Hkv, D, P] contiguous (a helm_kv_pool of n slots), each value fp16(code *
+ * scale); pages outside [0, num_slots) give zeros.  What helm_prefill_attn attends a prompt
+ * over that continues 8-bit pages. */
+int helm_dequantize_pages(const helm_kv_pool_q8* pool, const int32_t* pages, int n, void* k_out,
+                          void* v_out, int Hkv, int D, int P, void* stream);
+
+/* helm_paged_decode_attn and helm_paged_attn_reduce over 8-bit pages: out [B, Hq, D] fp16
+ * contiguous = softmax(scale * q . K^T) V; zeros for an item of 0 tokens.  num_splits
+ * splits, which take the table's 64-token steps round robin (at most
+ * helm_paged_attn_max_split_pages() entries each); more than one needs part_o [B, Hq,
+ * num_splits, D] and part_ml [B, Hq, num_splits, 2] (fp32), one writes out by itself.
+ * Replaces perform_streaming_attention (helm/runtime/kv_cache.py:318-442). */
+int helm_paged_decode_attn_q8(const void* q, int64_t q_stride_b, int64_t q_stride_h,
+                              const helm_kv_pool_q8* pool, const int32_t* page_table,
+                              int64_t pt_stride, const int32_t* seq_lens, float* part_o,
+                              float* part_ml, void* out, int B, int Hq, int Hkv, int D, int P,
+                              int max_pages, int num_splits, float scale, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Decode-step glue (widening around the path; no single reference counterpart) */
 /* ------------------------------------------------------------------------ */
 
@@ -408,6 +496,27 @@ int helm_argmax_f16(const void* x, int64_t ldx, int M, int N, int64_t* out, void
 int64_t helm_argmax_workspace_bytes(int M);
 int helm_argmax_f16_ws(const void* x, int64_t ldx, int M, int N, int64_t* out,
                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* A token drawn from each row of fp16 logits x [M, N] (row stride ldx), from the given
+ * random numbers u[m] in [0, 1):
+ *   1. temperature t: weights w_i = exp((x_i - max x) / t); t <= 0 takes the first
+ *      maximum (helm_argmax_f16; u and the filters are not looked at)
+ *   2. top-k (k >= 1): the k largest, of equal logits those of lower index
+ *   3. top-p (p < 1): in that order, the tokens before which less than a share p of
+ *      the weight left by step 2 lies (the first always)
+ *   4. min-p: of these, the tokens with w_i >= min_p (the first always)
+ *   5. in index order, the first token at which the weight of the tokens left, summed up
+ *      to and with it, exceeds u times the sum of all (the last with any weight for u >= 1)
+ * Weights and sums in 64 bits (a weight below 2^-45 of its neighbourhood's largest counts
+ * as 0).  NaN logits have no weight (t > 0).  A row without any logit above -inf gives
+ * its first index.  temperature / top_p / min_p (fp32 [M]) and top_k (int32 [M]) are read
+ * per row, or, where null, t / k / p / lo serve every row.  workspace: 16-byte aligned,
+ * helm_sample_workspace_bytes(M, N) bytes, contents on entry do not matter.  The sampled
+ * form of the argmax of pipeline_runtime.py:160. */
+int64_t helm_sample_workspace_bytes(int M, int N);
+int helm_sample(const void* x, int64_t ldx, int M, int N, const float* u, const float* temperature,
+                const int32_t* top_k, const float* top_p, const float* min_p, float t, int k, float p,
+                float lo, int64_t* out, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* RMSNorm: y = fp16(w * fp16(x * rsqrt(mean(x^2) + eps))), x/y [M, K] fp16. */
 int helm_rmsnorm(const void* x, const void* w, float eps, void* y,
