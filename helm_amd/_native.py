@@ -66,8 +66,8 @@ _SIGNATURES = {
     "helm_qk_norm_rope_append_q8": [_vp, _i64, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _i32,
                                     _i32, _i32, _i32, _i32, _vp],
     "helm_dequantize_pages": [_vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp],
-    "helm_paged_decode_attn_q8": [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32,
-                                  _i32, _i32, _i32, _i32, _i32, _f32, _vp],
+    "helm_paged_decode_attn_q8": [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32,
+                                  _i32, _i32, _f32, _i32, _vp, _i64, _vp],
     "helm_sample": [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _f32, _i32, _f32, _f32, _vp, _vp,
                     _i64, _vp],
     "helm_argmax_f16_ws": [_vp, _i64, _i32, _i32, _vp, _vp, _i64, _vp],
@@ -79,6 +79,7 @@ _OTHER = {
     "helm_paged_attn_max_split_pages": ([], _i32),
     "helm_paged_attn_noalloc_max_floats": ([], _i64),
     "helm_int4_linear_workspace_bytes": ([_i32, _i32, _i32], _i64),
+    "helm_paged_attn_q8_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32], _i64),
     "helm_sample_workspace_bytes": ([_i32, _i32], _i64),
     "helm_argmax_workspace_bytes": ([_i32], _i64),
     "helm_prefill_attn_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32], _i64),
@@ -152,14 +153,37 @@ def call(name: str, *args) -> None:
         check(rc)
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """`call` with `device` as the current GPU: a launch belongs to the GPU of its
+_cuda_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def call_on(index: int, name: str, *args) -> None:
+    """`call` with GPU `index` as the current one: a launch belongs to the GPU of its
     stream, whichever one is current in the caller's program."""
-    if device.index == torch.cuda.current_device():
+    if index == _cuda_device():
         call(name, *args)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             call(name, *args)
+
+
+def raw_stream(index: int) -> int:
+    """stream_ptr of GPU `index`."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def gpu_of(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """Index of the one GPU that all these tensors are on (None: an argument not given);
+    raises RuntimeError for tensors on the CPU or on several GPUs."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            index = -1
+            break
+    if index < 0:
+        require_cuda(first, *others, what=what)
+        raise RuntimeError(f"{what}: tensors must be on one GPU (got " + ", ".join(
+            sorted({str(t.device) for t in (first, *others) if t is not None})) + ")")
+    return index
 
 
 def version() -> str:
@@ -189,12 +213,6 @@ def require_cuda(*tensors: Optional[torch.Tensor], what: str = "helm_amd") -> No
         if t is not None and not t.is_cuda:
             raise RuntimeError(f"{what}: tensors must be on the GPU (got {t.device}); "
                                "this library has no CPU path")
-
-
-def require_same_device(what: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"{what}: tensors must be on one GPU (got {first.device} and {t.device})")
 
 
 def workspace_floats(B: int, Hq: int, D: int, total_splits: int) -> int:

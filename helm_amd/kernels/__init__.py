@@ -30,7 +30,6 @@ from __future__ import annotations
 
 import functools
 import os
-from dataclasses import dataclass
 from typing import Iterable, Optional, Tuple
 
 import torch
@@ -285,16 +284,24 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 128) -> Tuple[torch.Te
     return c.to(torch.int8).view(N, K), scale.contiguous()
 
 
-@dataclass
 class Int4Weight:
     """4-bit weights in the layout the kernels read (helm_int4_linear): `qweight` int32
     [ceil(N/16), ceil(K/128), 64, 4], `scale` fp16 [ceil(N/16), ceil(K/128),
-    128/group_size, 16]; made once by `pack`, from codes or a weight."""
-    qweight: torch.Tensor
-    scale: torch.Tensor
-    out_features: int
-    in_features: int
-    group_size: int
+    128/group_size, 16]; made once by `pack`, from codes and scales, or by `from_weight`.
+    Its tensors are not to be exchanged (they are checked here, once)."""
+
+    __slots__ = ("qweight", "scale", "out_features", "in_features", "group_size")
+
+    def __init__(self, qweight: torch.Tensor, scale: torch.Tensor, out_features: int, in_features: int,
+                 group_size: int):
+        nt, kt = -(-out_features // 16), -(-in_features // 128)
+        if (group_size not in (32, 64, 128) or in_features % group_size or out_features < 1 or in_features < 1
+                or qweight.dtype != torch.int32 or qweight.shape != (nt, kt, 64, 4) or not qweight.is_contiguous()
+                or scale.dtype != torch.float16 or scale.shape != (nt, kt, 128 // group_size, 16)
+                or not scale.is_contiguous() or qweight.device != scale.device):
+            raise RuntimeError("Int4Weight: tensors must be laid out by Int4Weight.pack")
+        self.qweight, self.scale = qweight, scale
+        self.out_features, self.in_features, self.group_size = out_features, in_features, group_size
 
     @staticmethod
     def pack(codes: torch.Tensor, scale: torch.Tensor) -> "Int4Weight":
@@ -367,33 +374,29 @@ def int4_linear(input: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Te
     input [..., K] fp16, weight an Int4Weight of [N, K], bias [N] fp16 or None.  Decode
     (<= 16 tokens) scales each group's sum in fp32; above, the weights enter the product
     as fp16(code * scale)."""
-    q, s = weight.qweight, weight.scale
-    _native.require_cuda(input, q, s, bias, what="int4_linear")
+    q = weight.qweight
+    index = _native.gpu_of("int4_linear", input, q, bias, out)
+    N, K = weight.out_features, weight.in_features
     if input.dtype != torch.float16:
         raise RuntimeError(f"int4_linear: input must be fp16 (got {input.dtype})")
-    N, K, gs = weight.out_features, weight.in_features, weight.group_size
-    nt, kt = -(-N // 16), -(-K // 128)
-    if (q.dtype != torch.int32 or q.shape != (nt, kt, 64, 4) or not q.is_contiguous()
-            or s.dtype != torch.float16 or s.shape != (nt, kt, 128 // gs, 16) or not s.is_contiguous()):
-        raise RuntimeError("int4_linear: weight must be laid out by Int4Weight.pack")
     if bias is not None and (bias.dtype != torch.float16 or bias.shape != (N,) or not bias.is_contiguous()):
         raise RuntimeError("int4_linear: bias must be fp16 [N], contiguous")
-    _native.require_same_device("int4_linear", input, q, s, bias, out)
     x2 = _flatten(input, K, "int4_linear")
     M = x2.shape[0]
-    if M > 1 and x2.stride(0) < K or x2.data_ptr() % 16:   # rows that overlap (an expanded input), or lie askew
-        x2 = x2.clone(memory_format=torch.contiguous_format)
+    ldx = x2.stride(0) if M > 1 else K
+    if ldx < K or x2.data_ptr() % 16:       # rows that overlap (an expanded input), or lie askew
+        x2, ldx = x2.clone(memory_format=torch.contiguous_format), K
     if out is None:
-        out = torch.empty((*input.shape[:-1], N), dtype=torch.float16, device=input.device)
+        out = input.new_empty((*input.shape[:-1], N))
     elif out.dtype != torch.float16 or out.shape != (*input.shape[:-1], N) or not out.is_contiguous():
         raise RuntimeError("int4_linear: out must be a contiguous fp16 tensor [..., N]")
     if M == 0:
         return out
     need = int4_workspace_bytes(M, N, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=input.device) if need else None
-    _native.call_on(input.device, "helm_int4_linear", x2.data_ptr(), x2.stride(0) if M > 1 else K, q.data_ptr(),
-                    s.data_ptr(), gs, _native.ptr(bias), out.data_ptr(), N, M, N, K, _native.ptr(ws), need,
-                    _native.stream_ptr(input.device))
+    ws = input.new_empty(need // 2) if need else None
+    _native.call_on(index, "helm_int4_linear", x2.data_ptr(), ldx, q.data_ptr(), weight.scale.data_ptr(),
+                    weight.group_size, None if bias is None else bias.data_ptr(), out.data_ptr(), N, M, N, K,
+                    None if ws is None else ws.data_ptr(), need, _native.raw_stream(index))
     return out
 
 
@@ -410,6 +413,7 @@ class Int4Linear(nn.Module):
         self.register_buffer("qweight", weight.qweight)
         self.register_buffer("scale", weight.scale)
         self.register_buffer("bias", bias)
+        self._packed = weight
 
     @classmethod
     def from_linear(cls, linear: nn.Linear, group_size: int = 128) -> "Int4Linear":
@@ -418,7 +422,11 @@ class Int4Linear(nn.Module):
 
     @property
     def packed(self) -> Int4Weight:
-        return Int4Weight(self.qweight, self.scale, self.out_features, self.in_features, self.group_size)
+        w = self._packed
+        if w.qweight is not self.qweight or w.scale is not self.scale:     # moved, or loaded anew
+            w = self._packed = Int4Weight(self.qweight, self.scale, self.out_features, self.in_features,
+                                          self.group_size)
+        return w
 
     @property
     def weight(self) -> torch.Tensor:

@@ -266,6 +266,14 @@ class AttnWorkspace:
             self.buf = torch.empty(n, dtype=torch.float32, device=self.device)
         return self.buf[:n_o], self.buf[n_o:n]
 
+    def reserve(self, index: int, nbytes: int) -> int:
+        """Address of at least `nbytes`, for a call on GPU `index`."""
+        if self.buf.numel() * 4 < nbytes:
+            self.buf = torch.empty(-(-nbytes // 4), dtype=torch.float32, device=self.device)
+        if self.buf.get_device() != index:
+            raise RuntimeError(f"AttnWorkspace: on {self.buf.device}, the call on GPU {index}")
+        return self.buf.data_ptr()
+
 
 def paged_decode_attention_partial(q: torch.Tensor, pool: PoolView, page_table: torch.Tensor,
                                    seq_lens: torch.Tensor, page_size: int, scale: float,
@@ -370,9 +378,6 @@ def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, pool: PoolView, slots: t
 
 # ── pages held in 8 bits ─────────────────────────────────────────────────────
 
-Q8_STEP_TOKENS = 64       # tokens of one wave step of the 8-bit decode attention
-
-
 class KvPoolQ8Struct(ctypes.Structure):
     """helm_kv_pool_q8 (include/helm_mi355x.h)."""
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
@@ -413,7 +418,8 @@ class Q8PoolView:
             raise RuntimeError("Q8PoolView: scales must be [slots, Hkv, P] with contiguous pages and one slot stride")
         if slots > 1 and (ss < hkv * p * d or sss < hkv * p):
             raise RuntimeError("Q8PoolView: slots overlap")
-        _native.require_same_device("Q8PoolView", k, v, k_scale, v_scale)
+        if not k.device == v.device == k_scale.device == v_scale.device:
+            raise RuntimeError("Q8PoolView: tensors must be on one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_slots, self.num_kv_heads, self.page_size, self.head_dim = slots, hkv, p, d
         self._struct = KvPoolQ8Struct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ss, sss,
@@ -443,70 +449,68 @@ def alloc_q8_pool(num_slots: int, num_kv_heads: int, page_size: int, head_dim: i
 
 
 @functools.lru_cache(maxsize=4096)
-def choose_q8_splits(batch: int, num_kv_heads: int, max_pages: int, page_size: int = 16) -> int:
-    """Split count of paged_decode_attention_q8: workgroups for the GPU's 256 CUs, each
-    split at least one 64-token step for each of its four waves."""
-    tokens = max(1, int(max_pages)) * page_size
-    n = max(1, min(256 // max(1, batch * num_kv_heads), tokens // (4 * Q8_STEP_TOKENS)))
-    while -(-(-(-tokens // Q8_STEP_TOKENS)) // n) * (Q8_STEP_TOKENS // page_size) > MAX_SPLIT_PAGES:
-        n += 1
-    return n
+def q8_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
+                       max_pages: int, num_splits: int = 0) -> int:
+    """Workspace of helm_paged_decode_attn_q8 (0: none)."""
+    return int(_native.lib().helm_paged_attn_q8_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim, page_size,
+                                                                max_pages, num_splits))
 
 
 def paged_decode_attention_q8(q: torch.Tensor, pool: Q8PoolView, page_table: torch.Tensor,
                               seq_lens: torch.Tensor, page_size: Optional[int] = None,
-                              scale: Optional[float] = None, num_splits: Optional[int] = None,
+                              scale: Optional[float] = None, num_splits: int = 0,
                               workspace: Optional[AttnWorkspace] = None,
                               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """paged_decode_attention over 8-bit pages: out[b, h] = softmax(scale q[b,h] K_b^T) V_b,
     K and V the values that codes and scales stand for.
 
-    q [B, Hq, D] fp16; page_table [B, max_pages] int32 slots; seq_lens [B] int32.
-    Returns out [B, Hq, D] fp16 (zeros for an empty item)."""
+    q [B, Hq, D] fp16; page_table [B, max_pages] int32 slots; seq_lens [B] int32.  `num_splits`
+    splits share an item's tokens (0: as many as suit the shape).  Returns out [B, Hq, D] fp16
+    (zeros for an empty item).  `workspace` is allocated here when not given; calls that overlap, or
+    two graphs that may replay at once, need one each."""
     what = "paged_decode_attention_q8"
-    _native.require_cuda(q, pool.k, page_table, seq_lens, out, what=what)
-    _native.require_same_device(what, q, pool.k, page_table, seq_lens, out)
-    if q.dtype != torch.float16 or q.dim() != 3 or q.stride(-1) != 1:
+    index = _native.gpu_of(what, q, pool.k, page_table, seq_lens, out)
+    if q.dtype != torch.float16 or q.dim() != 3 or q.stride(2) != 1:
         raise RuntimeError(f"{what}: q must be fp16 [B, Hq, D] with unit stride on D")
     B, Hq, D = q.shape
     P = pool._check_page_size(page_size, what)
     if D != pool.head_dim:
         raise RuntimeError(f"{what}: q has head_dim {D}, the pool {pool.head_dim}")
-    if (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B
-            or page_table.stride(1) != 1 and page_table.shape[1] > 1):
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B:
         raise RuntimeError(f"{what}: page_table must be int32 [B, max_pages], row-major")
-    if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,) or not seq_lens.is_contiguous():
+    max_pages = page_table.shape[1]
+    pts, pcs = page_table.stride()
+    if pcs != 1 and max_pages > 1:
+        raise RuntimeError(f"{what}: page_table must be int32 [B, max_pages], row-major")
+    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or seq_lens.shape[0] != B or not seq_lens.is_contiguous():
         raise RuntimeError(f"{what}: seq_lens must be int32 [B], contiguous")
     if out is None:
-        out = torch.empty(B, Hq, D, dtype=torch.float16, device=q.device)
+        out = q.new_empty((B, Hq, D))
     elif out.dtype != torch.float16 or out.shape != (B, Hq, D) or not out.is_contiguous():
         raise RuntimeError(f"{what}: out must be fp16 [B, Hq, D], contiguous")
     if B == 0:
         return out
-    max_pages = page_table.shape[1]
     if max_pages == 0:
         return out.zero_()
-    if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+    sb, sh, _ = q.stride()
+    if sb % 8 or sh % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
-    if num_splits is None:
-        num_splits = choose_q8_splits(B, pool.num_kv_heads, max_pages, P)
-    part_o = part_ml = None
-    if num_splits > 1:
-        ws = workspace if workspace is not None else AttnWorkspace(q.device)
-        part_o, part_ml = ws.get(B, Hq, D, num_splits)
-    pts = page_table.stride(0) if B > 1 else max_pages
-    _native.call_on(q.device, "helm_paged_decode_attn_q8", q.data_ptr(), q.stride(0), q.stride(1), pool.c_ref(),
-                    page_table.data_ptr(), pts, seq_lens.data_ptr(), _native.ptr(part_o), _native.ptr(part_ml),
-                    out.data_ptr(), B, Hq, pool.num_kv_heads, D, P, max_pages, num_splits, float(scale),
-                    _native.stream_ptr(q.device))
+        sb, sh, _ = q.stride()
+    need = q8_workspace_bytes(B, Hq, pool.num_kv_heads, D, P, max_pages, num_splits)
+    ws = None
+    if need:
+        if workspace is None:
+            workspace = AttnWorkspace(q.device)
+        ws = workspace.reserve(index, need)
+    _native.call_on(index, "helm_paged_decode_attn_q8", q.data_ptr(), sb, sh, pool.c_ref(), page_table.data_ptr(),
+                    pts if B > 1 else max_pages, seq_lens.data_ptr(), out.data_ptr(), B, Hq, pool.num_kv_heads, D, P,
+                    max_pages, D ** -0.5 if scale is None else scale, num_splits, ws, need, _native.raw_stream(index))
     return out
 
 
 def _check_places(what: str, slots: torch.Tensor, offsets: torch.Tensor, n: int) -> None:
     for name, t in (("slots", slots), ("offsets", offsets)):
-        if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
             raise RuntimeError(f"{what}: {name} must be int32 [{n}], contiguous")
 
 
@@ -517,8 +521,7 @@ def kv_append_q8(k_new: torch.Tensor, v_new: torch.Tensor, pool: Q8PoolView, slo
     nearest even.  Tokens whose slot is outside the pool or whose offset is outside the page
     are skipped; of two tokens for one place, one is kept (which one is not defined)."""
     what = "kv_append_q8"
-    _native.require_cuda(k_new, v_new, pool.k, slots, offsets, what=what)
-    _native.require_same_device(what, k_new, v_new, pool.k, slots, offsets)
+    index = _native.gpu_of(what, k_new, v_new, pool.k, slots, offsets)
     P = pool._check_page_size(page_size, what)
     if k_new.dtype != torch.float16 or v_new.dtype != torch.float16 or k_new.dim() != 4 or k_new.shape != v_new.shape:
         raise RuntimeError(f"{what}: k_new and v_new must be fp16 [B, Hkv, n_tok, D]")
@@ -530,8 +533,8 @@ def kv_append_q8(k_new: torch.Tensor, v_new: torch.Tensor, pool: Q8PoolView, slo
         return
     k_new = k_new.contiguous()
     v_new = v_new.contiguous()
-    _native.call_on(k_new.device, "helm_kv_append_q8", k_new.data_ptr(), v_new.data_ptr(), pool.c_ref(),
-                    slots.data_ptr(), offsets.data_ptr(), B, Hkv, n_tok, D, P, _native.stream_ptr(k_new.device))
+    _native.call_on(index, "helm_kv_append_q8", k_new.data_ptr(), v_new.data_ptr(), pool.c_ref(), slots.data_ptr(),
+                    offsets.data_ptr(), B, Hkv, n_tok, D, P, _native.raw_stream(index))
 
 
 def dequantize_pages(pool: Q8PoolView, pages: torch.Tensor) -> PoolView:
@@ -540,19 +543,18 @@ def dequantize_pages(pool: Q8PoolView, pages: torch.Tensor) -> PoolView:
     `prefill_attention` over it (page table arange(n)) attends a prompt that continues
     8-bit pages."""
     what = "dequantize_pages"
-    _native.require_cuda(pool.k, pages, what=what)
-    _native.require_same_device(what, pool.k, pages)
+    index = _native.gpu_of(what, pool.k, pages)
     if pages.dtype != torch.int32 or pages.dim() != 1 or not pages.is_contiguous():
         raise RuntimeError(f"{what}: pages must be a contiguous int32 vector")
-    n = pages.numel()
-    shape = (n, pool.num_kv_heads, pool.page_size, pool.head_dim)
-    k = torch.empty(shape, dtype=torch.float16, device=pages.device)
-    v = alloc_v(shape, device=pages.device)
+    n = pages.shape[0]
+    Hkv, P, D = pool.num_kv_heads, pool.page_size, pool.head_dim
+    k = pool.k_scale.new_empty((n, Hkv, P, D))
+    v = pool.v_scale.new_empty((n, Hkv, D, P)).transpose(2, 3)
     if n:
-        _native.call_on(pages.device, "helm_dequantize_pages", pool.c_ref(), pages.data_ptr(), n, k.data_ptr(),
-                        v.data_ptr(), pool.num_kv_heads, pool.head_dim, pool.page_size,
-                        _native.stream_ptr(pages.device))
-    return PoolView.of_pool(k, v)
+        _native.call_on(index, "helm_dequantize_pages", pool.c_ref(), pages.data_ptr(), n, k.data_ptr(), v.data_ptr(),
+                        Hkv, D, P, _native.raw_stream(index))
+    page = Hkv * P * D
+    return PoolView(k, v, page, P * D, page, P * D, P, n, Hkv)
 
 
 def stage_pages_h2d(host_pool: torch.Tensor, dev_staging: torch.Tensor, host_slots,

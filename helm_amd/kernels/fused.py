@@ -14,6 +14,7 @@ import torch
 
 from .. import _native
 from . import gemv_split_bytes
+from .attention import _check_places
 
 
 def _check_fp16(*ts):
@@ -150,37 +151,39 @@ def qk_norm_rope_append_q8(qkv: torch.Tensor, q_norm_w: Optional[torch.Tensor],
     in 64 bits; the rotated q rounded to fp16 once into q_out [B, Hq, D], k and v quantised
     into (slots[b], offsets[b]) with a scale per token and head, as kv_append_q8 does."""
     what = "qk_norm_rope_append_q8"
-    _native.require_cuda(qkv, q_norm_w, k_norm_w, positions, inv_freq, q_out, pool.k, slots, offsets, what=what)
-    _native.require_same_device(what, qkv, q_norm_w, k_norm_w, positions, inv_freq, q_out, pool.k, slots, offsets)
+    index = _native.gpu_of(what, qkv, q_norm_w, k_norm_w, positions, inv_freq, q_out, pool.k, slots, offsets)
     _check_fp16(qkv, q_norm_w, k_norm_w, q_out)
     Hq, Hkv, D = num_q_heads, num_kv_heads, head_dim
     if qkv.dim() != 2 or qkv.shape[1] != (Hq + 2 * Hkv) * D or qkv.stride(1) != 1:
         raise RuntimeError(f"{what}: qkv must be [B, (Hq + 2 Hkv) * D] with unit stride")
-    if (Hkv, D) != (pool.num_kv_heads, pool.head_dim):
+    if Hkv != pool.num_kv_heads or D != pool.head_dim:
         raise RuntimeError(f"{what}: {Hkv} heads of {D} do not fit the pool's {pool.num_kv_heads} of {pool.head_dim}")
     P = pool._check_page_size(page_size, what)
-    B = qkv.shape[0]
-    for name, t, n, dtype in (("positions", positions, B, torch.int32), ("slots", slots, B, torch.int32),
-                              ("offsets", offsets, B, torch.int32), ("inv_freq", inv_freq, D // 2, torch.float32)):
-        if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
-            raise RuntimeError(f"{what}: {name} must be {dtype} [{n}], contiguous")
+    B, width = qkv.shape
+    if (positions.dtype != torch.int32 or positions.dim() != 1 or positions.shape[0] != B
+            or not positions.is_contiguous()):
+        raise RuntimeError(f"{what}: positions must be int32 [{B}], contiguous")
+    _check_places(what, slots, offsets, B)
+    if (inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or inv_freq.shape[0] != D // 2
+            or not inv_freq.is_contiguous()):
+        raise RuntimeError(f"{what}: inv_freq must be fp32 [{D // 2}], contiguous")
     if (q_norm_w is None) != (k_norm_w is None):
         raise RuntimeError(f"{what}: give both q / k norm weights or neither")
     for w in (q_norm_w, k_norm_w):
-        if w is not None and (w.shape != (D,) or not w.is_contiguous()):
+        if w is not None and (w.dim() != 1 or w.shape[0] != D or not w.is_contiguous()):
             raise RuntimeError(f"{what}: norm weights must be [D], contiguous")
     if q_out is None:
-        q_out = torch.empty(B, Hq, D, dtype=torch.float16, device=qkv.device)
+        q_out = qkv.new_empty((B, Hq, D))
     elif q_out.shape != (B, Hq, D) or not q_out.is_contiguous():
         raise RuntimeError(f"{what}: q_out must be [B, Hq, D], contiguous")
     if B == 0:
         return q_out
-    if B > 1 and (qkv.stride(0) % 8 or qkv.stride(0) < qkv.shape[1]) or qkv.data_ptr() % 16:
-        qkv = qkv.clone(memory_format=torch.contiguous_format)
-    _native.call_on(qkv.device, "helm_qk_norm_rope_append_q8", qkv.data_ptr(),
-                    qkv.stride(0) if B > 1 else qkv.shape[1], _native.ptr(q_norm_w), _native.ptr(k_norm_w),
-                    float(eps), positions.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(), pool.c_ref(),
-                    slots.data_ptr(), offsets.data_ptr(), B, Hq, Hkv, D, P, _native.stream_ptr(qkv.device))
+    stride = qkv.stride(0) if B > 1 else width
+    if stride % 8 or stride < width or qkv.data_ptr() % 16:
+        qkv, stride = qkv.clone(memory_format=torch.contiguous_format), width
+    _native.call_on(index, "helm_qk_norm_rope_append_q8", qkv.data_ptr(), stride, _native.ptr(q_norm_w),
+                    _native.ptr(k_norm_w), eps, positions.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(),
+                    pool.c_ref(), slots.data_ptr(), offsets.data_ptr(), B, Hq, Hkv, D, P, _native.raw_stream(index))
     return q_out
 
 
@@ -267,17 +270,15 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
     setting is a number, or a tensor with one per row (fp32, top_k int32).  NaN logits are
     never drawn; a row with no logit above -inf gives 0.  `workspace` from
     sample_workspace, allocated here when not given."""
-    what = "sample"
     tensors = [x for x in (temperature, top_k, top_p, min_p) if torch.is_tensor(x)]
-    _native.require_cuda(logits, u, out, workspace, *tensors, what=what)
-    _native.require_same_device(what, logits, u, out, workspace, *tensors)
+    index = _native.gpu_of("sample", logits, u, out, workspace, *tensors)
     _check_fp16(logits)
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise RuntimeError("sample: logits must be [..., N] with N >= 1")
     N = logits.shape[-1]
-    x2 = logits.reshape(-1, N)
+    x2 = logits if logits.dim() == 2 else logits.reshape(-1, N)
     M = x2.shape[0]
-    if x2.stride(-1) != 1 and N > 1 or M > 1 and x2.stride(0) < N:
+    if x2.stride(1) != 1 and N > 1 or M > 1 and x2.stride(0) < N:
         x2 = x2.contiguous()
 
     def rows(x, dtype, name):
@@ -295,7 +296,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
     if not (t >= 0.0 and k >= 0 and p >= 0.0 and lo >= 0.0):
         raise RuntimeError("sample: temperature, top_k, top_p and min_p must not be negative")
     if out is None:
-        out = torch.empty(logits.shape[:-1], dtype=torch.int64, device=logits.device)
+        out = logits.new_empty(logits.shape[:-1], dtype=torch.int64)
     elif out.dtype != torch.int64 or out.numel() != M or not out.is_contiguous():
         raise RuntimeError("sample: out must be int64 with one token per row, contiguous")
     if M == 0:
@@ -304,7 +305,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
         workspace = sample_workspace(M, N, logits.device)
     elif not workspace.is_contiguous():
         raise RuntimeError("sample: workspace must be contiguous")
-    _native.call_on(logits.device, "helm_sample", x2.data_ptr(), x2.stride(0) if M > 1 else N, M, N, up, tp, kp, pp,
-                    lp, float(t), min(int(k), 2**31 - 1), float(p), float(lo), out.data_ptr(), workspace.data_ptr(),
-                    workspace.numel() * workspace.element_size(), _native.stream_ptr(logits.device))
+    _native.call_on(index, "helm_sample", x2.data_ptr(), x2.stride(0) if M > 1 else N, M, N, up, tp, kp, pp, lp, t,
+                    min(int(k), 2**31 - 1), p, lo, out.data_ptr(), workspace.data_ptr(), workspace.nbytes,
+                    _native.raw_stream(index))
     return out

@@ -430,15 +430,18 @@ int helm_dequantize_pages(const helm_kv_pool_q8* pool, const int32_t* pages, int
 
 /* helm_paged_decode_attn and helm_paged_attn_reduce over 8-bit pages: out [B, Hq, D] fp16
  * contiguous = softmax(scale * q . K^T) V; zeros for an item of 0 tokens.  num_splits
- * splits, which take the table's 64-token steps round robin (at most
- * helm_paged_attn_max_split_pages() entries each); more than one needs part_o [B, Hq,
- * num_splits, D] and part_ml [B, Hq, num_splits, 2] (fp32), one writes out by itself.
- * Replaces perform_streaming_attention (helm/runtime/kv_cache.py:318-442). */
+ * splits take an item's 64-token steps round robin (0: as many as suit the shape; more than
+ * asked for where one would cover over helm_paged_attn_max_split_pages() table entries).
+ * workspace (16-byte aligned, contents on entry do not matter) of
+ * helm_paged_attn_q8_workspace_bytes for the same num_splits; 0: may be NULL.  Replaces
+ * perform_streaming_attention (helm/runtime/kv_cache.py:318-442). */
+int64_t helm_paged_attn_q8_workspace_bytes(int B, int Hq, int Hkv, int D, int P, int max_pages,
+                                           int num_splits);
 int helm_paged_decode_attn_q8(const void* q, int64_t q_stride_b, int64_t q_stride_h,
                               const helm_kv_pool_q8* pool, const int32_t* page_table,
-                              int64_t pt_stride, const int32_t* seq_lens, float* part_o,
-                              float* part_ml, void* out, int B, int Hq, int Hkv, int D, int P,
-                              int max_pages, int num_splits, float scale, void* stream);
+                              int64_t pt_stride, const int32_t* seq_lens, void* out, int B,
+                              int Hq, int Hkv, int D, int P, int max_pages, float scale,
+                              int num_splits, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Decode-step glue (widening around the path; no single reference counterpart) */

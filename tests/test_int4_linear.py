@@ -166,7 +166,7 @@ def test_strides_shapes_and_out(cuda, m):
     with pytest.raises(RuntimeError, match="fp16"):
         hk.int4_linear(x.float(), w)
     with pytest.raises(RuntimeError, match="laid out"):
-        hk.int4_linear(x, hk.Int4Weight(w.qweight, w.scale, 90, 256, 64))
+        hk.Int4Weight(w.qweight, w.scale, 90, 256, 64)
 
 
 @pytest.mark.gpu

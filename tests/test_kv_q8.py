@@ -82,15 +82,18 @@ def test_c_entry_refusals():
     def pool(k=16, ss=H * P * D, sss=H * P, n=4):
         return ctypes.byref(ka.KvPoolQ8Struct(k, 16, 16, 16, ss, sss, n))
 
-    def attn(pool=pool(), d=D, p=P, hq=32, hkv=H, pages=4, splits=1, po=None, pts=4, qs=128):
-        return lib.helm_paged_decode_attn_q8(fake, qs, qs, pool, fake, pts, fake, po, po, fake, 1, hq, hkv, d, p, pages,
-                                             splits, 0.1, None)
-    assert attn(pool=None) == -1 and attn(pool=pool(k=0)) == -1 and attn(pool=pool(n=0)) == -1
+    def attn(pool=pool(), d=D, p=P, hq=32, hkv=H, pages=4, splits=0, ws=None, nbytes=0, pts=4, qs=128, b=1, out=fake):
+        return lib.helm_paged_decode_attn_q8(fake, qs, qs, pool, fake, pts, fake, out, b, hq, hkv, d, p, pages, 0.1,
+                                             splits, ws, nbytes, None)
+    assert attn(pool=None) == -1 and attn(pool=pool(k=0)) == -1 and attn(pool=pool(n=0)) == -1 and attn(out=None) == -1
     assert attn(pool=pool(k=8)) == -2 and attn(pool=pool(ss=H * P * D - 16)) == -1
     assert attn(pool=pool(ss=H * P * D + 8)) == -2 and attn(pool=pool(sss=H * P + 4)) == -2
     assert attn(d=96) == -2 and attn(p=8) == -2 and attn(hq=31) == -1 and attn(hq=8 * 17) == -2
-    assert attn(splits=2) == -1 and attn(pts=3) == -1 and attn(qs=4) == -2
-    assert attn(pages=5000, pts=5000) == -2 and b"pages per split" in lib.helm_last_error()
+    assert attn(splits=-1) == -1 and attn(pts=3) == -1 and attn(qs=4) == -2 and attn(b=0) == -1
+    assert attn(pages=64, pts=64) == -1 and b"workspace" in lib.helm_last_error()
+    need = lib.helm_paged_attn_q8_workspace_bytes(1, 32, H, D, P, 64, 0)
+    assert need > 0 and attn(pages=64, pts=64, ws=ctypes.c_void_p(8), nbytes=need) == -1
+    assert attn(pages=64, pts=64, ws=fake, nbytes=need - 1) == -1
     assert lib.helm_kv_append_q8(fake, None, pool(), fake, fake, 1, H, 1, D, P, None) == -1
     assert lib.helm_kv_append_q8(fake, fake, pool(), fake, fake, 1, H, 17, D, P, None) == -1
     assert lib.helm_dequantize_pages(pool(), None, 1, fake, fake, H, D, P, None) == -1
@@ -105,9 +108,9 @@ def test_c_entry_refusals():
 @pytest.mark.parametrize("pages,p", [(1, 16), (44, 32), (1024, 16), (100000, 16), (60000, 64)])
 def test_splits_fit_their_staged_pages(pages, p):
     for b in (1, 4, 16, 100):
-        n = ka.choose_q8_splits(b, 8, pages, p)
-        steps = -(-pages * p // 64)
-        assert n >= 1 and -(-steps // n) * (64 // p) <= ka.MAX_SPLIT_PAGES
+        for want in (0, 1, 7):
+            n = ka.q8_workspace_bytes(b, 16, 8, 64, p, pages, want) // (b * 16 * 66 * 4) or 1
+            assert n >= want and -(-(-(-pages * p // 64)) // n) * (64 // p) <= ka.MAX_SPLIT_PAGES
 
 
 # ── writes and the way back ──────────────────────────────────────────────────
@@ -275,7 +278,7 @@ def check_attention(o, q, pool, table, lens, scale):
 @pytest.mark.gpu
 @pytest.mark.parametrize("hq,hkv,p,d", [(32, 8, 16, 128), (5, 5, 32, 64), (16, 1, 64, 128), (40, 8, 16, 64), (12, 2, 32, 128),
                                         (8, 8, 64, 64)])
-@pytest.mark.parametrize("splits", [None, 1, 3])
+@pytest.mark.parametrize("splits", [0, 1, 3, 40])
 def test_attention_against_fp64(cuda, hq, hkv, p, d, splits):
     lens = torch.tensor([0, 1, 63, 64, 65, 200, 777], dtype=torch.int32)
     cols = -(-777 // p)
@@ -325,16 +328,58 @@ def test_attention_lengths_past_the_table_end_with_it(cuda):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("splits", [1, 4])
-def test_a_nan_in_a_live_token_reaches_its_item_alone(cuda, splits):
-    pool = random_pool(32, 2, 16, 128, 2)
-    table = torch.arange(32, dtype=torch.int32, device=cuda).view(2, 16)
-    lens = torch.tensor([256, 256], dtype=torch.int32, device=cuda)
+@pytest.mark.parametrize("splits,n", [(1, 256), (8, 2000)])
+def test_a_nan_in_a_live_token_reaches_its_item_alone(cuda, splits, n):
+    pool = random_pool(2 * n // 16, 2, 16, 128, 2)
+    table = torch.arange(2 * n // 16, dtype=torch.int32, device=cuda).view(2, -1)
+    lens = torch.tensor([n, n], dtype=torch.int32, device=cuda)
     q = torch.randn(2, 4, 128, generator=torch.Generator().manual_seed(1)).half().cuda()
     clean = ka.paged_decode_attention_q8(q, pool, table, lens, num_splits=splits)
-    pool.k_scale[3, 1, 5] = float("nan")
+    for t in (pool.k_scale, pool.v_scale):
+        old = t[3, 1, 5].clone()
+        t[3, 1, 5] = float("nan")
+        o = ka.paged_decode_attention_q8(q, pool, table, lens, num_splits=splits)
+        assert o[0, 2:].isnan().all() and torch.equal(o[0, :2], clean[0, :2]) and torch.equal(o[1], clean[1])
+        t[3, 1, 5] = old
+    q[1, 0, 7] = float("inf")                            # and one in q its head alone
     o = ka.paged_decode_attention_q8(q, pool, table, lens, num_splits=splits)
-    assert o[0, 2:].isnan().all() and torch.equal(o[0, :2], clean[0, :2]) and torch.equal(o[1], clean[1])
+    assert o[1, 0].isnan().all() and torch.equal(o[1, 1:], clean[1, 1:]) and torch.equal(o[0], clean[0])
+
+
+@pytest.mark.gpu
+def test_attention_of_many_items_follows_their_lengths(cuda):
+    """150 items (three waves of lengths), most of them empty or short, one long; the same bits
+    whatever the other items hold."""
+    b, hq, hkv, p, d = 150, 4, 2, 16, 64
+    lens = torch.zeros(b, dtype=torch.int32)
+    lens[::7], lens[77], lens[149] = 33, 3000, 129
+    cols = -(-3000 // p)
+    pool = random_pool(400, hkv, p, d, 3)
+    table = torch.randint(0, 400, (b, cols), generator=torch.Generator().manual_seed(2), dtype=torch.int32)
+    q = torch.randn(b, hq, d, generator=torch.Generator().manual_seed(1)).half()
+    o = ka.paged_decode_attention_q8(q.cuda(), pool, table.cuda(), lens.cuda(), p)
+    some = torch.tensor([0, 1, 7, 70, 76, 77, 78, 147, 149])
+    check_attention(o[some.cuda()], q[some], pool, table[some], lens[some], d ** -0.5)
+    assert not o[lens.cuda() == 0].any()
+
+
+@pytest.mark.gpu
+def test_captured_attention_follows_new_lengths(cuda):
+    b, hq, hkv, p, d = 3, 8, 2, 16, 128
+    pool = random_pool(3 * 128, hkv, p, d, 3)
+    table = torch.arange(3 * 128, dtype=torch.int32, device=cuda).view(3, 128)
+    q = torch.randn(b, hq, d, generator=torch.Generator().manual_seed(1)).half().cuda()
+    lens = torch.tensor([5, 2000, 900], dtype=torch.int32, device=cuda)
+    ws = ka.AttnWorkspace(cuda)
+    ka.paged_decode_attention_q8(q, pool, table, lens, workspace=ws)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = ka.paged_decode_attention_q8(q, pool, table, lens, workspace=ws)
+    for n in ([2048, 1, 0], [64, 64, 65], [0, 0, 0], [700, 2048, 2048]):
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, ka.paged_decode_attention_q8(q, pool, table, lens))
 
 
 @pytest.mark.gpu
