@@ -78,7 +78,7 @@ _OTHER = {
     "helm_paged_attn_workspace_floats": ([_i32, _i32, _i32, _i32], _i64),
     "helm_paged_attn_max_split_pages": ([], _i32),
     "helm_paged_attn_noalloc_max_floats": ([], _i64),
-    "helm_int4_linear_workspace_bytes": ([_i32, _i32, _i32], _i64),
+    "helm_int4_linear_workspace_bytes": ([_i32, _i32, _i32, _i32], _i64),
     "helm_paged_attn_q8_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32], _i64),
     "helm_sample_workspace_bytes": ([_i32, _i32], _i64),
     "helm_argmax_workspace_bytes": ([_i32], _i64),

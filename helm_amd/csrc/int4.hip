@@ -9,8 +9,7 @@
 // holding inputs 128 kt + 32 t + 8 (l / 16) + 0..7.  So one coalesced 16-byte load
 // per lane is the operand of four MFMAs and nothing is shuffled.  A word keeps the
 // even inputs' codes (plus 8) in its low half and the odd ones' in its high half,
-// input 2p / 2p + 1 at bit 4p of either: one shift, mask and or give two fp16
-// numbers 16 + u (u = c + 8 in the top mantissa bits of [16, 32)), exactly.
+// input 2p / 2p + 1 at bit 4p of either, so two codes at a time become fp16 numbers.
 // Scales follow the tiles: [NT][KT][128 / group][16] fp16.  N is padded to 16
 // outputs and K to 128 inputs with codes of 0 and scales of 0.
 #include <algorithm>
@@ -26,30 +25,92 @@ typedef __attribute__((address_space(3))) void lds_void_t;
 
 constexpr int kTileWords = 256;       // 32-bit words of a 16 x 128 tile
 
-// Pair p of a word as two fp16 numbers 16 + u (exact).
-template <int PAIR>
-__device__ __forceinline__ uint32_t pair16(uint32_t w) {
-  constexpr int sh = 6 - 4 * PAIR;
-  const uint32_t v = sh >= 0 ? w << (sh >= 0 ? sh : 0) : w >> (sh < 0 ? -sh : 0);
-  return (v & 0x03C003C0u) | 0x4C004C00u;
+// The eight codes of a word as fp16 numbers b + u, exact: u in mantissa bits 2-5 of [256,
+// 512) for inputs 0, 1, 4, 5, in bits 6-9 of [16, 32) for inputs 2, 3, 6, 7; two shifts and four
+// and-ors.  The masks and exponents live in registers (as literals they take an and and an
+// or, eight bytes each).
+struct Unpack {
+  uint32_t m0 = 0x003C003Cu, m1 = 0x03C003C0u, o0 = 0x5C005C00u, o1 = 0x4C004C00u;
+  __device__ __forceinline__ Unpack() {
+    asm("" : "+s"(m0), "+s"(m1), "+v"(o0), "+v"(o1));
+  }
+  __device__ __forceinline__ u32x4_t operator()(uint32_t w) const {
+    const uint32_t l = w << 2, r = w >> 6;
+    return u32x4_t{(l & m0) | o0, (l & m1) | o1, (r & m0) | o0, (r & m1) | o1};
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+  asm volatile("" ::: "memory");
 }
-__device__ __forceinline__ h8_t word16(uint32_t w) {
-  const u32x4_t r = {pair16<0>(w), pair16<1>(w), pair16<2>(w), pair16<3>(w)};
-  return __builtin_bit_cast(h8_t, r);
+__device__ __forceinline__ void wait_vm_n(int n) {      // n: a constant once inlined
+  asm volatile("" ::: "memory");
+  switch (n) {
+    case 5: __builtin_amdgcn_s_waitcnt(5 | (7 << 4) | (15 << 8)); break;
+    case 6: __builtin_amdgcn_s_waitcnt(6 | (7 << 4) | (15 << 8)); break;
+    case 7: __builtin_amdgcn_s_waitcnt(7 | (7 << 4) | (15 << 8)); break;
+    case 8: __builtin_amdgcn_s_waitcnt(8 | (7 << 4) | (15 << 8)); break;
+    case 10: __builtin_amdgcn_s_waitcnt(10 | (7 << 4) | (15 << 8)); break;
+    default: __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8)); break;
+  }
+  asm volatile("" ::: "memory");
+}
+// One wave's global -> LDS copies: lane l moves 16 (4) bytes to LDS byte lds + 16 (4) l.  In
+// assembly so that the compiler does not count them: it would wait for every copy in
+// flight before each LDS read.  The kernels wait for them by number (wait_vm).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // m0 is named as clobbered on purpose
+__device__ __forceinline__ void copy_to_lds(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src)
+               : "memory", "m0");
+}
+// the same from a scalar base
+__device__ __forceinline__ void copy_to_lds(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void copy4_to_lds(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// a pointer that is the same in every lane, as a scalar
+__device__ __forceinline__ const void* uniform(const void* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+  return reinterpret_cast<const void*>((uint64_t)hi << 32 | lo);
 }
 
 // ---------------------------------------------------------------------------
 // 1 to 16 tokens
 // ---------------------------------------------------------------------------
-// Bound by the weight stream.  x^T operands of a wave's inputs stay in registers;
-// a workgroup's eight waves split the inputs of a k slice (UW tiles each) and walk
-// row tiles tb, tb + nb, ..., the next row tile's weights requested before this
-// one's products.  The products run on 16 + u; the -24 sum(x) that turns them into
-// codes is the same for every output, so it is computed once per wave and group (an
-// MFMA with a constant operand) and starts each accumulation.  It costs no accuracy:
-// the sums are fp32 and 24 is 3 times the largest code.  A group's sum is scaled by
-// its outputs' scales in fp32.
-constexpr int kW = 8;
+// Bound by the weight stream, and by the instructions that unpack it: x^T operands of a
+// wave's inputs stay in registers; a workgroup's 16 waves (four a SIMD: a wave alone takes 950
+// cycles a tile, mostly latencies) split the inputs of a k slice (UW tiles each) and walk
+// row tiles tb, tb + nb, ....  Weights go global -> LDS through a private ring of kDepth
+// tiles per wave, and the scales of a row tile's share through another, waited for by count:
+// 96 KB on the way per CU, and no register holds any (two or three row tiles in registers
+// instead spilled, or kept less on the way: 4.2 TB/s).  A tile is read back as it lies, a
+// 16-byte operand word group per lane.
+// The products run on b + u; the -sum((b + 8) x) that turns them into codes is the same for
+// every output, so it is computed once per wave and group (an MFMA with a constant operand)
+// and starts each accumulation: fp32 sums of numbers up to 264 |x| (2^-24 of them: 2^-13 of a
+// code's unit).  A group's sum is scaled by its outputs' scales in fp32.  The waves' partial
+// tiles meet in LDS, one barrier per row tile, and take turns at the epilogue.
+constexpr int kW = 16;
+constexpr int kDepth = 6;             // tiles of a wave on the way
+constexpr int kScSlots = 7;           // row tiles whose scales are (256 bytes each)
 constexpr int kMaxTiles = 64;         // row tiles a workgroup may walk (staged biases)
 
 struct Int4Args {
@@ -66,12 +127,16 @@ struct Int4Args {
   int S;                              // k slices
 };
 
-// UW: tiles of a wave's k share.  GU: groups per tile.
+// UW: tiles of a wave's k share.  GU: groups per tile (UW * GU <= 8: a row tile's scales are
+// one copy).
 template <int UW, int GU, bool PART>
 __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t s_w[kW][kDepth * 1024];
+  __shared__ __attribute__((aligned(16))) uint8_t s_s[kW][kScSlots * 256];
   __shared__ __attribute__((aligned(16))) f4_t s_c[2][kW][64];
-  __shared__ float s_bias[PART ? 1 : kMaxTiles * 16];
+  __shared__ uint16_t s_bias[PART ? 2 : kMaxTiles * 16];
   constexpr int TG = 4 / GU;          // MFMAs per group
+  static_assert(UW * GU <= 8 && (kDepth + UW - 1) / UW + 1 <= kScSlots, "scale ring");
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -83,52 +148,70 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
   const int sl = PART ? (int)blockIdx.x % a.S : 0;
   const int tb = PART ? (int)blockIdx.x / a.S : (int)blockIdx.x;
   const int nb = PART ? (int)gridDim.x / a.S : (int)gridDim.x;
-  const int T = tb < a.NT ? (a.NT - 1 - tb) / nb + 1 : 0;
+  const int T = __builtin_amdgcn_readfirstlane((a.NT - 1 - tb) / nb + 1);   // nb <= NT: at least one
   const int sa = (int)((int64_t)sl * a.KT / a.S), sn = (int)((int64_t)(sl + 1) * a.KT / a.S) - sa;
-  const int u0 = sa + wave * sn / kW, u1 = sa + (wave + 1) * sn / kW;   // at most UW tiles
+  const int u0 = __builtin_amdgcn_readfirstlane(sa + wave * sn / kW);      // [u0, u1): at most UW tiles
+  const int u1 = __builtin_amdgcn_readfirstlane(sa + (wave + 1) * sn / kW);
+  const int own = u1 - u0;
 
-  struct Buf {
-    uint4 w[UW];
-    uint2 s[UW][GU];
-  };
-  // Row tile tb + t nb (clamped to the last one) of this wave's k share; tiles past the
-  // share re-read its last one (their x operands are zero).
-  auto load = [&](Buf& b, int t) {
-    const int64_t row = (int64_t)min(tb + t * nb, a.NT - 1) * a.KT;
-#pragma unroll
-    for (int u = 0; u < UW; ++u) {
-      const int64_t tile = row + min(min(u0 + u, max(u1 - 1, u0)), a.KT - 1);
-      b.w[u] = ld_nt16(a.w + tile * kTileWords + lane * 4);
-#pragma unroll
-      for (int g = 0; g < GU; ++g)
-        b.s[u][g] = *reinterpret_cast<const uint2*>(a.scale + (tile * GU + g) * 16 + grp * 4);
+  // Tile u of the wave's share in row tile t, with the row tile's scales ahead of tile 0.  Past
+  // the share all lanes copy the same 16 bytes, so that the copies can be counted.  Addresses
+  // are scalar: the vector ALU has the unpacking to do.
+  const uint32_t lds_w = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t*)&s_w[wave][0]);
+  const uint32_t lds_s = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t*)&s_s[wave][0]);
+  const uint32_t soff = (uint32_t)min(lane * 4, max(own, 1) * GU * 32 - 4), woff = (uint32_t)lane * 16;
+  const int64_t first = (int64_t)tb * a.KT + min(u0, a.KT - 1), stride = (int64_t)nb * a.KT;
+  const uint8_t* wbase = static_cast<const uint8_t*>(uniform(a.w + first * kTileWords));
+  const uint8_t* sbase = static_cast<const uint8_t*>(uniform(a.scale + first * (GU * 16)));
+  uint32_t at_w = lds_w, at_s = lds_s;          // slots of the next copies
+  auto issue = [&](int t, int u) {
+    const int64_t tile = t * stride;
+    if (u == 0) {
+      copy4_to_lds(uniform(sbase + tile * (GU * 32)), soff, at_s);
+      at_s = at_s + 256 == lds_s + kScSlots * 256 ? lds_s : at_s + 256;
     }
+    copy_to_lds(uniform(wbase + (tile + (u < own ? u : 0)) * 1024), u < own ? woff : 0u, at_w);
+    at_w = at_w + 1024 == lds_w + kDepth * 1024 ? lds_w : at_w + 1024;
   };
-  Buf b0, b1;
-  load(b0, 0);
+  // the first row tile's share goes out ahead of x (at one row tile it is all there is)
+#pragma unroll
+  for (int u = 0; u < UW; ++u) issue(0, u);
 
   h8_t xr[UW][4];
   const uint16_t* xrow = a.x + (int64_t)min(col, M - 1) * a.ldx;
 #pragma unroll
   for (int u = 0; u < UW; ++u)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int k = (u0 + u) * 128 + t * 32 + grp * 8;
-      xr[u][t] = *reinterpret_cast<const h8_t*>(xrow + min(k, a.K - 8));
-      if (u0 + u >= u1 || k >= a.K) xr[u][t] = h8_t{};
-    }
+    for (int t = 0; t < 4; ++t)
+      xr[u][t] = *reinterpret_cast<const h8_t*>(xrow + min((u0 + u) * 128 + t * 32 + grp * 8, a.K - 8));
+  // bias of the workgroup's outputs, one of each per thread
+  uint16_t bs = 0;
   if constexpr (!PART) {
-    for (int i = tid; i < T * 16; i += kW * 64) {
-      const int n = min((tb + (i >> 4) * nb) * 16 + (i & 15), a.N - 1);
-      s_bias[i] = a.bias ? h2f(a.bias[n]) : 0.f;
-    }
+    const int64_t n = min((int64_t)(tb + (int64_t)(tid >> 4) * nb) * 16 + (tid & 15), (int64_t)a.N - 1);
+    if (a.bias) bs = a.bias[n];
   }
-  // -24 * (sum of a group's x): every row of the product with a constant operand
+  // x has arrived: from here on the ring fills while the prologue computes
+#pragma unroll
+  for (int u = 0; u < UW; ++u)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(xr[u][t]));
+  if constexpr (!PART) {
+    static_assert(kMaxTiles * 16 == kW * 64, "one bias per thread");
+    s_bias[tid] = bs;
+  }
+#pragma unroll
+  for (int n = UW; n < kDepth; ++n)
+    if (n / UW < T) issue(n / UW, n % UW);
+#pragma unroll
+  for (int u = 0; u < UW; ++u)
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (u >= own || (u0 + u) * 128 + t * 32 >= a.K) xr[u][t] = h8_t{};
+  // -sum((b + 8) x) of each group: every row of the product with a constant operand
   float nbias[UW][GU];
   {
-    h8_t c;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = (_Float16)-24.0f;
+    const _Float16 p = (_Float16)-264.0f, q = (_Float16)-24.0f;
+    const h8_t c = {p, p, q, q, p, p, q, q};
 #pragma unroll
     for (int u = 0; u < UW; ++u)
 #pragma unroll
@@ -139,32 +222,59 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
         nbias[u][g] = s[0];
       }
   }
-  lds_barrier();
+  const Unpack unpack;
+  lds_barrier();                      // staged biases
 
-  auto tile = [&](const Buf& b, int t) {
+  const uint8_t* pw = &s_w[wave][0];  // slots read next
+  const uint8_t* ps = &s_s[wave][0];
+  const int total = T * UW;
+  for (int t = 0; t < T; ++t) {
     f4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < UW; ++u) {
-      const uint32_t wd[4] = {b.w[u].x, b.w[u].y, b.w[u].z, b.w[u].w};
+      // tile landed: at most the kDepth - 1 later tiles' copies are on the way, and those of
+      // the row tiles that begin among them (the stream's end, where fewer follow, waits for
+      // all)
+      constexpr auto later = [](int u_) {
+        int n = kDepth - 1;
+        for (int j = 1; j < kDepth; ++j) n += (u_ + j) % UW == 0;
+        return n;
+      };
+      if (t * UW + u + kDepth <= total) wait_vm_n(later(u));
+      else wait_vm<0>();
+      uint4 w = *reinterpret_cast<const uint4*>(pw + lane * 16);
+      uint2 sc[GU];
+#pragma unroll
+      for (int g = 0; g < GU; ++g) sc[g] = *reinterpret_cast<const uint2*>(ps + (u * GU + g) * 32 + grp * 8);
+      pw = pw + 1024 == &s_w[wave][kDepth * 1024] ? &s_w[wave][0] : pw + 1024;
+      // the slot is refilled once this wave's reads have returned
+      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w) :: "memory");
+#pragma unroll
+      for (int g = 0; g < GU; ++g) asm volatile("" : "+v"(sc[g].x), "+v"(sc[g].y));
+      if (t + (u + kDepth) / UW < T) issue(t + (u + kDepth) / UW, (u + kDepth) % UW);
+      if (u >= own) continue;         // not this wave's (uniform)
+      const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int g = 0; g < GU; ++g) {
-        const float z = nbias[u][g];
+        float z = nbias[u][g];
+        asm("" : "+v"(z));            // (or four copies of each would be kept)
         f4_t c = {z, z, z, z};
 #pragma unroll
         for (int q = 0; q < TG; ++q)
-          c = __builtin_amdgcn_mfma_f32_16x16x32_f16(word16(wd[g * TG + q]), xr[u][g * TG + q], c, 0, 0, 0);
-        acc[0] = fmaf(lo_h(b.s[u][g].x), c[0], acc[0]);
-        acc[1] = fmaf(hi_h(b.s[u][g].x), c[1], acc[1]);
-        acc[2] = fmaf(lo_h(b.s[u][g].y), c[2], acc[2]);
-        acc[3] = fmaf(hi_h(b.s[u][g].y), c[3], acc[3]);
+          c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, unpack(wd[g * TG + q])), xr[u][g * TG + q], c, 0, 0, 0);
+        acc[0] = fmaf(lo_h(sc[g].x), c[0], acc[0]);
+        acc[1] = fmaf(hi_h(sc[g].x), c[1], acc[1]);
+        acc[2] = fmaf(lo_h(sc[g].y), c[2], acc[2]);
+        acc[3] = fmaf(hi_h(sc[g].y), c[3], acc[3]);
       }
     }
+    ps = ps + 256 == &s_s[wave][kScSlots * 256] ? &s_s[wave][0] : ps + 256;
     f4_t (*sc)[64] = s_c[t & 1];
     sc[wave][lane] = acc;
     lds_barrier();      // buffer t & 1 is written again only after tile t + 1's barrier
     if (wave == (t & (kW - 1))) {
       f4_t v = sc[0][lane];
-#pragma unroll
+#pragma unroll 5
       for (int w = 1; w < kW; ++w) {
         const f4_t o = sc[w][lane];
 #pragma unroll
@@ -178,19 +288,11 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
           uint16_t* yp = a.y + (int64_t)col * a.ldy + n0;
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (n0 + r < a.N) yp[r] = f2h(v[r] + s_bias[t * 16 + grp * 4 + r]);
+            if (n0 + r < a.N) yp[r] = f2h(v[r] + h2f(s_bias[t * 16 + grp * 4 + r]));
         }
       }
     }
-  };
-  int t = 0;
-  for (; t + 1 < T; t += 2) {
-    load(b1, t + 1);
-    tile(b0, t);
-    if (t + 2 < T) load(b0, t + 2);
-    tile(b1, t + 1);
   }
-  if (t < T) tile(b0, t);
 }
 
 // Adds the S partial sums of four outputs of a token, and the bias.
@@ -212,37 +314,47 @@ __global__ __launch_bounds__(256) void int4_reduce_kernel(const float* __restric
     if (n + r < N) y[(int64_t)m * ldy + n + r] = f2h(v[r] + (bias ? h2f(bias[n + r]) : 0.f));
 }
 
-// k slices and tiles per wave of a GEMV: the fewest slices of at most kMaxUw tiles per
-// wave.
-constexpr int kMaxUw = 6;
+// k slices of a GEMV, tiles per wave (at most what x^T leaves of 128 registers), workgroups per
+// slice.  Every workgroup is on a CU from the start, so the longest one counts: row tiles x
+// tiles per wave, 0.67 us each (16 KB at 6 TB/s / 256), its x (45 KB / us from L2), the partial
+// sums' traffic (4 TB/s) and the second launch (3 us).
+constexpr int max_uw(int GU) { return GU == 1 ? 4 : GU == 2 ? 3 : 2; }
 struct GemvPlan {
-  int S, uw;
+  int S, uw, nb;
 };
-GemvPlan plan_gemv(int NT, int KT) {
-  (void)NT;
-  GemvPlan p;
-  p.S = (KT + kW * kMaxUw - 1) / (kW * kMaxUw);
-  const int sn = (KT + p.S - 1) / p.S;
-  p.uw = (sn + kW - 1) / kW;
-  return p;
+GemvPlan plan_gemv(int M, int NT, int KT, int GU) {
+  GemvPlan best{1, 1, 1};
+  double least = -1.0;
+  for (int S = (KT + kW * max_uw(GU) - 1) / (kW * max_uw(GU)); S <= std::min(KT, 256); ++S) {
+    GemvPlan p;
+    p.S = S;
+    p.uw = ((KT + S - 1) / S + kW - 1) / kW;
+    p.nb = S > 1 ? std::min(NT, 256 / S) : std::max(std::min(NT, 256), (NT + kMaxTiles - 1) / kMaxTiles);
+    const double c = 0.67 * ((NT + p.nb - 1) / p.nb) * (p.uw + 0.25) + M * KT * 256.0 / S / 45e3 + (S > 1 ? 3.0 + (double)S * M * NT * 128.0 / 4e6 : 0.0);
+    if (least < 0.0 || c < least) {
+      least = c;
+      best = p;
+    }
+    if (S > 1 && p.uw == 1) break;
+  }
+  return best;
 }
 
 template <int UW, int GU>
-void launch_gemv(const Int4Args& a, hipStream_t s) {
-  const int nb = std::max(std::min(a.NT, std::max(1, 256 / a.S)), (a.NT + kMaxTiles - 1) / kMaxTiles);
+void launch_gemv(const Int4Args& a, int nb, hipStream_t s) {
   if (a.S > 1) hipLaunchKernelGGL((int4_gemv_kernel<UW, GU, true>), dim3(nb * a.S), dim3(kW * 64), 0, s, a);
   else hipLaunchKernelGGL((int4_gemv_kernel<UW, GU, false>), dim3(nb), dim3(kW * 64), 0, s, a);
 }
 template <int GU>
-void launch_gemv_uw(int uw, const Int4Args& a, hipStream_t s) {
-  switch (uw) {
-    case 1: return launch_gemv<1, GU>(a, s);
-    case 2: return launch_gemv<2, GU>(a, s);
-    case 3: return launch_gemv<3, GU>(a, s);
-    case 4: return launch_gemv<4, GU>(a, s);
-    case 5: return launch_gemv<5, GU>(a, s);
-    default: return launch_gemv<6, GU>(a, s);
+void launch_gemv_uw(const GemvPlan& p, const Int4Args& a, hipStream_t s) {
+  if (p.uw == 1) return launch_gemv<1, GU>(a, p.nb, s);
+  if constexpr (GU <= 2) {
+    if (p.uw == 3) return launch_gemv<3, GU>(a, p.nb, s);
   }
+  if constexpr (GU == 1) {
+    if (p.uw == 4) return launch_gemv<4, GU>(a, p.nb, s);
+  }
+  launch_gemv<2, GU>(a, p.nb, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -260,37 +372,19 @@ constexpr int kGThreads = 256;
 constexpr int kStages = 3;
 __device__ __forceinline__ int aswz(int r) { return (r >> 1) & 7; }   // 128-byte rows
 
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  static_assert(N >= 0 && N < 64, "vmcnt range");
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
-  asm volatile("" ::: "memory");
-}
-// One wave's 1 KiB global -> LDS copy: lane l moves 16 bytes from `src` to LDS byte
-// lds + 16 l; waited for by the kernel itself.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"   // m0 is named as clobbered on purpose
-__device__ __forceinline__ void copy_to_lds(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src)
-               : "memory", "m0");
-}
-#pragma clang diagnostic pop
 __device__ __forceinline__ void lds_read_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// Word of eight codes times a scale, each product rounded to fp16 once (16 + u - 24 is
+// Word of eight codes times a scale, each product rounded to fp16 once (b + u - b - 8 is
 // exact).
-__device__ __forceinline__ h8_t word_scaled(uint32_t w, h2_t s) {
-  const h2_t off = {(_Float16)-24.0f, (_Float16)-24.0f};
-  const uint32_t p[4] = {pair16<0>(w), pair16<1>(w), pair16<2>(w), pair16<3>(w)};
+__device__ __forceinline__ h8_t word_scaled(const Unpack& unpack, uint32_t w, h2_t s) {
+  const h2_t off0 = {(_Float16)-264.0f, (_Float16)-264.0f}, off1 = {(_Float16)-24.0f, (_Float16)-24.0f};
+  const u32x4_t p = unpack(w);
   h8_t r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const h2_t v = (__builtin_bit_cast(h2_t, p[i]) + off) * s;
+    const h2_t v = (__builtin_bit_cast(h2_t, (uint32_t)p[i]) + (i & 1 ? off1 : off0)) * s;
     r[2 * i] = v[0];
     r[2 * i + 1] = v[1];
   }
@@ -366,6 +460,7 @@ __global__ __launch_bounds__(kGThreads, 2) void int4_gemm_kernel(Int4Args a) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
 
+  const Unpack unpack;
   auto step = [&](const BBuf& b, int kb, auto half_c) {
     constexpr int half = decltype(half_c)::value;
     if (kb + 1 < nk) wait_vm<kCopies>();
@@ -373,19 +468,19 @@ __global__ __launch_bounds__(kGThreads, 2) void int4_gemm_kernel(Int4Args a) {
     lds_read_barrier();
     if (kb + 2 < nk) copy(kb + 2);
     const uint8_t* As = smem + (kb % kStages) * kStageBytes;
-    h8_t af[RI];
-#pragma unroll
-    for (int i = 0; i < RI; ++i) {
-      const int r = 16 * i + col;
-      af[i] = *reinterpret_cast<const h8_t*>(As + r * 128 + (((4 * kh + grp) ^ aswz(r)) << 4));
-    }
+    h8_t bf[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const _Float16 s1 = __builtin_bit_cast(_Float16, b.s[j][SG == 2 ? half : 0]);
-      const h8_t bf = word_scaled(half ? b.w[j].y : b.w[j].x, h2_t{s1, s1});
+      bf[j] = word_scaled(unpack, half ? b.w[j].y : b.w[j].x, h2_t{s1, s1});
+    }
 #pragma unroll
-      for (int i = 0; i < RI; ++i)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[i], bf, acc[i][j], 0, 0, 0);
+    for (int i = 0; i < RI; ++i) {
+      const int r = 16 * i + col;
+      const h8_t af = *reinterpret_cast<const h8_t*>(As + r * 128 + (((4 * kh + grp) ^ aswz(r)) << 4));
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af, bf[j], acc[i][j], 0, 0, 0);
     }
   };
 
@@ -445,16 +540,27 @@ __global__ __launch_bounds__(kGThreads, 2) void int4_gemm_kernel(Int4Args a) {
   else finish(std::integral_constant<int, RI / 2>{});
 }
 
-// Row tiles and k slices of a prompt: tiles as tall as the rows need, k split until the
-// workgroups fill two per CU.
+// Row tiles (16 RI rows) and k slices of a prompt: rounds of the workgroup slots (three a CU at
+// RI = 4, two above) x the tile's cost (its MFMAs, and what unpacking and the step itself
+// cost whatever the height).  1500 x 4096 -> 12288: RI = 8 takes 1152 tiles, 2.25 rounds of 512, RI =
+// 6 1536, exactly 3 of three quarters the height.  Few tiles split k until the slots fill.
 struct GemmPlan {
   int ri, S;
 };
 GemmPlan plan_gemm(int M, int NT, int KT) {
-  GemmPlan p;
-  p.ri = M <= 32 ? 2 : M <= 64 ? 4 : 8;
-  const int64_t tiles = (int64_t)((NT + 7) / 8) * ((M + 16 * p.ri - 1) / (16 * p.ri));
-  p.S = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / std::max<int64_t>(tiles, 1), KT / 4), 16));
+  GemmPlan p{8, 1};
+  double least = -1.0;
+  for (int ri = 8; ri >= 2; ri -= 2) {
+    if (ri > 2 && 16 * (ri - 2) >= M) continue;        // taller than the rows need
+    const int64_t tiles = (int64_t)((NT + 7) / 8) * ((M + 16 * ri - 1) / (16 * ri));
+    const int64_t slots = ri <= 4 ? 768 : 512;
+    const int S = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(slots / std::max<int64_t>(tiles, 1), KT / 4), 16));
+    const double c = (double)((tiles * S + slots - 1) / slots) * ((KT + S - 1) / S) * (ri + 1.5) + (S > 1 ? 30.0 : 0.0);
+    if (least < 0.0 || c < 0.97 * least) {
+      least = c;
+      p = {ri, S};
+    }
+  }
   return p;
 }
 
@@ -468,17 +574,17 @@ template <int GU>
 void launch_gemm_ri(int ri, const Int4Args& a, hipStream_t s) {
   if (ri == 2) launch_gemm<2, GU>(a, s);
   else if (ri == 4) launch_gemm<4, GU>(a, s);
+  else if (ri == 6) launch_gemm<6, GU>(a, s);
   else launch_gemm<8, GU>(a, s);
 }
 
-int slices(int M, int NT, int KT) { return M <= 16 ? plan_gemv(NT, KT).S : plan_gemm(M, NT, KT).S; }
-
 }  // namespace
 
-extern "C" int64_t helm_int4_linear_workspace_bytes(int M, int N, int K) {
-  if (M < 1 || N < 1 || K < 1 || N > (1 << 30) || K > (1 << 30)) return 0;
+extern "C" int64_t helm_int4_linear_workspace_bytes(int M, int N, int K, int group_size) {
+  if (M < 1 || N < 1 || K < 1 || N > (1 << 27) || K > (1 << 19)) return 0;
+  if (group_size != 32 && group_size != 64 && group_size != 128) return 0;
   const int NT = (N + 15) / 16, KT = (K + 127) / 128;
-  const int S = slices(M, NT, KT);
+  const int S = M <= 16 ? plan_gemv(M, NT, KT, 128 / group_size).S : plan_gemm(M, NT, KT).S;
   return S > 1 ? (int64_t)S * M * NT * 16 * (int64_t)sizeof(float) : 0;
 }
 
@@ -487,7 +593,7 @@ extern "C" int helm_int4_linear(const void* x, int64_t ldx, const void* qweight,
                                 void* workspace, int64_t workspace_bytes, void* stream) {
   HELM_CHECK_ARG(x && qweight && scale && y, "helm_int4_linear: null pointer");
   HELM_CHECK_ARG(M >= 1 && N >= 1 && K >= 1, "helm_int4_linear: M, N, K must be positive");
-  HELM_CHECK_SUPPORTED(N <= (1 << 30) && K <= (1 << 30) && M <= (1 << 22), "helm_int4_linear: shape too large");
+  HELM_CHECK_SUPPORTED(N <= (1 << 27) && K <= (1 << 19) && M <= (1 << 22), "helm_int4_linear: shape too large");
   HELM_CHECK_ARG(ldx >= K && ldy >= N, "helm_int4_linear: leading dimension too small");
   HELM_CHECK_SUPPORTED(group_size == 32 || group_size == 64 || group_size == 128,
                        "helm_int4_linear: group size must be 32, 64 or 128");
@@ -502,23 +608,24 @@ extern "C" int helm_int4_linear(const void* x, int64_t ldx, const void* qweight,
   a.y = static_cast<uint16_t*>(y); a.ldy = ldy;
   a.M = M; a.N = N; a.K = K;
   a.NT = (N + 15) / 16; a.KT = (K + 127) / 128; a.np = a.NT * 16;
-  a.S = slices(M, a.NT, a.KT);
-  const int64_t need = helm_int4_linear_workspace_bytes(M, N, K);
+  const int GU = 128 / group_size;
+  const GemvPlan gp = M <= 16 ? plan_gemv(M, a.NT, a.KT, GU) : GemvPlan{};
+  const GemmPlan mp = M <= 16 ? GemmPlan{} : plan_gemm(M, a.NT, a.KT);
+  a.S = M <= 16 ? gp.S : mp.S;
+  const int64_t need = a.S > 1 ? (int64_t)a.S * M * a.np * (int64_t)sizeof(float) : 0;
   HELM_CHECK_ARG(need == 0 || (workspace && helm::aligned16(workspace) && workspace_bytes >= need),
                  "helm_int4_linear: this shape needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
   a.part = static_cast<float*>(workspace);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (M <= 16) {
-    const int uw = plan_gemv(a.NT, a.KT).uw;
-    if (group_size == 128) launch_gemv_uw<1>(uw, a, s);
-    else if (group_size == 64) launch_gemv_uw<2>(uw, a, s);
-    else launch_gemv_uw<4>(uw, a, s);
+    if (GU == 1) launch_gemv_uw<1>(gp, a, s);
+    else if (GU == 2) launch_gemv_uw<2>(gp, a, s);
+    else launch_gemv_uw<4>(gp, a, s);
   } else {
-    const int ri = plan_gemm(M, a.NT, a.KT).ri;
-    HELM_CHECK_SUPPORTED((M + 16 * ri - 1) / (16 * ri) <= 65535, "helm_int4_linear: too many rows");
-    if (group_size == 128) launch_gemm_ri<1>(ri, a, s);
-    else if (group_size == 64) launch_gemm_ri<2>(ri, a, s);
-    else launch_gemm_ri<4>(ri, a, s);
+    HELM_CHECK_SUPPORTED((M + 16 * mp.ri - 1) / (16 * mp.ri) <= 65535, "helm_int4_linear: too many rows");
+    if (GU == 1) launch_gemm_ri<1>(mp.ri, a, s);
+    else if (GU == 2) launch_gemm_ri<2>(mp.ri, a, s);
+    else launch_gemm_ri<4>(mp.ri, a, s);
   }
   HELM_CHECK_LAUNCH("helm_int4_linear launch");
   if (a.S > 1) {

@@ -360,10 +360,10 @@ class Int4Weight:
 
 
 @functools.lru_cache(maxsize=4096)
-def int4_workspace_bytes(M: int, N: int, K: int) -> int:
+def int4_workspace_bytes(M: int, N: int, K: int, group_size: int) -> int:
     """Workspace helm_int4_linear needs at this shape (0: none): fp32 partial sums of
     inputs split over workgroups."""
-    return int(_native.lib().helm_int4_linear_workspace_bytes(int(M), int(N), int(K)))
+    return int(_native.lib().helm_int4_linear_workspace_bytes(int(M), int(N), int(K), int(group_size)))
 
 
 def int4_linear(input: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Tensor] = None,
@@ -392,7 +392,7 @@ def int4_linear(input: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Te
         raise RuntimeError("int4_linear: out must be a contiguous fp16 tensor [..., N]")
     if M == 0:
         return out
-    need = int4_workspace_bytes(M, N, K)
+    need = int4_workspace_bytes(M, N, K, weight.group_size)
     ws = input.new_empty(need // 2) if need else None
     _native.call_on(index, "helm_int4_linear", x2.data_ptr(), ldx, q.data_ptr(), weight.scale.data_ptr(),
                     weight.group_size, None if bias is None else bias.data_ptr(), out.data_ptr(), N, M, N, K,

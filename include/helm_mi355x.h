@@ -151,7 +151,7 @@ int helm_int8_gemm_ws(const void* x, int64_t ldx, const int8_t* q, int64_t ldq,
  * workspace (16-byte aligned, contents on entry do not matter) of at least
  * helm_int4_linear_workspace_bytes (0: may be NULL).  Beside helm_int8_gemv_ws and
  * helm_int8_gemm_ws, the counterparts of fp16_gemv.cpp:105-157. */
-int64_t helm_int4_linear_workspace_bytes(int M, int N, int K);
+int64_t helm_int4_linear_workspace_bytes(int M, int N, int K, int group_size);
 int helm_int4_linear(const void* x, int64_t ldx, const void* qweight, const void* scale,
                      int group_size, const void* bias, void* y, int64_t ldy, int M, int N, int K,
                      void* workspace, int64_t workspace_bytes, void* stream);

@@ -2,9 +2,10 @@
 against fp64.
 
 Tolerance of one output.  The last rounding is off by at most 2^-11 |y|.  Up to 16 tokens
-a group's sum runs over (16 + u) x with 16 + u < 32 and a start of 24 sum(x), in at most 32
-fp32 additions of partial sums no larger than 40 sum|x|, each off by at most 2^-23 of
-that: 32 * 2^-23 * 40 * s sum|x|, summed over the groups.  Above 16 tokens every weight is
+a group's sum runs over (b + u) x with b + u < 272 for half of the inputs and < 32 for the
+others, and a start of sum((b + 8) x), in at most 32 fp32 additions of partial sums no larger
+than 300 sum|x|, each off by at most 2^-24 of that: 32 * 2^-24 * 300 * s sum|x|, summed over
+the groups.  Above 16 tokens every weight is
 rounded to fp16 (2^-11 |w|) and the sum has K / 8 additions of partial sums no larger than
 sum|w x|.  These are worst cases; as a whole, rounding errors are independent: the norm of
 the error is at most 2^-11 / sqrt(3) of the norm of y for the last rounding and as much for
@@ -91,7 +92,7 @@ def test_refusals():
         return lib.helm_int4_linear(x, ldx, q, fake, gs, None, fake, ldy, m, n, k, ws, ws_bytes, None)
     assert call(x=None) == -1 and call(ldx=64) == -1 and call(ldy=8) == -1 and call(m=0) == -1
     assert call(gs=48) == -2 and call(k=96) == -2 and call(ldx=132) == -2 and call(q=ctypes.c_void_p(8)) == -2
-    assert lib.helm_int4_linear_workspace_bytes(1, 4096, 17408) > 0
+    assert lib.helm_int4_linear_workspace_bytes(1, 4096, 17408, 64) > 0
     assert call(n=4096, ldy=4096, k=17408, ldx=17408) == -1
     assert b"workspace" in lib.helm_last_error()
 
@@ -115,7 +116,7 @@ def check(y, x, codes, scale, bias, gs):
     e = x64 @ w.t() + (0 if bias is None else bias.double().cpu())
     tol = 2.0 ** -11 * e.abs() + 2.0 ** -25
     if m <= 16:
-        tol += 32 * 2.0 ** -23 * 40 * (x64.abs() @ s.t())
+        tol += 32 * 2.0 ** -24 * 300 * (x64.abs() @ s.t())
     else:
         tol += (2.0 ** -11 + w.shape[1] / 8 * 2.0 ** -23) * (x64.abs() @ w.abs().t())
     err = (y.double().cpu() - e).abs()
@@ -126,7 +127,7 @@ def check(y, x, codes, scale, bias, gs):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,k,gs", SHAPES)
-@pytest.mark.parametrize("m", [1, 2, 5, 16, 17, 33, 70, 200])
+@pytest.mark.parametrize("m", [1, 2, 5, 16, 17, 33, 70, 90, 200])
 def test_against_fp64(cuda, m, n, k, gs):
     codes, scale = make(n, k, gs, 7 * m + n)
     g = torch.Generator().manual_seed(m)
