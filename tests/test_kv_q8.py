@@ -227,9 +227,9 @@ def test_norm_rope_append(cuda, n, hq, hkv, p, d, first, norm):
 
 
 @pytest.mark.gpu
-def test_append_does_not_depend_on_the_batch(cuda):
+@pytest.mark.parametrize("hq,hkv,p,d,n", [(32, 8, 16, 128, 500), (20, 5, 32, 64, 500)])
+def test_append_does_not_depend_on_the_batch(cuda, hq, hkv, p, d, n):
     """A token's bits are the same written alone, in a small batch and in a prompt."""
-    hq, hkv, p, d, n = 32, 8, 16, 128, 500
     g = torch.Generator().manual_seed(8)
     wide = torch.randn(n, (hq + 2 * hkv) * d + 8, generator=g).half().cuda()
     qkv = wide[:, :-8]
@@ -245,6 +245,39 @@ def test_append_does_not_depend_on_the_batch(cuda):
     for a, b in zip((pools[0].k, pools[0].v, pools[0].k_scale, pools[0].v_scale),
                     (pools[1].k, pools[1].v, pools[1].k_scale, pools[1].v_scale)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,p,d", [(32, 8, 16, 128), (20, 5, 32, 64)])
+@pytest.mark.parametrize("places", ["any", "runs"])
+def test_append_to_any_places(cuda, hq, hkv, p, d, places):
+    """Tokens of a prompt in any order of places, some outside the pool, some not finite."""
+    n = 509
+    g = torch.Generator().manual_seed(9)
+    qkv = torch.randn(n, (hq + 2 * hkv) * d, generator=g).half()
+    qkv[77, 5], qkv[78, hq * d + 3], qkv[79, -1], qkv[80] = float("nan"), float("inf"), float("nan"), 0
+    at = torch.randperm(40 * p, generator=g)[:n]
+    if places == "runs":                                 # starts and lengths of every kind, in pages in any order
+        at, page = [], iter(torch.randperm(40 * p // 16, generator=g).tolist())
+        for i in range(n):
+            first, length = i % 5, 1 + i % 11
+            base = next(page, None)
+            at += [] if base is None else [base * 16 + j for j in range(first, min(first + length, 16))]
+        at = torch.tensor((at + [-p] * n)[:n])
+    slots, offs = (at // p).int(), (at % p).int()
+    slots[100], slots[101], offs[102], offs[103] = -1, 40, p, -1
+    w = (1 + 0.1 * torch.randn(d, generator=g)).half().cuda()
+    pos = torch.arange(n, dtype=torch.int32, device=cuda)
+    inv = (1e6 ** (-torch.arange(0, d, 2).double() / d)).float().cuda()
+    pools = [random_pool(40, hkv, p, d, 11) for _ in range(2)]
+    qkv, slots, offs = qkv.cuda(), slots.cuda(), offs.cuda()
+    q0 = fused.qk_norm_rope_append_q8(qkv, w, w, EPS, pos, inv, None, pools[0], slots, offs, hq, hkv, d)
+    q1 = torch.cat([fused.qk_norm_rope_append_q8(qkv[i:i + 100], w, w, EPS, pos[i:i + 100], inv, None, pools[1], slots[i:i + 100],
+                                                 offs[i:i + 100], hq, hkv, d) for i in range(0, n, 100)])
+    assert torch.equal(q0.nan_to_num(77.0), q1.nan_to_num(77.0))
+    for name in ("k", "v", "k_scale", "v_scale"):
+        a, b = (getattr(x, name) for x in pools)
+        assert torch.equal(a.view(torch.int8), b.view(torch.int8))
 
 
 # ── attention ────────────────────────────────────────────────────────────────
