@@ -304,10 +304,14 @@ __global__ __launch_bounds__(256) void int4_reduce_kernel(const float* __restric
   if (i >= (int64_t)M * nq) return;
   const int m = (int)(i / nq), n = (int)(i - (int64_t)m * nq) * 4;
   f4_t v = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < S; ++s) {
-    const f4_t o = *reinterpret_cast<const f4_t*>(part + ((int64_t)s * M + m) * np + n);
+  for (int s = 0; s < S; s += 8) {      // eight loads on the way; past the last they repeat it
+    f4_t o[8];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] += o[r];
+    for (int j = 0; j < 8; ++j) o[j] = *reinterpret_cast<const f4_t*>(part + ((int64_t)min(s + j, S - 1) * M + m) * np + n);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += s + j < S ? o[j][r] : 0.f;
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r)
