@@ -64,14 +64,14 @@ __device__ __forceinline__ void wait_vm_n(int n) {      // n: a constant once in
 // flight before each LDS read.  The kernels wait for them by number (wait_vm).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"   // m0 is named as clobbered on purpose
-__device__ __forceinline__ void copy_to_lds(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+__device__ __forceinline__ void copy_to_lds(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
-               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src)
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(base)
                : "memory", "m0");
 }
-// the same from a scalar base
-__device__ __forceinline__ void copy_to_lds(const void* base, uint32_t off, uint32_t lds) {
+// the same of what is read once
+__device__ __forceinline__ void copy_nt_to_lds(const void* base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(base)
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
       copy4_to_lds(uniform(sbase + tile * (GU * 32)), soff, at_s);
       at_s = at_s + 256 == lds_s + kScSlots * 256 ? lds_s : at_s + 256;
     }
-    copy_to_lds(uniform(wbase + (tile + (u < own ? u : 0)) * 1024), u < own ? woff : 0u, at_w);
+    copy_nt_to_lds(uniform(wbase + (tile + (u < own ? u : 0)) * 1024), u < own ? woff : 0u, at_w);
     at_w = at_w + 1024 == lds_w + kDepth * 1024 ? lds_w : at_w + 1024;
   };
   // the first row tile's share goes out ahead of x (at one row tile it is all there is)
@@ -368,7 +368,10 @@ void launch_gemv_uw(const GemvPlan& p, const Int4Args& a, hipStream_t s) {
 // 64 outputs of its side over half kh of the inputs, so that every weight is turned
 // into fp16 by one wave only; the halves are added through LDS at the end.  x goes
 // global -> LDS (16-byte copies, XOR-swizzled, a ring of three 64-input steps), the
-// weights straight into registers, a tile ahead.  A weight enters the products as
+// weights straight into registers, one tile ahead (three at 32 rows).  Copies and loads share one
+// counter: a step waits for its x by the number of what was requested later, weights included
+// (waiting for those too, as they had just been requested, took 183 us instead of 160 for 1500 x
+// 4096 -> 12288, now 940 TFLOP/s; 2048 x 4096 -> 4096 reaches 985).  A weight enters the products as
 // fp16(code * scale), the number that Int4Weight.dequantize() gives rounded to fp16: one
 // rounding of 2^-12 relative at most, and it spares a scaling of every accumulator
 // per group.
@@ -396,8 +399,9 @@ __device__ __forceinline__ h8_t word_scaled(const Unpack& unpack, uint32_t w, h2
 }
 
 template <int RI, int GU, bool PART>
-__global__ __launch_bounds__(kGThreads, 2) void int4_gemm_kernel(Int4Args a) {
+__global__ __launch_bounds__(kGThreads, RI <= 4 ? 3 : 2) void int4_gemm_kernel(Int4Args a) {
   constexpr int TN = 4;
+  constexpr int NB = RI == 2 ? 4 : 2;  // tiles of weights on the way or in use
   constexpr int kStageBytes = 16 * RI * 128;
   constexpr int kCopies = kStageBytes / 1024 / 4 > 0 ? kStageBytes / 1024 / 4 : 1;   // per wave and step
   constexpr int kRing = kStages * kStageBytes;
@@ -422,39 +426,47 @@ __global__ __launch_bounds__(kGThreads, 2) void int4_gemm_kernel(Int4Args a) {
   // 0-3 and 4-7 of a row: the two waves' halves), chunk g of row r in slot g ^ aswz(r).
   // Rows past M read the last row, inputs past K the row's last chunk (weights there are
   // zero).
-  int64_t arow[kCopies];
+  uint32_t arow[kCopies];               // bytes from row m0 (ldx is below 2^23)
   int akc[kCopies];
 #pragma unroll
   for (int i = 0; i < kCopies; ++i) {
     const int c = (wave * kCopies + i) * 64 + lane;
     const int r = c >> 3;
     const int g = (c & 7) ^ aswz(r);
-    arow[i] = (int64_t)min(m0 + r, M - 1) * a.ldx;
+    arow[i] = (uint32_t)min(r, M - 1 - m0) * (uint32_t)(a.ldx * 2);
     akc[i] = (g >> 2) * 64 + (g & 3) * 8;
   }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)smem;
+  const void* xbase = uniform(a.x + (int64_t)m0 * a.ldx);
   auto copy = [&](int kb) {
     const uint32_t base = lds0 + (kb % kStages) * kStageBytes;
     const int k0 = (kt0 + (kb >> 1)) * 128 + (kb & 1) * 32;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i)
-      copy_to_lds(a.x + arow[i] + min(k0 + akc[i], K - 8), base + (wave * kCopies + i) * 1024);
+      copy_to_lds(xbase, arow[i] + 2 * min(k0 + akc[i], K - 8), base + (wave * kCopies + i) * 1024);
   };
 
   // a tile's weights of this wave: words 2 kh, 2 kh + 1 and their scales
   constexpr int SG = GU == 4 ? 2 : 1;   // scales per half tile
+  typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
   struct BBuf {
-    uint2 w[TN];
-    uint16_t s[TN][SG];
+    u32x2_t w[TN];
+    uint32_t s[TN][SG];
   };
+  // (buffer loads: offsets of a tile are scalar)
+  const int ntb = min(nt0, a.NT - 1), tiles = min(TN, a.NT - ntb) * a.KT;
+  const auto wrsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint32_t*>(a.w + (int64_t)ntb * a.KT * kTileWords), 0,
+                                                       tiles * 1024, 0x20000);
+  const auto srsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.scale + (int64_t)ntb * a.KT * (GU * 16)), 0,
+                                                       tiles * (GU * 32), 0x20000);
+  const int wv = lane * 16 + kh * 8, sv = col * 2 + (GU == 4 ? 2 * kh : GU == 2 ? kh : 0) * 32;
   auto load = [&](BBuf& b, int kt) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int64_t tile = (int64_t)min(nt0 + j, a.NT - 1) * a.KT + min(kt, kt1 - 1);
-      b.w[j] = *reinterpret_cast<const uint2*>(a.w + tile * kTileWords + lane * 4 + 2 * kh);
+      const int tile = (min(nt0 + j, a.NT - 1) - ntb) * a.KT + min(kt, kt1 - 1);
+      b.w[j] = __builtin_amdgcn_raw_buffer_load_b64(wrsrc, wv, tile * 1024, 0);
 #pragma unroll
-      for (int g = 0; g < SG; ++g)
-        b.s[j][g] = a.scale[(tile * GU + (GU == 4 ? 2 * kh + g : GU == 2 ? kh : 0)) * 16 + col];
+      for (int g = 0; g < SG; ++g) b.s[j][g] = __builtin_amdgcn_raw_buffer_load_b16(srsrc, sv + 32 * g, tile * (GU * 32), 0);
     }
   };
 
@@ -465,9 +477,10 @@ __global__ __launch_bounds__(kGThreads, 2) void int4_gemm_kernel(Int4Args a) {
     for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
 
   const Unpack unpack;
-  auto step = [&](const BBuf& b, int kb, auto half_c) {
+  auto step = [&](const BBuf& b, int kb, auto half_c, auto more_c) {
     constexpr int half = decltype(half_c)::value;
-    if (kb + 1 < nk) wait_vm<kCopies>();
+    // x of step kb landed: newer are the next step's copies and, with `more`, one tile's weights
+    if (kb + 1 < nk) wait_vm<kCopies + (decltype(more_c)::value ? TN * (1 + SG) : 0)>();
     else wait_vm<0>();
     lds_read_barrier();
     if (kb + 2 < nk) copy(kb + 2);
@@ -475,8 +488,8 @@ __global__ __launch_bounds__(kGThreads, 2) void int4_gemm_kernel(Int4Args a) {
     h8_t bf[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const _Float16 s1 = __builtin_bit_cast(_Float16, b.s[j][SG == 2 ? half : 0]);
-      bf[j] = word_scaled(unpack, half ? b.w[j].y : b.w[j].x, h2_t{s1, s1});
+      const _Float16 s1 = __builtin_bit_cast(_Float16, (uint16_t)b.s[j][SG == 2 ? half : 0]);
+      bf[j] = word_scaled(unpack, half ? b.w[j][1] : b.w[j][0], h2_t{s1, s1});
     }
 #pragma unroll
     for (int i = 0; i < RI; ++i) {
@@ -488,24 +501,33 @@ __global__ __launch_bounds__(kGThreads, 2) void int4_gemm_kernel(Int4Args a) {
     }
   };
 
-  BBuf b0, b1;
-  load(b0, kt0);
+  BBuf b[NB];
+#pragma unroll
+  for (int i = 0; i + 1 < NB; ++i) load(b[i], kt0 + i);
   copy(0);
   if (nk > 1) copy(1);
+  auto tile = [&](int kt, auto i_c, auto more_c) {
+    constexpr int i = decltype(i_c)::value;
+    if constexpr (decltype(more_c)::value) load(b[(i + NB - 1) % NB], kt + NB - 1);
+    step(b[i], 2 * (kt - kt0), std::integral_constant<int, 0>{}, more_c);
+    step(b[i], 2 * (kt - kt0) + 1, std::integral_constant<int, 1>{}, more_c);
+  };
+  using std::integral_constant;
+  const std::true_type more{};
   int kt = kt0;
-  for (; kt + 1 < kt1; kt += 2) {
-    const int kb = 2 * (kt - kt0);
-    load(b1, kt + 1);
-    step(b0, kb, std::integral_constant<int, 0>{});
-    step(b0, kb + 1, std::integral_constant<int, 1>{});
-    load(b0, kt + 2);
-    step(b1, kb + 2, std::integral_constant<int, 0>{});
-    step(b1, kb + 3, std::integral_constant<int, 1>{});
+  for (; kt + NB <= kt1; kt += NB) {    // (without exits: they would make the compiler wait for all loads)
+    tile(kt, integral_constant<int, 0>{}, more);
+    tile(kt + 1, integral_constant<int, 1>{}, more);
+    if constexpr (NB == 4) {
+      tile(kt + 2, integral_constant<int, 2>{}, more);
+      tile(kt + 3, integral_constant<int, 3>{}, more);
+    }
   }
-  if (kt < kt1) {
-    const int kb = 2 * (kt - kt0);
-    step(b0, kb, std::integral_constant<int, 0>{});
-    step(b0, kb + 1, std::integral_constant<int, 1>{});
+  const std::false_type last{};         // all weights are on the way
+  if (kt < kt1) tile(kt, integral_constant<int, 0>{}, last);
+  if constexpr (NB == 4) {
+    if (kt + 1 < kt1) tile(kt + 1, integral_constant<int, 1>{}, last);
+    if (kt + 2 < kt1) tile(kt + 2, integral_constant<int, 2>{}, last);
   }
 
   // wave (kh, side) keeps half of the row tiles and hands the others to wave ^ 2
@@ -544,26 +566,33 @@ __global__ __launch_bounds__(kGThreads, 2) void int4_gemm_kernel(Int4Args a) {
   else finish(std::integral_constant<int, RI / 2>{});
 }
 
-// Row tiles (16 RI rows) and k slices of a prompt: rounds of the workgroup slots (three a CU at
-// RI = 4, two above) x the tile's cost (its MFMAs, and what unpacking and the step itself
-// cost whatever the height).  1500 x 4096 -> 12288: RI = 8 takes 1152 tiles, 2.25 rounds of 512, RI =
-// 6 1536, exactly 3 of three quarters the height.  Few tiles split k until the slots fill.
+// Row tiles (16 RI rows) and k slices of a prompt, by the time of a slice's 128-input tiles: a
+// CU's workgroups share its matrix and vector units (us per tile for each that it gets), and a
+// round of them (three a CU at RI <= 4, two above) takes at least a wave's own latencies; slices
+// add the partial sums' way out and back and a second launch.  Fitted to 1670 timed (shape, RI,
+// S) of 20 to 2048 tokens, within 7% of each; what it picks is 1% off the fastest on average, 11%
+// at most.  1500 x 4096 -> 12288 takes 159 us in tiles of 96 rows (exactly six workgroups a CU), 169
+// in 64 and 162 in 128; 150 x 5120 -> 17408 takes 51 us in tiles of 64 and 57 in 32 or 96.
 struct GemmPlan {
   int ri, S;
 };
 GemmPlan plan_gemm(int M, int NT, int KT) {
   GemmPlan p{8, 1};
   double least = -1.0;
-  for (int ri = 8; ri >= 2; ri -= 2) {
-    if (ri > 2 && 16 * (ri - 2) >= M) continue;        // taller than the rows need
+  for (int ri = 2; ri <= 8; ri += 2) {
     const int64_t tiles = (int64_t)((NT + 7) / 8) * ((M + 16 * ri - 1) / (16 * ri));
     const int64_t slots = ri <= 4 ? 768 : 512;
-    const int S = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(slots / std::max<int64_t>(tiles, 1), KT / 4), 16));
-    const double c = (double)((tiles * S + slots - 1) / slots) * ((KT + S - 1) / S) * (ri + 1.5) + (S > 1 ? 30.0 : 0.0);
-    if (least < 0.0 || c < 0.97 * least) {
-      least = c;
-      p = {ri, S};
+    for (int S = 1; S <= std::min(KT, 16); ++S) {
+      const int64_t w = tiles * S;
+      const double shared = (double)((w + 255) / 256) * (0.24 + 0.079 * ri);
+      const double alone = (double)((w + slots - 1) / slots) * (0.38 + 0.126 * ri);
+      const double c = ((KT + S - 1) / S) * std::max(shared, alone) + (S > 1 ? 2.75 + (double)S * M * NT * 128.0 / 6e6 : 0.0);
+      if (least < 0.0 || c < least) {
+        least = c;
+        p = {ri, S};
+      }
     }
+    if (16 * ri >= M) break;            // taller than the rows need
   }
   return p;
 }
@@ -602,6 +631,7 @@ extern "C" int helm_int4_linear(const void* x, int64_t ldx, const void* qweight,
   HELM_CHECK_SUPPORTED(group_size == 32 || group_size == 64 || group_size == 128,
                        "helm_int4_linear: group size must be 32, 64 or 128");
   HELM_CHECK_SUPPORTED(K % group_size == 0, "helm_int4_linear: K must be a multiple of the group size");
+  HELM_CHECK_SUPPORTED(M == 1 || ldx <= (1 << 23), "helm_int4_linear: ldx above 2^23");
   HELM_CHECK_SUPPORTED(ldx % 8 == 0 && helm::aligned16(x) && helm::aligned16(qweight) && helm::aligned16(scale),
                        "helm_int4_linear: x rows, qweight and scale must be 16-byte aligned");
   Int4Args a{};

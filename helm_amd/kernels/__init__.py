@@ -384,7 +384,7 @@ def int4_linear(input: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Te
     x2 = _flatten(input, K, "int4_linear")
     M = x2.shape[0]
     ldx = x2.stride(0) if M > 1 else K
-    if ldx < K or x2.data_ptr() % 16:       # rows that overlap (an expanded input), or lie askew
+    if ldx < K or ldx > 1 << 23 or x2.data_ptr() % 16:   # rows that overlap (an expanded input), lie askew or far apart
         x2, ldx = x2.clone(memory_format=torch.contiguous_format), K
     if out is None:
         out = input.new_empty((*input.shape[:-1], N))

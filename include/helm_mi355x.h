@@ -147,8 +147,8 @@ int helm_int8_gemm_ws(const void* x, int64_t ldx, const int8_t* q, int64_t ldq,
  *           inputs past K hold code 0 (nibble 8).
  *   scale   fp16 [NT][KT][128 / group_size][16], 0 past N and K
  *   bias    [N] fp16 or NULL
- * Requirements: K % group_size == 0, ldx % 8 == 0, x, qweight and scale 16-byte aligned;
- * workspace (16-byte aligned, contents on entry do not matter) of at least
+ * Requirements: K % group_size == 0, N <= 2^27, K <= 2^19, ldx % 8 == 0 (and <= 2^23 at M > 1),
+ * x, qweight and scale 16-byte aligned; workspace (16-byte aligned, contents on entry do not matter) of at least
  * helm_int4_linear_workspace_bytes (0: may be NULL).  Beside helm_int8_gemv_ws and
  * helm_int8_gemm_ws, the counterparts of fp16_gemv.cpp:105-157. */
 int64_t helm_int4_linear_workspace_bytes(int M, int N, int K, int group_size);

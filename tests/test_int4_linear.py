@@ -207,3 +207,32 @@ def test_captured_and_on_another_stream(cuda, m):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, eager[i])
+
+
+def test_rows_too_far_apart_for_the_c_entry():
+    import ctypes
+    fake = ctypes.c_void_p(16)
+    far = _native.lib().helm_int4_linear
+    assert far(fake, (1 << 23) + 8, fake, fake, 64, None, fake, 16, 2, 16, 128, None, 0, None) == -2
+    assert b"2^23" in _native.lib().helm_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [2, 20])
+def test_rows_far_apart(cuda, m):
+    codes, scale = make(40, 256, 64, 6)
+    w = hk.Int4Weight.pack(codes, scale).to(cuda)
+    for ldx in (1 << 23, (1 << 23) + 8):
+        x = torch.empty((m - 1) * ldx + 256, dtype=torch.float16, device=cuda).as_strided((m, 256), (ldx, 1))
+        x.copy_(torch.randn(m, 256, generator=torch.Generator().manual_seed(m)).half())
+        check(hk.int4_linear(x, w), x, codes, scale, None, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gs", [32, 64, 128])
+@pytest.mark.parametrize("m,n,k", [(20, 4096, 4096), (60, 900, 2176), (95, 2000, 1152), (127, 4100, 1408), (260, 1300, 640),
+                                   (500, 2064, 896), (129, 300, 128), (33, 130, 384)])
+def test_prompts_of_every_tile_height_and_slicing(cuda, m, n, k, gs):
+    codes, scale = make(n, k, gs, m)
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(n)).half().cuda()
+    check(hk.int4_linear(x, hk.Int4Weight.pack(codes.cuda(), scale.cuda())), x, codes, scale, None, gs)
