@@ -101,7 +101,8 @@ __device__ __forceinline__ const void* uniform(const void* p) {
 // row tiles tb, tb + nb, ....  Weights go global -> LDS through a private ring of kDepth
 // tiles per wave, and the scales of a row tile's share through another, waited for by count:
 // 96 KB on the way per CU, and no register holds any (two or three row tiles in registers
-// instead spilled, or kept less on the way: 4.2 TB/s).  A tile is read back as it lies, a
+// instead spilled, or kept less on the way: 4.2 TB/s; this streams 151936 x 4096, 321 MB, at
+// 5.6, and 5120 -> 34816, 92 MB in 20.4 us, at 4.5, of which 5 us are its start).  A tile is read back as it lies, a
 // 16-byte operand word group per lane.
 // The products run on b + u; the -sum((b + 8) x) that turns them into codes is the same for
 // every output, so it is computed once per wave and group (an MFMA with a constant operand)
@@ -319,9 +320,11 @@ __global__ __launch_bounds__(256) void int4_reduce_kernel(const float* __restric
 }
 
 // k slices of a GEMV, tiles per wave (at most what x^T leaves of 128 registers), workgroups per
-// slice.  Every workgroup is on a CU from the start, so the longest one counts: row tiles x
-// tiles per wave, 0.67 us each (16 KB at 6 TB/s / 256), its x (45 KB / us from L2), the partial
-// sums' traffic (4 TB/s) and the second launch (3 us).
+// slice.  Every workgroup is on a CU from the start, so the longest one counts: its row tiles,
+// the x that it reads, and where there are slices the partial sums' traffic and a second
+// launch.  Fitted (us) to 810 timed (shape, tokens, S), within 5% of each; what it picks is 1% off
+// the fastest on average, 8% at most.  5120 x 17408 at 16 tokens: 20 us in 9 slices, 17.6 in 5, 18.4
+// in 3; 4096 x 4096 at 1: 5.6 in one, 7.5 in 2.
 constexpr int max_uw(int GU) { return GU == 1 ? 4 : GU == 2 ? 3 : 2; }
 struct GemvPlan {
   int S, uw, nb;
@@ -334,7 +337,8 @@ GemvPlan plan_gemv(int M, int NT, int KT, int GU) {
     p.S = S;
     p.uw = ((KT + S - 1) / S + kW - 1) / kW;
     p.nb = S > 1 ? std::min(NT, 256 / S) : std::max(std::min(NT, 256), (NT + kMaxTiles - 1) / kMaxTiles);
-    const double c = 0.67 * ((NT + p.nb - 1) / p.nb) * (p.uw + 0.25) + M * KT * 256.0 / S / 45e3 + (S > 1 ? 3.0 + (double)S * M * NT * 128.0 / 4e6 : 0.0);
+    const double c = ((NT + p.nb - 1) / p.nb) * (0.45 + 0.32 * p.uw + 0.034 * p.uw * (GU - 1)) + 0.88 * p.uw +
+                     0.0062 * M * KT / S + (S > 1 ? 2.76 + (double)S * M * NT * 128.0 / 4.2e6 : 0.0);
     if (least < 0.0 || c < least) {
       least = c;
       best = p;
