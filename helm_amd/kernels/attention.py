@@ -519,7 +519,8 @@ def kv_append_q8(k_new: torch.Tensor, v_new: torch.Tensor, pool: Q8PoolView, slo
     """Quantise k_new/v_new [B, Hkv, n_tok, D] fp16 into (slots[b], offsets[b] + t) of an
     8-bit pool: scale = fp16(max |x| / 127) per token and head, code = x / scale rounded to
     nearest even.  Tokens whose slot is outside the pool or whose offset is outside the page
-    are skipped; of two tokens for one place, one is kept (which one is not defined)."""
+    are skipped.  Two tokens of a call must not name one place (what it holds then is not
+    defined)."""
     what = "kv_append_q8"
     index = _native.gpu_of(what, k_new, v_new, pool.k, slots, offsets)
     P = pool._check_page_size(page_size, what)

@@ -149,7 +149,8 @@ def qk_norm_rope_append_q8(qkv: torch.Tensor, q_norm_w: Optional[torch.Tensor],
     """qk_norm_rope_append into an 8-bit pool (an attention.Q8PoolView): q/k RMSNorm (when
     the norm weights are given) + RoPE of the fused qkv [B, (Hq+2Hkv)*D] in fp32, the angle
     in 64 bits; the rotated q rounded to fp16 once into q_out [B, Hq, D], k and v quantised
-    into (slots[b], offsets[b]) with a scale per token and head, as kv_append_q8 does."""
+    into (slots[b], offsets[b]) with a scale per token and head, as kv_append_q8 does (tokens
+    with a place outside the pool are not kept, and no two name one place)."""
     what = "qk_norm_rope_append_q8"
     index = _native.gpu_of(what, qkv, q_norm_w, k_norm_w, positions, inv_freq, q_out, pool.k, slots, offsets)
     _check_fp16(qkv, q_norm_w, k_norm_w, q_out)
@@ -268,7 +269,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
     the ones of at least min_p times the largest; then, in index order, the token at which
     the summed weight passes u times the sum of all.  temperature 0 is `argmax`.  Each
     setting is a number, or a tensor with one per row (fp32, top_k int32).  NaN logits are
-    never drawn; a row with no logit above -inf gives 0.  `workspace` from
+    never drawn; a row with no logit above -inf gives 0.  N is at most 262144.  `workspace` from
     sample_workspace, allocated here when not given."""
     tensors = [x for x in (temperature, top_k, top_p, min_p) if torch.is_tensor(x)]
     index = _native.gpu_of("sample", logits, u, out, workspace, *tensors)

@@ -402,7 +402,8 @@ typedef struct helm_kv_pool_q8 {
  * and head, code = x / scale rounded to nearest even, in [-127, 127] (0 where the scale
  * rounds to 0; values that are not finite give a scale that is not).  k_new / v_new
  * [B, Hkv, n_tok, D] fp16 contiguous, token t of item b to (slots[b], offsets[b] + t);
- * slots outside [0, num_slots) and offsets outside [0, P) are skipped.  Replaces the same
+ * slots outside [0, num_slots) and offsets outside [0, P) are skipped, and two tokens of a
+ * call must not name one place (what it holds then is not defined).  Replaces the same
  * copies as helm_kv_append (helm/runtime/kv_cache.py:103-107). */
 int helm_kv_append_q8(const void* k_new, const void* v_new, const helm_kv_pool_q8* pool,
                       const int32_t* slots, const int32_t* offsets,
@@ -413,7 +414,7 @@ int helm_kv_append_q8(const void* k_new, const void* v_new, const helm_kv_pool_q
  * angle positions[b] * inv_freq[i] in 64 bits, so far positions keep theirs), q rounded
  * to fp16 once into q_out [B, Hq, D], k and v quantised as by helm_kv_append_q8 (k from
  * fp32) into page slot slots[b] at offset offsets[b].  qkv [B, (Hq + 2*Hkv) * D] fp16,
- * row stride qkv_stride_b (a multiple of 8; rows 16-byte aligned).  Follows
+ * row stride qkv_stride_b (a multiple of 8; rows, norm weights and q_out 16-byte aligned).  Follows
  * helm/runtime/kv_offload.py:244-249 and kv_cache.py:103-107. */
 int helm_qk_norm_rope_append_q8(const void* qkv, int64_t qkv_stride_b, const void* q_norm_w,
                                 const void* k_norm_w, float eps, const int32_t* positions,
@@ -429,7 +430,8 @@ int helm_dequantize_pages(const helm_kv_pool_q8* pool, const int32_t* pages, int
                           void* v_out, int Hkv, int D, int P, void* stream);
 
 /* helm_paged_decode_attn and helm_paged_attn_reduce over 8-bit pages: out [B, Hq, D] fp16
- * contiguous = softmax(scale * q . K^T) V; zeros for an item of 0 tokens.  num_splits
+ * contiguous = softmax(scale * q . K^T) V; zeros for an item of 0 tokens, and tokens past
+ * the table's max_pages * P are left out.  num_splits
  * splits take an item's 64-token steps round robin (0: as many as suit the shape; more than
  * asked for where one would cover over helm_paged_attn_max_split_pages() table entries).
  * workspace (16-byte aligned, contents on entry do not matter) of
@@ -514,7 +516,8 @@ int helm_argmax_f16_ws(const void* x, int64_t ldx, int M, int N, int64_t* out,
  * as 0).  NaN logits have no weight (t > 0).  A row without any logit above -inf gives
  * its first index.  temperature / top_p / min_p (fp32 [M]) and top_k (int32 [M]) are read
  * per row, or, where null, t / k / p / lo serve every row.  workspace: 16-byte aligned,
- * helm_sample_workspace_bytes(M, N) bytes, contents on entry do not matter.  The sampled
+ * helm_sample_workspace_bytes(M, N) bytes, contents on entry do not matter.  M is at most
+ * 65535, N 262144.  The sampled
  * form of the argmax of pipeline_runtime.py:160. */
 int64_t helm_sample_workspace_bytes(int M, int N);
 int helm_sample(const void* x, int64_t ldx, int M, int N, const float* u, const float* temperature,
