@@ -464,10 +464,11 @@ def paged_decode_attention_q8(q: torch.Tensor, pool: Q8PoolView, page_table: tor
     """paged_decode_attention over 8-bit pages: out[b, h] = softmax(scale q[b,h] K_b^T) V_b,
     K and V the values that codes and scales stand for.
 
-    q [B, Hq, D] fp16; page_table [B, max_pages] int32 slots; seq_lens [B] int32.  `num_splits`
-    splits share an item's tokens (0: as many as suit the shape).  Returns out [B, Hq, D] fp16
-    (zeros for an empty item).  `workspace` is allocated here when not given; calls that overlap, or
-    two graphs that may replay at once, need one each."""
+    q [B, Hq, D] fp16, up to 16 heads per kv head; page_table [B, max_pages] int32 slots; seq_lens
+    [B] int32 (tokens past the table's pages are left out).  `num_splits` splits share an item's
+    tokens (0: as many as suit the shape).  Returns out [B, Hq, D] fp16 (zeros for an empty
+    item).  `workspace` is allocated here when not given; calls that overlap, or two graphs that
+    may replay at once, need one each."""
     what = "paged_decode_attention_q8"
     index = _native.gpu_of(what, q, pool.k, page_table, seq_lens, out)
     if q.dtype != torch.float16 or q.dim() != 3 or q.stride(2) != 1:

@@ -431,7 +431,7 @@ int helm_dequantize_pages(const helm_kv_pool_q8* pool, const int32_t* pages, int
 
 /* helm_paged_decode_attn and helm_paged_attn_reduce over 8-bit pages: out [B, Hq, D] fp16
  * contiguous = softmax(scale * q . K^T) V; zeros for an item of 0 tokens, and tokens past
- * the table's max_pages * P are left out.  num_splits
+ * the table's max_pages * P are left out; up to 16 query heads per kv head.  num_splits
  * splits take an item's 64-token steps round robin (0: as many as suit the shape; more than
  * asked for where one would cover over helm_paged_attn_max_split_pages() table entries).
  * workspace (16-byte aligned, contents on entry do not matter) of
