@@ -102,7 +102,7 @@ __device__ __forceinline__ const void* uniform(const void* p) {
 // tiles per wave, and the scales of a row tile's share through another, waited for by count:
 // 96 KB on the way per CU, and no register holds any (two or three row tiles in registers
 // instead spilled, or kept less on the way: 4.2 TB/s; this streams 151936 x 4096, 321 MB, at
-// 5.6, and 5120 -> 34816, 92 MB in 20.4 us, at 4.5, of which 5 us are its start).  A tile is read back as it lies, a
+// 6.1, and 5120 -> 34816, 92 MB in 20 us, at 4.6, of which 5 us are its start).  A tile is read back as it lies, a
 // 16-byte operand word group per lane.
 // The products run on b + u; the -sum((b + 8) x) that turns them into codes is the same for
 // every output, so it is computed once per wave and group (an MFMA with a constant operand)
@@ -174,10 +174,6 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
     copy_nt_to_lds(uniform(wbase + (tile + (u < own ? u : 0)) * 1024), u < own ? woff : 0u, at_w);
     at_w = at_w + 1024 == lds_w + kDepth * 1024 ? lds_w : at_w + 1024;
   };
-  // the first row tile's share goes out ahead of x (at one row tile it is all there is)
-#pragma unroll
-  for (int u = 0; u < UW; ++u) issue(0, u);
-
   h8_t xr[UW][4];
   const uint16_t* xrow = a.x + (int64_t)min(col, M - 1) * a.ldx;
 #pragma unroll
@@ -185,6 +181,12 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
 #pragma unroll
     for (int t = 0; t < 4; ++t)
       xr[u][t] = *reinterpret_cast<const h8_t*>(xrow + min((u0 + u) * 128 + t * 32 + grp * 8, a.K - 8));
+  asm volatile("" ::: "memory");
+  // the first row tile's share right behind x; x's wait covers both (ahead of x: 7.1 us instead
+  // of 6.9 at 4096 x 4096 and 16 tokens, the same at one)
+#pragma unroll
+  for (int u = 0; u < UW; ++u) issue(0, u);
+
   // bias of the workgroup's outputs, one of each per thread
   uint16_t bs = 0;
   if constexpr (!PART) {
@@ -224,7 +226,6 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
       }
   }
   const Unpack unpack;
-  lds_barrier();                      // staged biases
 
   const uint8_t* pw = &s_w[wave][0];  // slots read next
   const uint8_t* ps = &s_s[wave][0];
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
     lds_barrier();      // buffer t & 1 is written again only after tile t + 1's barrier
     if (wave == (t & (kW - 1))) {
       f4_t v = sc[0][lane];
-#pragma unroll 5
+#pragma unroll (UW <= 2 ? 15 : 5)       // (as many reads on the way as registers are left: 57 -> 53 us at 151936 x 4096)
       for (int w = 1; w < kW; ++w) {
         const f4_t o = sc[w][lane];
 #pragma unroll
