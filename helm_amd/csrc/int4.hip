@@ -50,6 +50,8 @@ __device__ __forceinline__ void wait_vm() {
 __device__ __forceinline__ void wait_vm_n(int n) {      // n: a constant once inlined
   asm volatile("" ::: "memory");
   switch (n) {
+    case 3: __builtin_amdgcn_s_waitcnt(3 | (7 << 4) | (15 << 8)); break;
+    case 4: __builtin_amdgcn_s_waitcnt(4 | (7 << 4) | (15 << 8)); break;
     case 5: __builtin_amdgcn_s_waitcnt(5 | (7 << 4) | (15 << 8)); break;
     case 6: __builtin_amdgcn_s_waitcnt(6 | (7 << 4) | (15 << 8)); break;
     case 7: __builtin_amdgcn_s_waitcnt(7 | (7 << 4) | (15 << 8)); break;
@@ -93,7 +95,7 @@ __device__ __forceinline__ const void* uniform(const void* p) {
 }
 
 // ---------------------------------------------------------------------------
-// 1 to 16 tokens
+// 1 to 32 tokens
 // ---------------------------------------------------------------------------
 // Bound by the weight stream, and by the instructions that unpack it: x^T operands of a
 // wave's inputs stay in registers; a workgroup's 16 waves (four a SIMD: a wave alone takes 950
@@ -102,16 +104,18 @@ __device__ __forceinline__ const void* uniform(const void* p) {
 // tiles per wave, and the scales of a row tile's share through another, waited for by count:
 // 96 KB on the way per CU, and no register holds any (two or three row tiles in registers
 // instead spilled, or kept less on the way: 4.2 TB/s; this streams 151936 x 4096, 321 MB, at
-// 6.1, and 5120 -> 34816, 92 MB in 20 us, at 4.6, of which 5 us are its start).  A tile is read back as it lies, a
-// 16-byte operand word group per lane.
+// 6.1, and 5120 -> 34816, 92 MB in 20 us, at 4.6, of which 5 us are its start).  A tile is read
+// back as it lies, a 16-byte operand word group per lane.
 // The products run on b + u; the -sum((b + 8) x) that turns them into codes is the same for
 // every output, so it is computed once per wave and group (an MFMA with a constant operand)
 // and starts each accumulation: fp32 sums of numbers up to 264 |x| (2^-24 of them: 2^-13 of a
 // code's unit).  A group's sum is scaled by its outputs' scales in fp32.  The waves' partial
 // tiles meet in LDS, one barrier per row tile, and take turns at the epilogue.
+// 17 to 32 tokens are two operands of each unpacked weight: 12288 x 4096 at 24 tokens 12.5 us
+// against the tiled product's 17.2, 4096 x 12288 at 32 16.5 against 17.3, 1.17 times as fast over
+// 12 shapes.
+constexpr int kGemvTokens = 32;
 constexpr int kW = 16;
-constexpr int kDepth = 6;             // tiles of a wave on the way
-constexpr int kScSlots = 7;           // row tiles whose scales are (256 bytes each)
 constexpr int kMaxTiles = 64;         // row tiles a workgroup may walk (staged biases)
 
 struct Int4Args {
@@ -130,11 +134,15 @@ struct Int4Args {
 
 // UW: tiles of a wave's k share.  GU: groups per tile (UW * GU <= 8: a row tile's scales are
 // one copy).
-template <int UW, int GU, bool PART>
+// MB: blocks of 16 tokens.
+template <int UW, int GU, bool PART, int MB>
 __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
+  // tiles of a wave on the way, and row tiles whose scales are (256 bytes each): what the
+  // partial tiles leave of LDS
+  constexpr int kDepth = MB == 1 ? 6 : 4, kScSlots = kDepth + 1;
   __shared__ __attribute__((aligned(1024))) uint8_t s_w[kW][kDepth * 1024];
   __shared__ __attribute__((aligned(16))) uint8_t s_s[kW][kScSlots * 256];
-  __shared__ __attribute__((aligned(16))) f4_t s_c[2][kW][64];
+  __shared__ __attribute__((aligned(16))) f4_t s_c[2][MB][kW][64];
   __shared__ uint16_t s_bias[PART ? 2 : kMaxTiles * 16];
   constexpr int TG = 4 / GU;          // MFMAs per group
   static_assert(UW * GU <= 8 && (kDepth + UW - 1) / UW + 1 <= kScSlots, "scale ring");
@@ -174,13 +182,16 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
     copy_nt_to_lds(uniform(wbase + (tile + (u < own ? u : 0)) * 1024), u < own ? woff : 0u, at_w);
     at_w = at_w + 1024 == lds_w + kDepth * 1024 ? lds_w : at_w + 1024;
   };
-  h8_t xr[UW][4];
-  const uint16_t* xrow = a.x + (int64_t)min(col, M - 1) * a.ldx;
+  h8_t xr[MB][UW][4];
 #pragma unroll
-  for (int u = 0; u < UW; ++u)
+  for (int mb = 0; mb < MB; ++mb) {
+    const uint16_t* xrow = a.x + (int64_t)min(mb * 16 + col, M - 1) * a.ldx;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      xr[u][t] = *reinterpret_cast<const h8_t*>(xrow + min((u0 + u) * 128 + t * 32 + grp * 8, a.K - 8));
+    for (int u = 0; u < UW; ++u)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        xr[mb][u][t] = *reinterpret_cast<const h8_t*>(xrow + min((u0 + u) * 128 + t * 32 + grp * 8, a.K - 8));
+  }
   asm volatile("" ::: "memory");
   // the first row tile's share right behind x; x's wait covers both (ahead of x: 7.1 us instead
   // of 6.9 at 4096 x 4096 and 16 tokens, the same at one)
@@ -195,9 +206,11 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
   }
   // x has arrived: from here on the ring fills while the prologue computes
 #pragma unroll
-  for (int u = 0; u < UW; ++u)
+  for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(xr[u][t]));
+    for (int u = 0; u < UW; ++u)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) asm volatile("" : "+v"(xr[mb][u][t]));
   if constexpr (!PART) {
     static_assert(kMaxTiles * 16 == kW * 64, "one bias per thread");
     s_bias[tid] = bs;
@@ -206,24 +219,28 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
   for (int n = UW; n < kDepth; ++n)
     if (n / UW < T) issue(n / UW, n % UW);
 #pragma unroll
-  for (int u = 0; u < UW; ++u)
+  for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      if (u >= own || (u0 + u) * 128 + t * 32 >= a.K) xr[u][t] = h8_t{};
+    for (int u = 0; u < UW; ++u)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (u >= own || (u0 + u) * 128 + t * 32 >= a.K) xr[mb][u][t] = h8_t{};
   // -sum((b + 8) x) of each group: every row of the product with a constant operand
-  float nbias[UW][GU];
+  float nbias[MB][UW][GU];
   {
     const _Float16 p = (_Float16)-264.0f, q = (_Float16)-24.0f;
     const h8_t c = {p, p, q, q, p, p, q, q};
 #pragma unroll
-    for (int u = 0; u < UW; ++u)
+    for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int g = 0; g < GU; ++g) {
-        f4_t s = {0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < UW; ++u)
 #pragma unroll
-        for (int t = 0; t < TG; ++t) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, xr[u][g * TG + t], s, 0, 0, 0);
-        nbias[u][g] = s[0];
-      }
+        for (int g = 0; g < GU; ++g) {
+          f4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = 0; t < TG; ++t) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, xr[mb][u][g * TG + t], s, 0, 0, 0);
+          nbias[mb][u][g] = s[0];
+        }
   }
   const Unpack unpack;
 
@@ -231,7 +248,9 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
   const uint8_t* ps = &s_s[wave][0];
   const int total = T * UW;
   for (int t = 0; t < T; ++t) {
-    f4_t acc = {0.f, 0.f, 0.f, 0.f};
+    f4_t acc[MB];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) acc[mb] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < UW; ++u) {
       // tile landed: at most the kDepth - 1 later tiles' copies are on the way, and those of
@@ -258,36 +277,44 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
       const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int g = 0; g < GU; ++g) {
-        float z = nbias[u][g];
-        asm("" : "+v"(z));            // (or four copies of each would be kept)
-        f4_t c = {z, z, z, z};
+        h8_t wf[TG];
 #pragma unroll
-        for (int q = 0; q < TG; ++q)
-          c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, unpack(wd[g * TG + q])), xr[u][g * TG + q], c, 0, 0, 0);
-        acc[0] = fmaf(lo_h(sc[g].x), c[0], acc[0]);
-        acc[1] = fmaf(hi_h(sc[g].x), c[1], acc[1]);
-        acc[2] = fmaf(lo_h(sc[g].y), c[2], acc[2]);
-        acc[3] = fmaf(hi_h(sc[g].y), c[3], acc[3]);
+        for (int q = 0; q < TG; ++q) wf[q] = __builtin_bit_cast(h8_t, unpack(wd[g * TG + q]));
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          float z = nbias[mb][u][g];
+          asm("" : "+v"(z));          // (or four copies of each would be kept)
+          f4_t c = {z, z, z, z};
+#pragma unroll
+          for (int q = 0; q < TG; ++q) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[q], xr[mb][u][g * TG + q], c, 0, 0, 0);
+          acc[mb][0] = fmaf(lo_h(sc[g].x), c[0], acc[mb][0]);
+          acc[mb][1] = fmaf(hi_h(sc[g].x), c[1], acc[mb][1]);
+          acc[mb][2] = fmaf(lo_h(sc[g].y), c[2], acc[mb][2]);
+          acc[mb][3] = fmaf(hi_h(sc[g].y), c[3], acc[mb][3]);
+        }
       }
     }
     ps = ps + 256 == &s_s[wave][kScSlots * 256] ? &s_s[wave][0] : ps + 256;
-    f4_t (*sc)[64] = s_c[t & 1];
-    sc[wave][lane] = acc;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) s_c[t & 1][mb][wave][lane] = acc[mb];
     lds_barrier();      // buffer t & 1 is written again only after tile t + 1's barrier
-    if (wave == (t & (kW - 1))) {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      if (wave != ((t * MB + mb) & (kW - 1))) continue;
+      const f4_t(*sc)[64] = s_c[t & 1][mb];
       f4_t v = sc[0][lane];
-#pragma unroll (UW <= 2 ? 15 : 5)       // (as many reads on the way as registers are left: 57 -> 53 us at 151936 x 4096)
+#pragma unroll (UW * MB <= 2 ? 15 : 5)  // (as many reads on the way as registers are left: 57 -> 53 us at 151936 x 4096)
       for (int w = 1; w < kW; ++w) {
         const f4_t o = sc[w][lane];
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] += o[r];
       }
-      const int n0 = (tb + t * nb) * 16 + grp * 4;   // v[r]: output n0 + r of token col
-      if (col < M && n0 < a.N) {
+      const int n0 = (tb + t * nb) * 16 + grp * 4, m = mb * 16 + col;   // v[r]: output n0 + r of token m
+      if (m < M && n0 < a.N) {
         if constexpr (PART) {
-          *reinterpret_cast<f4_t*>(a.part + ((int64_t)sl * M + col) * a.np + n0) = v;
+          *reinterpret_cast<f4_t*>(a.part + ((int64_t)sl * M + m) * a.np + n0) = v;
         } else {
-          uint16_t* yp = a.y + (int64_t)col * a.ldy + n0;
+          uint16_t* yp = a.y + (int64_t)m * a.ldy + n0;
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             if (n0 + r < a.N) yp[r] = f2h(v[r] + h2f(s_bias[t * 16 + grp * 4 + r]));
@@ -323,23 +350,25 @@ __global__ __launch_bounds__(256) void int4_reduce_kernel(const float* __restric
 // k slices of a GEMV, tiles per wave (at most what x^T leaves of 128 registers), workgroups per
 // slice.  Every workgroup is on a CU from the start, so the longest one counts: its row tiles,
 // the x that it reads, and where there are slices the partial sums' traffic and a second
-// launch.  Fitted (us) to 810 timed (shape, tokens, S), within 5% of each; what it picks is 1% off
+// launch.  Fitted (us) to 1149 timed (shape, tokens, S), within 5% of each; what it picks is 1% off
 // the fastest on average, 8% at most.  5120 x 17408 at 16 tokens: 20 us in 9 slices, 17.6 in 5, 18.4
 // in 3; 4096 x 4096 at 1: 5.6 in one, 7.5 in 2.
-constexpr int max_uw(int GU) { return GU == 1 ? 4 : GU == 2 ? 3 : 2; }
+constexpr int max_uw(int GU, int M) { return M > 16 ? (GU == 4 ? 1 : 2) : GU == 1 ? 4 : GU == 2 ? 3 : 2; }
 struct GemvPlan {
   int S, uw, nb;
 };
 GemvPlan plan_gemv(int M, int NT, int KT, int GU) {
   GemvPlan best{1, 1, 1};
   double least = -1.0;
-  for (int S = (KT + kW * max_uw(GU) - 1) / (kW * max_uw(GU)); S <= std::min(KT, 256); ++S) {
+  for (int S = (KT + kW * max_uw(GU, M) - 1) / (kW * max_uw(GU, M)); S <= std::min(KT, 256); ++S) {
     GemvPlan p;
     p.S = S;
     p.uw = ((KT + S - 1) / S + kW - 1) / kW;
     p.nb = S > 1 ? std::min(NT, 256 / S) : std::max(std::min(NT, 256), (NT + kMaxTiles - 1) / kMaxTiles);
-    const double c = ((NT + p.nb - 1) / p.nb) * (0.45 + 0.32 * p.uw + 0.034 * p.uw * (GU - 1)) + 0.88 * p.uw +
-                     0.0062 * M * KT / S + (S > 1 ? 2.76 + (double)S * M * NT * 128.0 / 4.2e6 : 0.0);
+    const int rows = (NT + p.nb - 1) / p.nb;
+    const double sums = (double)S * M * NT * 128.0, x = 0.006 * M * KT / S;
+    const double c = M <= 16 ? rows * (0.45 + 0.32 * p.uw + 0.034 * p.uw * (GU - 1)) + 0.88 * p.uw + x + (S > 1 ? 2.8 + sums / 4.2e6 : 0.0)
+                             : rows * (0.2 + 0.61 * p.uw + 0.08 * p.uw * (GU - 1)) + 0.54 * p.uw + x + (S > 1 ? 3.6 + sums / 5.4e6 : 0.0);
     if (least < 0.0 || c < least) {
       least = c;
       best = p;
@@ -349,21 +378,27 @@ GemvPlan plan_gemv(int M, int NT, int KT, int GU) {
   return best;
 }
 
-template <int UW, int GU>
+template <int UW, int GU, int MB>
 void launch_gemv(const Int4Args& a, int nb, hipStream_t s) {
-  if (a.S > 1) hipLaunchKernelGGL((int4_gemv_kernel<UW, GU, true>), dim3(nb * a.S), dim3(kW * 64), 0, s, a);
-  else hipLaunchKernelGGL((int4_gemv_kernel<UW, GU, false>), dim3(nb), dim3(kW * 64), 0, s, a);
+  if (a.S > 1) hipLaunchKernelGGL((int4_gemv_kernel<UW, GU, true, MB>), dim3(nb * a.S), dim3(kW * 64), 0, s, a);
+  else hipLaunchKernelGGL((int4_gemv_kernel<UW, GU, false, MB>), dim3(nb), dim3(kW * 64), 0, s, a);
 }
 template <int GU>
 void launch_gemv_uw(const GemvPlan& p, const Int4Args& a, hipStream_t s) {
-  if (p.uw == 1) return launch_gemv<1, GU>(a, p.nb, s);
+  if (a.M > 16) {
+    if constexpr (GU <= 2) {
+      if (p.uw == 2) return launch_gemv<2, GU, 2>(a, p.nb, s);
+    }
+    return launch_gemv<1, GU, 2>(a, p.nb, s);
+  }
+  if (p.uw == 1) return launch_gemv<1, GU, 1>(a, p.nb, s);
   if constexpr (GU <= 2) {
-    if (p.uw == 3) return launch_gemv<3, GU>(a, p.nb, s);
+    if (p.uw == 3) return launch_gemv<3, GU, 1>(a, p.nb, s);
   }
   if constexpr (GU == 1) {
-    if (p.uw == 4) return launch_gemv<4, GU>(a, p.nb, s);
+    if (p.uw == 4) return launch_gemv<4, GU, 1>(a, p.nb, s);
   }
-  launch_gemv<2, GU>(a, p.nb, s);
+  launch_gemv<2, GU, 1>(a, p.nb, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -622,7 +657,7 @@ extern "C" int64_t helm_int4_linear_workspace_bytes(int M, int N, int K, int gro
   if (M < 1 || N < 1 || K < 1 || N > (1 << 27) || K > (1 << 19)) return 0;
   if (group_size != 32 && group_size != 64 && group_size != 128) return 0;
   const int NT = (N + 15) / 16, KT = (K + 127) / 128;
-  const int S = M <= 16 ? plan_gemv(M, NT, KT, 128 / group_size).S : plan_gemm(M, NT, KT).S;
+  const int S = M <= kGemvTokens ? plan_gemv(M, NT, KT, 128 / group_size).S : plan_gemm(M, NT, KT).S;
   return S > 1 ? (int64_t)S * M * NT * 16 * (int64_t)sizeof(float) : 0;
 }
 
@@ -648,15 +683,15 @@ extern "C" int helm_int4_linear(const void* x, int64_t ldx, const void* qweight,
   a.M = M; a.N = N; a.K = K;
   a.NT = (N + 15) / 16; a.KT = (K + 127) / 128; a.np = a.NT * 16;
   const int GU = 128 / group_size;
-  const GemvPlan gp = M <= 16 ? plan_gemv(M, a.NT, a.KT, GU) : GemvPlan{};
-  const GemmPlan mp = M <= 16 ? GemmPlan{} : plan_gemm(M, a.NT, a.KT);
-  a.S = M <= 16 ? gp.S : mp.S;
+  const GemvPlan gp = M <= kGemvTokens ? plan_gemv(M, a.NT, a.KT, GU) : GemvPlan{};
+  const GemmPlan mp = M <= kGemvTokens ? GemmPlan{} : plan_gemm(M, a.NT, a.KT);
+  a.S = M <= kGemvTokens ? gp.S : mp.S;
   const int64_t need = a.S > 1 ? (int64_t)a.S * M * a.np * (int64_t)sizeof(float) : 0;
   HELM_CHECK_ARG(need == 0 || (workspace && helm::aligned16(workspace) && workspace_bytes >= need),
                  "helm_int4_linear: this shape needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
   a.part = static_cast<float*>(workspace);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (M <= 16) {
+  if (M <= kGemvTokens) {
     if (GU == 1) launch_gemv_uw<1>(gp, a, s);
     else if (GU == 2) launch_gemv_uw<2>(gp, a, s);
     else launch_gemv_uw<4>(gp, a, s);

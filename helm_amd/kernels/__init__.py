@@ -372,7 +372,7 @@ def int4_linear(input: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Te
     output and group of inputs) on the GPU, fp32 accumulate.
 
     input [..., K] fp16, weight an Int4Weight of [N, K], bias [N] fp16 or None.  Decode
-    (<= 16 tokens) scales each group's sum in fp32; above, the weights enter the product
+    (<= 32 tokens) scales each group's sum in fp32; above, the weights enter the product
     as fp16(code * scale)."""
     q = weight.qweight
     index = _native.gpu_of("int4_linear", input, q, bias, out)

@@ -236,3 +236,24 @@ def test_prompts_of_every_tile_height_and_slicing(cuda, m, n, k, gs):
     codes, scale = make(n, k, gs, m)
     x = torch.randn(m, k, generator=torch.Generator().manual_seed(n)).half().cuda()
     check(hk.int4_linear(x, hk.Int4Weight.pack(codes.cuda(), scale.cuda())), x, codes, scale, None, gs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gs", [32, 64, 128])
+@pytest.mark.parametrize("n,k", [(1, 128), (40, 640), (250, 1152), (4100, 2560), (4096, 12288), (17408, 5120)])
+def test_two_blocks_of_tokens(cuda, n, k, gs):
+    """17 to 32 tokens: the decode form's bound, and rows that do not depend on their neighbours."""
+    codes, scale = make(n, k, gs, n)
+    w = hk.Int4Weight.pack(codes.cuda(), scale.cuda())
+    x = torch.randn(32, k, generator=torch.Generator().manual_seed(k)).half().cuda()
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(5)).half().cuda()
+    s = scale.double().repeat_interleave(gs, 1)
+    for m in (17, 24, 31, 32):
+        y = hk.int4_linear(x[:m], w, bias)
+        e = x[:m].double().cpu() @ (codes.double() * s).t() + bias.double().cpu()
+        err = (y.double().cpu() - e).abs()
+        assert (err <= 2.0 ** -11 * e.abs() + 2.0 ** -25 + 32 * 2.0 ** -24 * 300 * (x[:m].double().cpu().abs() @ s.t())).all()
+    x[20] = float("nan")
+    bad = hk.int4_linear(x, w, bias)
+    keep = [i for i in range(32) if i != 20]
+    assert bad[20].isnan().all() and torch.equal(bad[keep], y[keep])
