@@ -5,8 +5,8 @@
 // its value (equal values, equal keys), so every filter is a border (key, how many of its
 // equals stay): no sort, and ties go to the lowest index.  Keys fall into 64 chunks of
 // 1024 neighbours.  Two kernels:
-//   * slices: a workgroup per 4096 logits groups them by chunk (key and index, largest
-//     chunk first) and sums count and weight of each chunk;
+//   * slices: a workgroup per 4096 logits lists their keys by chunk, the largest first, and sums
+//     count and weight of each chunk;
 //   * pick: a workgroup per row finds the chunk that holds a border from those sums and
 //     resolves the key inside it from the few logits of that chunk, then the slice that
 //     holds the drawn token, then the token.
@@ -56,7 +56,7 @@ struct SampleArgs {
   float t, p, lo;
   int k;
   SliceSums* sums;                    // [M][S]
-  uint32_t* list;                     // [M][S][kSlice]: key << 16 | index in the slice
+  uint16_t* list;                     // [M][S][kSlice]: keys, largest chunk first
   int64_t* out;
 };
 
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kST) void sample_slice_kernel(SampleArgs a, bool ve
   __shared__ uint32_t s_cnt[kChunks * kRep];
   __shared__ unsigned long long s_mass[kChunks * kRep];
   __shared__ uint32_t s_n;
-  __shared__ __attribute__((aligned(16))) uint32_t s_list[kSlice];
+  __shared__ __attribute__((aligned(16))) uint16_t s_list[kSlice];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int sl = blockIdx.x, m = blockIdx.y;
   const int i0 = sl * kSlice + tid * 8;               // this thread's logits
@@ -276,16 +276,16 @@ __global__ __launch_bounds__(kST) void sample_slice_kernel(SampleArgs a, bool ve
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     if (key[e] < least) continue;
-    s_list[s_cnt[(key[e] >> 10) * kRep + rep] + rank[e]] = key[e] << 16 | (uint32_t)(tid * 8 + e);
+    s_list[s_cnt[(key[e] >> 10) * kRep + rep] + rank[e]] = (uint16_t)key[e];
   }
   __syncthreads();
   // the list, and its weights: evaluated here, where every lane has a listed logit
   const int n = (int)s_n;
-  uint32_t* list = a.list + ((int64_t)m * a.S + sl) * kSlice;
-  for (int i = tid * 4; i < n; i += kST * 4)           // whole 16-byte pieces: the list has room
+  uint16_t* list = a.list + ((int64_t)m * a.S + sl) * kSlice;
+  for (int i = tid * 8; i < n; i += kST * 8)           // whole 16-byte pieces: the list has room
     *reinterpret_cast<uint4*>(list + i) = *reinterpret_cast<const uint4*>(&s_list[i]);
   for (int i = tid; i < n; i += kST) {
-    const uint32_t ki = s_list[i] >> 16;
+    const uint32_t ki = s_list[i];
     atomicAdd(&s_mass[(ki >> 10) * kRep + rep], (unsigned long long)(weight(ki, top, c, s_tab) * kFix + 0.5));
   }
   __syncthreads();
@@ -389,20 +389,20 @@ __global__ __launch_bounds__(kPT) void sample_pick_kernel(SampleArgs a, bool vec
   const uint32_t icnt = wave_scan(cc);
   const double imass = wave_scan(cm);
 
-  const uint32_t* list = a.list + (int64_t)m * S * kSlice;
+  const uint16_t* list = a.list + (int64_t)m * S * kSlice;
   uint32_t el[kOwn];                                   // first 64 entries of chunk `held` in the wave's slices
   int held = -1, uses = 0, turn = 0;
   // f(i, key) of the entries past the first 64 of a chunk (lane cl) in the wave's slices, kOwn
   // kDeep loads at a time
   auto rest = [&](int cl, auto f) {
     int n[kOwn], last[kOwn], most = 0;
-    const uint32_t* q[kOwn];
+    const uint16_t* q[kOwn];
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       n[i] = (int)lane_of(cnt[i], cl);
       q[i] = list + (int64_t)(wave + kPW * i) * kSlice + lane_of(off[i], cl);
       last[i] = max(n[i] - 1, 0);
-      if (wave + kPW * i >= S) q[i] = list;              // no such slice: nothing is read but in range
+      if (n[i] == 0) q[i] = list;                        // nothing is read but in range
       most = max(most, n[i]);
     }
     for (int j = 64 + lane; j - lane < most; j += 64 * kDeep) {
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(kPT) void sample_pick_kernel(SampleArgs a, bool vec
       for (int i = 0; i < kOwn; ++i)
 #pragma unroll
         for (int d = 0; d < kDeep; ++d)
-          if (j + 64 * d < n[i]) f(i, v[i][d] >> 16);
+          if (j + 64 * d < n[i]) f(i, v[i][d]);
     }
   };
   // Number of this thread's key (1023 - tid of the chunk of lane cl), from the listed logits
@@ -425,13 +425,13 @@ __global__ __launch_bounds__(kPT) void sample_pick_kernel(SampleArgs a, bool vec
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int n = (int)lane_of(cnt[i], cl);
-      const uint32_t* p = list + (int64_t)(wave + kPW * i) * kSlice + lane_of(off[i], cl);
+      const uint16_t* p = list + (int64_t)(wave + kPW * i) * kSlice + lane_of(off[i], cl);
       el[i] = lane < n ? p[lane] : 0u;
     }
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
       const int n = (int)lane_of(cnt[i], cl);
-      if (lane < n) atomicAdd(&hist[(el[i] >> 16) & 1023u], 1u);
+      if (lane < n) atomicAdd(&hist[el[i] & 1023u], 1u);
     }
     rest(cl, [&](int, uint32_t key) { atomicAdd(&hist[key & 1023u], 1u); });
     __syncthreads();
@@ -535,7 +535,7 @@ __global__ __launch_bounds__(kPT) void sample_pick_kernel(SampleArgs a, bool vec
   for (int i = 0; i < kOwn; ++i) {
     const int n = (int)lane_of(cnt[i], bl);
     if (held != bl) {
-      const uint32_t* q = list + (int64_t)(wave + kPW * i) * kSlice + lane_of(off[i], bl);
+      const uint16_t* q = list + (int64_t)(wave + kPW * i) * kSlice + lane_of(off[i], bl);
       el[i] = lane < n ? q[lane] : 0u;
     }
   }
@@ -550,7 +550,7 @@ __global__ __launch_bounds__(kPT) void sample_pick_kernel(SampleArgs a, bool vec
   for (int i = 0; i < kOwn; ++i) {
     ms[i] = lane < bl ? mass[i] : 0.0;
     tie[i] = 0;
-    if (lane < (int)lane_of(cnt[i], bl)) count(i, el[i] >> 16);
+    if (lane < (int)lane_of(cnt[i], bl)) count(i, el[i]);
   }
   rest(bl, count);
 #pragma unroll
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(kPT) void sample_pick_kernel(SampleArgs a, bool vec
 
 extern "C" int64_t helm_sample_workspace_bytes(int M, int N) {
   if (M < 1 || N < 1) return 0;
-  return (int64_t)M * ((N + (int64_t)kSlice - 1) / kSlice) * (int64_t)(sizeof(SliceSums) + kSlice * 4);
+  return (int64_t)M * ((N + (int64_t)kSlice - 1) / kSlice) * (int64_t)(sizeof(SliceSums) + kSlice * 2);
 }
 
 extern "C" int helm_sample(const void* x, int64_t ldx, int M, int N, const float* u, const float* temperature,
@@ -646,7 +646,7 @@ extern "C" int helm_sample(const void* x, int64_t ldx, int M, int N, const float
   a.t = t; a.k = k; a.p = p; a.lo = lo;
   static_assert(sizeof(SliceSums) % 16 == 0, "the lists follow 16-byte aligned");
   a.sums = static_cast<SliceSums*>(workspace);
-  a.list = reinterpret_cast<uint32_t*>(a.sums + (int64_t)M * a.S);
+  a.list = reinterpret_cast<uint16_t*>(a.sums + (int64_t)M * a.S);
   a.out = out;
   const bool vec = helm::aligned16(x) && ldx % 8 == 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -204,3 +204,13 @@ def test_captured_graph_replays(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, eager[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k,p,lo", [(0, 0.999, 0.0), (40000, 1.0, 0.0), (50000, 0.99, 0.001)])
+def test_a_full_slice_without_the_border_s_chunk(cuda, k, p, lo):
+    """Slices of 4096 logits of which the last holds only numbers above the border's range."""
+    n = 17 * 4096
+    x = logits(3, n, 21).clamp_(-7.5, 7.5)
+    x[:, 16 * 4096:] = (8.0 + torch.rand(4096, generator=torch.Generator().manual_seed(3)) * 0.5).half().cuda()
+    check(x, np.array([0.1, 0.9, 0.9995], np.float32), 2.0, k, p, lo)
