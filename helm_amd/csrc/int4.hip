@@ -50,7 +50,6 @@ __device__ __forceinline__ void wait_vm() {
 __device__ __forceinline__ void wait_vm_n(int n) {      // n: a constant once inlined
   asm volatile("" ::: "memory");
   switch (n) {
-    case 3: __builtin_amdgcn_s_waitcnt(3 | (7 << 4) | (15 << 8)); break;
     case 4: __builtin_amdgcn_s_waitcnt(4 | (7 << 4) | (15 << 8)); break;
     case 5: __builtin_amdgcn_s_waitcnt(5 | (7 << 4) | (15 << 8)); break;
     case 6: __builtin_amdgcn_s_waitcnt(6 | (7 << 4) | (15 << 8)); break;
