@@ -483,7 +483,7 @@ def paged_decode_attention_q8(q: torch.Tensor, pool: Q8PoolView, page_table: tor
     pts, pcs = page_table.stride()
     if pcs != 1 and max_pages > 1:
         raise RuntimeError(f"{what}: page_table must be int32 [B, max_pages], row-major")
-    if seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or seq_lens.shape[0] != B or not seq_lens.is_contiguous():
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,) or not seq_lens.is_contiguous():
         raise RuntimeError(f"{what}: seq_lens must be int32 [B], contiguous")
     if out is None:
         out = q.new_empty((B, Hq, D))
@@ -511,7 +511,7 @@ def paged_decode_attention_q8(q: torch.Tensor, pool: Q8PoolView, page_table: tor
 
 def _check_places(what: str, slots: torch.Tensor, offsets: torch.Tensor, n: int) -> None:
     for name, t in (("slots", slots), ("offsets", offsets)):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
             raise RuntimeError(f"{what}: {name} must be int32 [{n}], contiguous")
 
 
@@ -550,12 +550,12 @@ def dequantize_pages(pool: Q8PoolView, pages: torch.Tensor) -> PoolView:
         raise RuntimeError(f"{what}: pages must be a contiguous int32 vector")
     n = pages.shape[0]
     Hkv, P, D = pool.num_kv_heads, pool.page_size, pool.head_dim
+    page = Hkv * P * D
     k = pool.k_scale.new_empty((n, Hkv, P, D))
-    v = pool.v_scale.new_empty((n, Hkv, D, P)).transpose(2, 3)
+    v = k.new_empty_strided((n, Hkv, P, D), (page, P * D, 1, P))
     if n:
         _native.call_on(index, "helm_dequantize_pages", pool.c_ref(), pages.data_ptr(), n, k.data_ptr(), v.data_ptr(),
                         Hkv, D, P, _native.raw_stream(index))
-    page = Hkv * P * D
     return PoolView(k, v, page, P * D, page, P * D, P, n, Hkv)
 
 

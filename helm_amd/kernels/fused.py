@@ -161,17 +161,15 @@ def qk_norm_rope_append_q8(qkv: torch.Tensor, q_norm_w: Optional[torch.Tensor],
         raise RuntimeError(f"{what}: {Hkv} heads of {D} do not fit the pool's {pool.num_kv_heads} of {pool.head_dim}")
     P = pool._check_page_size(page_size, what)
     B, width = qkv.shape
-    if (positions.dtype != torch.int32 or positions.dim() != 1 or positions.shape[0] != B
-            or not positions.is_contiguous()):
+    if positions.dtype != torch.int32 or positions.shape != (B,) or not positions.is_contiguous():
         raise RuntimeError(f"{what}: positions must be int32 [{B}], contiguous")
     _check_places(what, slots, offsets, B)
-    if (inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or inv_freq.shape[0] != D // 2
-            or not inv_freq.is_contiguous()):
+    if inv_freq.dtype != torch.float32 or inv_freq.shape != (D // 2,) or not inv_freq.is_contiguous():
         raise RuntimeError(f"{what}: inv_freq must be fp32 [{D // 2}], contiguous")
     if (q_norm_w is None) != (k_norm_w is None):
         raise RuntimeError(f"{what}: give both q / k norm weights or neither")
     for w in (q_norm_w, k_norm_w):
-        if w is not None and (w.dim() != 1 or w.shape[0] != D or not w.is_contiguous()):
+        if w is not None and (w.shape != (D,) or not w.is_contiguous()):
             raise RuntimeError(f"{what}: norm weights must be [D], contiguous")
     if q_out is None:
         q_out = qkv.new_empty((B, Hq, D))
