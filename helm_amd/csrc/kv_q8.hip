@@ -100,7 +100,8 @@ __device__ __forceinline__ void rope_factors(int pos, float inv_freq, float& c, 
 }
 
 // One wave per (token, head): q and k heads normed and rotated, q to q_out, k and v
-// quantised into their page.  Latency-bound at a few tokens.
+// quantised into their page.  Latency-bound at a few tokens: 3.6 us for 1 to 32 tokens of 40 + 8 + 8
+// heads of 128.
 template <int D>
 __global__ __launch_bounds__(256) void qk_norm_rope_append_q8_kernel(
     const uint16_t* __restrict__ qkv, int64_t qkv_sb, const uint16_t* __restrict__ q_norm_w,
@@ -381,7 +382,9 @@ __global__ __launch_bounds__(kPW * 64, 8) void qk_norm_rope_append_q8_prompt_ker
   }
 }
 
-// One wave per (item, kv head, token, K or V).
+// One wave per (item, kv head, token, K or V).  Latency-bound at a token per item (4.0 us, 16
+// items of 8 heads of 128); V's codes are a byte store each, P apart: 256 items of 16 tokens take
+// 24 us, a copy of their bytes 11.
 template <int D>
 __global__ __launch_bounds__(256) void kv_append_q8_kernel(const uint16_t* __restrict__ k_new,
                                                            const uint16_t* __restrict__ v_new, Q8Pool pool,
@@ -406,7 +409,8 @@ __global__ __launch_bounds__(256) void kv_append_q8_kernel(const uint16_t* __res
   store_row<D>(x, lane, is_v, pool, slot, (int)(bh - b * Hkv), (int)off, P);
 }
 
-// One thread per 16 codes: of a K token's dims, or of a V dim's tokens.
+// One thread per 16 codes: of a K token's dims, or of a V dim's tokens.  Bound by HBM: 2048 pages
+// of 8 heads, 16 tokens, D 128 (202 MB read and written) in 35 us, 5.8 TB/s; 16 pages in 4.5.
 __global__ __launch_bounds__(256) void dequantize_pages_kernel(Q8Pool pool, const int32_t* __restrict__ pages,
                                                                int64_t pieces, int Hkv, int D, int P,
                                                                uint16_t* __restrict__ k_out,

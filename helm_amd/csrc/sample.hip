@@ -17,7 +17,10 @@
 // Bound by latency: the logits are read once by as many CUs as there are slices; then a
 // row has four dependent round trips to memory (sums, the border's chunk, the slice's
 // borders, its logits) and a scan after each.  Scans run over DPP, and every wave repeats
-// the small ones for itself instead of waiting at a barrier for another.
+// the small ones for itself instead of waiting at a barrier for another.  A row of 151936 with
+// top-k 20 and top-p 0.8 takes 16 us (5 of them the slices); 16 rows without filters 19, with
+// top-p alone 31 (every logit is listed, and the border's chunk holds a third of them); 64 rows of
+// 50257 with min-p 20.
 #include "helm_common.h"
 
 namespace {
