@@ -467,3 +467,28 @@ def test_prompt_attends_dequantised_pages(cuda):
         k, _ = held(pool)
         move = 2.0 ** -11 * float(q[i].double().norm(dim=-1).max() * k.norm(dim=-1).max()) / math.sqrt(d)
         assert ((o[i].cpu().double() - e[0]).abs() <= (2 * move + 3 * 2.0 ** -11) * top[0] + 2.0 ** -11 * e[0].abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hkv,p,d", [(3, 16, 128), (2, 64, 64)])
+@pytest.mark.parametrize("n_tok", [1, 2, 3, 4, 6, 9, 16])
+def test_kv_append_at_every_place_of_a_word(cuda, hkv, p, d, n_tok):
+    """n_tok tokens from every offset, before and past the page too."""
+    offs = torch.arange(-5, p + 2, dtype=torch.int32)
+    n = len(offs)
+    g = torch.Generator().manual_seed(n_tok)
+    k, v = (torch.randn(n, hkv, n_tok, d, generator=g).half() for _ in range(2))
+    pool = random_pool(n, hkv, p, d, 6)
+    want = [t.cpu().clone() for t in (pool.k, pool.v, pool.k_scale, pool.v_scale)]
+    slots = torch.randperm(n, generator=g).int()
+    ka.kv_append_q8(k.cuda(), v.cuda(), pool, slots.cuda(), offs.cuda(), p)
+    for b in range(n):
+        for t in range(n_tok):
+            at = int(offs[b]) + t
+            if 0 <= at < p:
+                for i, x in ((0, k), (1, v)):
+                    c, s = quantised(x[b, :, t])
+                    want[i][slots[b], :, at] = c
+                    want[2 + i][slots[b], :, at] = s
+    for got, w in zip((pool.k, pool.v, pool.k_scale, pool.v_scale), want):
+        assert torch.equal(got.cpu(), w)
