@@ -519,6 +519,7 @@ __global__ __launch_bounds__(kGThreads, RI <= 4 ? 3 : 2) void int4_gemm_kernel(I
   auto step = [&](const BBuf& b, int kb, auto half_c, auto more_c) {
     constexpr int half = decltype(half_c)::value;
     // x of step kb landed: newer are the next step's copies and, with `more`, one tile's weights
+    // (each of load's TN (1 + SG) loads is an instruction: apart by more than any may join)
     if (kb + 1 < nk) wait_vm<kCopies + (decltype(more_c)::value ? TN * (1 + SG) : 0)>();
     else wait_vm<0>();
     lds_read_barrier();
