@@ -258,6 +258,7 @@ class AttnWorkspace:
     def __init__(self, device: torch.device):
         self.device = device
         self.buf = torch.empty(0, dtype=torch.float32, device=device)
+        self._outgrown = []
 
     def get(self, B: int, Hq: int, D: int, total_splits: int):
         n_o = B * Hq * total_splits * D
@@ -267,9 +268,12 @@ class AttnWorkspace:
         return self.buf[:n_o], self.buf[n_o:n]
 
     def reserve(self, index: int, nbytes: int) -> int:
-        """Address of at least `nbytes`, for a call on GPU `index`."""
+        """Address of at least `nbytes`, for a call on GPU `index`.  What the workspace has
+        outgrown stays (a captured call goes on using its address); it grows twofold at least, so
+        that this is no more than it holds."""
         if self.buf.numel() * 4 < nbytes:
-            self.buf = torch.empty(-(-nbytes // 4), dtype=torch.float32, device=self.device)
+            self._outgrown.append(self.buf)
+            self.buf = torch.empty(max(-(-nbytes // 4), 2 * self.buf.numel()), dtype=torch.float32, device=self.device)
         if self.buf.get_device() != index:
             raise RuntimeError(f"AttnWorkspace: on {self.buf.device}, the call on GPU {index}")
         return self.buf.data_ptr()

@@ -492,3 +492,40 @@ def test_kv_append_at_every_place_of_a_word(cuda, hkv, p, d, n_tok):
                     want[2 + i][slots[b], :, at] = s
     for got, w in zip((pool.k, pool.v, pool.k_scale, pool.v_scale), want):
         assert torch.equal(got.cpu(), w)
+
+
+def test_a_workspace_keeps_what_it_has_outgrown():
+    ws = ka.AttnWorkspace(torch.device("cpu"))
+    first = ws.reserve(-1, 1000)
+    ws.buf.fill_(5.0)
+    assert ws.reserve(-1, 900) == first
+    sizes = []
+    for n in (1004, 1100, 5000):
+        ws.reserve(-1, n)
+        assert ws.buf.nbytes >= n
+        sizes.append(ws.buf.nbytes)
+    assert sizes == [2000, 2000, 5000]
+    assert [t.data_ptr() for t in ws._outgrown if t.numel()][0] == first and (ws._outgrown[1] == 5.0).all()
+
+
+@pytest.mark.gpu
+def test_a_captured_call_outlives_its_workspace_s_growth(cuda):
+    g = torch.Generator().manual_seed(14)
+    pool = random_pool(64, 8, 16, 128, 15)
+    ws = ka.AttnWorkspace(torch.device("cuda", 0))
+    q = torch.randn(1, 32, 128, generator=g).half().cuda()
+    table = torch.randperm(64, generator=g).int().view(1, 64).cuda()
+    lens = torch.tensor([1000], dtype=torch.int32, device=cuda)
+    want = ka.paged_decode_attention_q8(q, pool, table, lens, num_splits=8, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ka.paged_decode_attention_q8(q, pool, table, lens, num_splits=8, workspace=ws)
+    many = q.expand(9, 32, 128).contiguous()
+    for n in (3, 9):                                     # the workspace grows; others take what is free
+        ka.paged_decode_attention_q8(many[:n], pool, table.expand(n, 64).contiguous(), lens.expand(n).contiguous(),
+                                     num_splits=16, workspace=ws)
+        others = [torch.full((1 << 18,), float(n), device=cuda) for _ in range(8)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all((t == float(n)).all() for t in others)
