@@ -412,7 +412,7 @@ void launch_gemv_uw(const GemvPlan& p, const Int4Args& a, hipStream_t s) {
 // (waiting for those too, as they had just been requested, took 183 us instead of 160 for 1500 x
 // 4096 -> 12288, now 940 TFLOP/s; 2048 x 4096 -> 4096 reaches 985).  A weight enters the products as
 // fp16(code * scale), the number that Int4Weight.dequantize() gives rounded to fp16: one
-// rounding of 2^-12 relative at most, and it spares a scaling of every accumulator
+// rounding of 2^-11 relative at most, and it spares a scaling of every accumulator
 // per group.
 constexpr int kGThreads = 256;
 constexpr int kStages = 3;
