@@ -257,3 +257,18 @@ def test_two_blocks_of_tokens(cuda, n, k, gs):
     bad = hk.int4_linear(x, w, bias)
     keep = [i for i in range(32) if i != 20]
     assert bad[20].isnan().all() and torch.equal(bad[keep], y[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 20, 40])
+def test_weights_past_32_bits_of_bytes(cuda, m):
+    """4.3 GB of codes: the last outputs against the product with their own tiles."""
+    nt, kt = 16384, 256
+    q = torch.randint(-2 ** 31, 2 ** 31 - 1, (nt, kt, 64, 4), dtype=torch.int32, device=cuda)
+    s = ((0.5 + torch.rand(nt, kt, 1, 16, device=cuda)) * 0.006).half()
+    w = hk.Int4Weight(q, s, nt * 16, kt * 128, 128)
+    x = torch.randn(m, kt * 128, generator=torch.Generator().manual_seed(m)).half().cuda()
+    y = hk.int4_linear(x, w)
+    for first in (0, nt // 2, nt - 2):
+        codes, scale = hk.Int4Weight(q[first:first + 2].clone(), s[first:first + 2].clone(), 32, kt * 128, 128).unpack()
+        check(y[:, first * 16:first * 16 + 32], x, codes, scale, None, 128)

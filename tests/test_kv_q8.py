@@ -529,3 +529,27 @@ def test_a_captured_call_outlives_its_workspace_s_growth(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and all((t == float(n)).all() for t in others)
+
+
+@pytest.mark.gpu
+def test_a_pool_past_32_bits_of_elements(cuda):
+    """Pages whose first element lies past 2^32: writes, attention and the way back, as in a small pool."""
+    n, hkv, p, d = 270000, 8, 16, 128
+    big, small = ka.alloc_q8_pool(n, hkv, p, d, cuda), ka.alloc_q8_pool(30, hkv, p, d, cuda)
+    g = torch.Generator().manual_seed(2)
+    qkv = torch.randn(400, (32 + 2 * hkv) * d, generator=g).half().cuda()
+    inv = (1e6 ** (-torch.arange(0, d, 2).double() / d)).float().cuda()
+    pos = torch.arange(400, dtype=torch.int32, device=cuda)
+    order = torch.randperm(25, generator=g).int().cuda()
+    outs = []
+    for pool, base in ((big, n - 25), (small, 3)):
+        slots = order[(pos // p).long()] + base
+        q = torch.cat([fused.qk_norm_rope_append_q8(qkv[a:b], None, None, EPS, pos[a:b], inv, None, pool, slots[a:b],
+                                                    pos[a:b] % p, 32, hkv, d) for a, b in ((0, 10), (10, 390))])
+        kv = qkv[390:].view(10, 48, d)[:, 32:].unsqueeze(2)
+        ka.kv_append_q8(kv[:, :hkv], kv[:, hkv:], pool, slots[390:], pos[390:] % p)
+        o = ka.paged_decode_attention_q8(q[-1:], pool, (order + base)[None], torch.tensor([400], dtype=torch.int32, device=cuda))
+        view = ka.dequantize_pages(pool, order + base)
+        outs.append((q, o, view.k, view.v))
+    assert all(torch.equal(a, b) for a, b in zip(*outs)) and outs[0][1].any()
+    assert not big.k[:n - 25].any() and not big.v[:1000].any()
