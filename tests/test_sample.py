@@ -214,3 +214,14 @@ def test_a_full_slice_without_the_border_s_chunk(cuda, k, p, lo):
     x = logits(3, n, 21).clamp_(-7.5, 7.5)
     x[:, 16 * 4096:] = (8.0 + torch.rand(4096, generator=torch.Generator().manual_seed(3)) * 0.5).half().cuda()
     check(x, np.array([0.1, 0.9, 0.9995], np.float32), 2.0, k, p, lo)
+
+
+@pytest.mark.gpu
+def test_the_largest_rows(cuda):
+    n = 64 * 4096
+    x = logits(4, n, 31)
+    x[3] = 0.5                                           # ties alone
+    check(x, np.float32([0.3, 0.999, 0.5, 0.25]), np.float32([1.0, 0.7, 1.5, 1.0]), [0, 64, 70000, 5000],
+          np.float32([0.95, 1.0, 0.999, 1.0]), np.float32([0.0, 0.0, 0.001, 0.5]), exact_ties=True)
+    with pytest.raises(RuntimeError, match="262144"):
+        fused.sample(logits(1, n + 1, 3), torch.zeros(1, device=cuda))
