@@ -40,6 +40,20 @@ struct Unpack {
   }
 };
 
+// Word of eight codes as fp16 (b + u - b - 8, exact).
+__device__ __forceinline__ h8_t word_codes(const Unpack& unpack, uint32_t w) {
+  const h2_t off0 = {(_Float16)-264.0f, (_Float16)-264.0f}, off1 = {(_Float16)-24.0f, (_Float16)-24.0f};
+  const u32x4_t p = unpack(w);
+  h8_t r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const h2_t v = __builtin_bit_cast(h2_t, (uint32_t)p[i]) + (i & 1 ? off1 : off0);
+    r[2 * i] = v[0];
+    r[2 * i + 1] = v[1];
+  }
+  return r;
+}
+
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   static_assert(N >= 0 && N < 64, "vmcnt range");
@@ -404,48 +418,28 @@ void launch_gemv_uw(const GemvPlan& p, const Int4Args& a, hipStream_t s) {
 // Prompts
 // ---------------------------------------------------------------------------
 // A 256-thread workgroup computes 16 RI rows x 128 outputs.  Wave (kh, side) owns the
-// 64 outputs of its side over half kh of the inputs, so that every weight is turned
-// into fp16 by one wave only; the halves are added through LDS at the end.  x goes
-// global -> LDS (16-byte copies, XOR-swizzled, a ring of three 64-input steps), the
-// weights straight into registers, one tile ahead (three at 32 rows).  Copies and loads share one
-// counter: a step waits for its x by the number of what was requested later, weights included
-// (waiting for those too, as they had just been requested, took 183 us instead of 160 for 1500 x
-// 4096 -> 12288, now 940 TFLOP/s; 2048 x 4096 -> 4096 reaches 985).  A weight enters the products as
-// fp16(code * scale), the number that Int4Weight.dequantize() gives rounded to fp16: one
-// rounding of 2^-11 relative at most, and it spares a scaling of every accumulator
-// per group.
+// 64 outputs of its side over half kh of the inputs, so that every weight is unpacked
+// by one wave only; the halves are added through LDS at the end.  A step is a tile of 128
+// inputs: x goes global -> LDS (16-byte copies, XOR-swizzled, two stages), the weights straight into
+// registers, both one step ahead.  A step begins by waiting for all of them: copies in assembly and
+// loads that the compiler places cannot be told apart by number.
+// The products run on the codes, exact in fp16, and the sums of 64 inputs (32 in groups of 32)
+// are scaled in fp32: a fused multiply-add per accumulator, where weights of fp16(code * scale)
+// would need none but be off by 2^-11 each, and infinite for scales above 8188.
 constexpr int kGThreads = 256;
-constexpr int kStages = 3;
-__device__ __forceinline__ int aswz(int r) { return (r >> 1) & 7; }   // 128-byte rows
+__device__ __forceinline__ int aswz(int r) { return r & 15; }         // 256-byte rows
 
 __device__ __forceinline__ void lds_read_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// Word of eight codes times a scale, each product rounded to fp16 once (b + u - b - 8 is
-// exact).
-__device__ __forceinline__ h8_t word_scaled(const Unpack& unpack, uint32_t w, h2_t s) {
-  const h2_t off0 = {(_Float16)-264.0f, (_Float16)-264.0f}, off1 = {(_Float16)-24.0f, (_Float16)-24.0f};
-  const u32x4_t p = unpack(w);
-  h8_t r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const h2_t v = (__builtin_bit_cast(h2_t, (uint32_t)p[i]) + (i & 1 ? off1 : off0)) * s;
-    r[2 * i] = v[0];
-    r[2 * i + 1] = v[1];
-  }
-  return r;
-}
-
 template <int RI, int GU, bool PART>
-__global__ __launch_bounds__(kGThreads, RI <= 4 ? 3 : 2) void int4_gemm_kernel(Int4Args a) {
+__global__ __launch_bounds__(kGThreads, RI <= 4 && (RI == 2 || GU < 4) ? 3 : 2) void int4_gemm_kernel(Int4Args a) {
   constexpr int TN = 4;
-  constexpr int NB = RI == 2 ? 4 : 2;  // tiles of weights on the way or in use
-  constexpr int kStageBytes = 16 * RI * 128;
-  constexpr int kCopies = kStageBytes / 1024 / 4 > 0 ? kStageBytes / 1024 / 4 : 1;   // per wave and step
-  constexpr int kRing = kStages * kStageBytes;
+  constexpr int kStageBytes = 16 * RI * 256;
+  constexpr int kCopies = kStageBytes / 1024 / 4;       // per wave and step
   constexpr int kRed = 4 * (RI / 2) * TN * 1024;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[kRing > kRed ? kRing : kRed];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStageBytes > kRed ? 2 * kStageBytes : kRed];
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -459,30 +453,30 @@ __global__ __launch_bounds__(kGThreads, RI <= 4 ? 3 : 2) void int4_gemm_kernel(I
   // this workgroup's 128-input tiles
   const int kt0 = PART ? (int)((int64_t)a.KT * blockIdx.z / gridDim.z) : 0;
   const int kt1 = PART ? (int)((int64_t)a.KT * (blockIdx.z + 1) / gridDim.z) : a.KT;
-  const int nk = 2 * (kt1 - kt0);      // steps: two per tile
 
-  // Step s of a tile holds inputs 32 s .. + 32 and 64 + 32 s .. + 32 of its 128 (chunks
-  // 0-3 and 4-7 of a row: the two waves' halves), chunk g of row r in slot g ^ aswz(r).
-  // Rows past M read the last row, inputs past K the row's last chunk (weights there are
-  // zero).
-  uint32_t arow[kCopies];               // bytes from row m0 (ldx is below 2^23)
-  int akc[kCopies];
-#pragma unroll
-  for (int i = 0; i < kCopies; ++i) {
-    const int c = (wave * kCopies + i) * 64 + lane;
-    const int r = c >> 3;
-    const int g = (c & 7) ^ aswz(r);
-    arow[i] = (uint32_t)min(r, M - 1 - m0) * (uint32_t)(a.ldx * 2);
-    akc[i] = (g >> 2) * 64 + (g & 3) * 8;
-  }
+  // 16-byte chunk g of row r of a tile lies in slot g ^ aswz(r).  Rows past M read the last row.
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)smem;
-  const void* xbase = uniform(a.x + (int64_t)m0 * a.ldx);
-  auto copy = [&](int kb) {
-    const uint32_t base = lds0 + (kb % kStages) * kStageBytes;
-    const int k0 = (kt0 + (kb >> 1)) * 128 + (kb & 1) * 32;
+  const uint8_t* xbase = static_cast<const uint8_t*>(uniform(a.x + (int64_t)m0 * a.ldx));
+  // slot c of the stage: its chunk's bytes from row m0, tile 0 (ldx is below 2^23)
+  auto chunk = [&](int c) { return (c & 15) ^ aswz(c >> 4); };
+  auto offset = [&](int c) { return (uint32_t)min(c >> 4, M - 1 - m0) * (uint32_t)(a.ldx * 2) + chunk(c) * 16; };
+  uint32_t aoff[kCopies];
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i)
-      copy_to_lds(xbase, arow[i] + 2 * min(k0 + akc[i], K - 8), base + (wave * kCopies + i) * 1024);
+  for (int i = 0; i < kCopies; ++i) aoff[i] = offset((wave * kCopies + i) * 64 + lane);
+  auto copy = [&](int kt, int stage) {
+    const uint32_t base = lds0 + stage * kStageBytes + wave * kCopies * 1024;
+    const uint8_t* xb = xbase + (int64_t)kt * 256;
+    if ((kt + 1) * 128 <= K) {
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) copy_to_lds(xb, aoff[i], base + i * 1024);
+      return;
+    }
+    // K ends inside the tile: chunks past it read the row's last one (weights there are zero)
+    int c = wave * kCopies * 64 + lane;
+    asm volatile("" : "+v"(c));         // (nothing of this is kept in registers around the loop)
+#pragma unroll 1
+    for (int i = 0; i < kCopies; ++i, c += 64)
+      copy_to_lds(xb, offset(c) - 2 * max(kt * 128 + chunk(c) * 8 - (K - 8), 0), base + i * 1024);
   };
 
   // a tile's weights of this wave: words 2 kh, 2 kh + 1 and their scales
@@ -490,7 +484,7 @@ __global__ __launch_bounds__(kGThreads, RI <= 4 ? 3 : 2) void int4_gemm_kernel(I
   typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
   struct BBuf {
     u32x2_t w[TN];
-    uint32_t s[TN][SG];
+    uint16_t s[TN][SG];
   };
   // (buffer loads: offsets of a tile are scalar)
   const int ntb = min(nt0, a.NT - 1), tiles = min(TN, a.NT - ntb) * a.KT;
@@ -502,7 +496,7 @@ __global__ __launch_bounds__(kGThreads, RI <= 4 ? 3 : 2) void int4_gemm_kernel(I
   auto load = [&](BBuf& b, int kt) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int tile = (min(nt0 + j, a.NT - 1) - ntb) * a.KT + min(kt, kt1 - 1);
+      const int tile = (min(nt0 + j, a.NT - 1) - ntb) * a.KT + kt;
       b.w[j] = __builtin_amdgcn_raw_buffer_load_b64(wrsrc, wv, tile * 1024, 0);
 #pragma unroll
       for (int g = 0; g < SG; ++g) b.s[j][g] = __builtin_amdgcn_raw_buffer_load_b16(srsrc, sv + 32 * g, tile * (GU * 32), 0);
@@ -516,59 +510,75 @@ __global__ __launch_bounds__(kGThreads, RI <= 4 ? 3 : 2) void int4_gemm_kernel(I
     for (int j = 0; j < TN; ++j) acc[i][j] = f4_t{0.f, 0.f, 0.f, 0.f};
 
   const Unpack unpack;
-  auto step = [&](const BBuf& b, int kb, auto half_c, auto more_c) {
-    constexpr int half = decltype(half_c)::value;
-    // x of step kb landed: newer are the next step's copies and, with `more`, one tile's weights
-    // (each of load's TN (1 + SG) loads is an instruction: apart by more than any may join)
-    if (kb + 1 < nk) wait_vm<kCopies + (decltype(more_c)::value ? TN * (1 + SG) : 0)>();
-    else wait_vm<0>();
+  // Tile kt from `stage` and b; the next one's requests go out as soon as their places are free:
+  // every wave has read the other stage before it came to the barrier.
+  BBuf b;
+  auto tile = [&](int kt, int stage) {
+    const uint8_t* As = smem + stage * kStageBytes;
+    wait_vm<0>();
     lds_read_barrier();
-    if (kb + 2 < nk) copy(kb + 2);
-    const uint8_t* As = smem + (kb % kStages) * kStageBytes;
-    h8_t bf[TN];
+    if (kt + 1 < kt1) copy(kt + 1, 1 - stage);
+    h8_t bf[2][TN];
+    float sc[SG][TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const _Float16 s1 = __builtin_bit_cast(_Float16, (uint16_t)b.s[j][SG == 2 ? half : 0]);
-      bf[j] = word_scaled(unpack, half ? b.w[j][1] : b.w[j][0], h2_t{s1, s1});
-    }
 #pragma unroll
-    for (int i = 0; i < RI; ++i) {
+      for (int h = 0; h < 2; ++h) bf[h][j] = word_codes(unpack, b.w[j][h]);
+#pragma unroll
+      for (int g = 0; g < SG; ++g) sc[g][j] = h2f(b.s[j][g]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (kt + 1 < kt1) load(b, kt + 1);
+    // Operands of row tile i + 1 are read, and the sums of the one before are scaled, beside the products
+    // of i; a barrier of the schedule after each keeps no more than that in registers.
+    auto rows = [&](int i, int h) {
       const int r = 16 * i + col;
-      const h8_t af = *reinterpret_cast<const h8_t*>(As + r * 128 + (((4 * kh + grp) ^ aswz(r)) << 4));
+      return *reinterpret_cast<const h8_t*>(As + r * 256 + (((8 * kh + 4 * h + grp) ^ aswz(r)) << 4));
+    };
+    constexpr bool kAhead = RI != 4;    // (three workgroups a CU leave no registers for it)
+    h8_t af[2], nf[2];
+    if (kAhead) {
+      nf[0] = rows(0, 0);
+      nf[1] = rows(0, 1);
+    }
+    f4_t last[TN];
+    auto scaled = [&](int s) {          // sum s: row tile s / SG, scale s % SG
 #pragma unroll
       for (int j = 0; j < TN; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af, bf[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          acc[s / SG][j][q] = fmaf(sc[s % SG][j], last[j][q], acc[s / SG][j][q]);
+    };
+#pragma unroll
+    for (int s = 0; s < RI * SG; ++s) {
+      const int i = s / SG;
+      if (s % SG == 0) {
+        af[0] = kAhead ? nf[0] : rows(i, 0);
+        af[1] = kAhead ? nf[1] : rows(i, 1);
+      }
+      if (kAhead && s % SG == 0 && i + 1 < RI) {
+        nf[0] = rows(i + 1, 0);
+        nf[1] = rows(i + 1, 1);
+      }
+      f4_t c[TN];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (SG == 2 && h != s % 2) continue;
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          c[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[h], bf[h][j], SG == 2 || h == 0 ? f4_t{0.f, 0.f, 0.f, 0.f} : c[j], 0, 0, 0);
+      }
+      if (s > 0) scaled(s - 1);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) last[j] = c[j];
+      __builtin_amdgcn_sched_barrier(0);
     }
+    scaled(RI * SG - 1);
   };
 
-  BBuf b[NB];
-#pragma unroll
-  for (int i = 0; i + 1 < NB; ++i) load(b[i], kt0 + i);
-  copy(0);
-  if (nk > 1) copy(1);
-  auto tile = [&](int kt, auto i_c, auto more_c) {
-    constexpr int i = decltype(i_c)::value;
-    if constexpr (decltype(more_c)::value) load(b[(i + NB - 1) % NB], kt + NB - 1);
-    step(b[i], 2 * (kt - kt0), std::integral_constant<int, 0>{}, more_c);
-    step(b[i], 2 * (kt - kt0) + 1, std::integral_constant<int, 1>{}, more_c);
-  };
-  using std::integral_constant;
-  const std::true_type more{};
-  int kt = kt0;
-  for (; kt + NB <= kt1; kt += NB) {    // (without exits: they would make the compiler wait for all loads)
-    tile(kt, integral_constant<int, 0>{}, more);
-    tile(kt + 1, integral_constant<int, 1>{}, more);
-    if constexpr (NB == 4) {
-      tile(kt + 2, integral_constant<int, 2>{}, more);
-      tile(kt + 3, integral_constant<int, 3>{}, more);
-    }
-  }
-  const std::false_type last{};         // all weights are on the way
-  if (kt < kt1) tile(kt, integral_constant<int, 0>{}, last);
-  if constexpr (NB == 4) {
-    if (kt + 1 < kt1) tile(kt + 1, integral_constant<int, 1>{}, last);
-    if (kt + 2 < kt1) tile(kt + 2, integral_constant<int, 2>{}, last);
-  }
+  copy(kt0, 0);
+  load(b, kt0);
+  for (int kt = kt0; kt < kt1; ++kt) tile(kt, (kt - kt0) & 1);
 
   // wave (kh, side) keeps half of the row tiles and hands the others to wave ^ 2
   __syncthreads();
@@ -607,26 +617,28 @@ __global__ __launch_bounds__(kGThreads, RI <= 4 ? 3 : 2) void int4_gemm_kernel(I
 }
 
 // Row tiles (16 RI rows) and k slices of a prompt, by the time of a slice's 128-input tiles: a
-// CU's workgroups share its matrix and vector units (us per tile for each that it gets), and a
-// round of them (three a CU at RI <= 4, two above) takes at least a wave's own latencies; slices
-// add the partial sums' way out and back and a second launch.  Fitted to 1670 timed (shape, RI,
-// S) of 20 to 2048 tokens, within 7% of each; what it picks is 1% off the fastest on average, 11%
-// at most.  1500 x 4096 -> 12288 takes 159 us in tiles of 96 rows (exactly six workgroups a CU), 169
-// in 64 and 162 in 128; 150 x 5120 -> 17408 takes 51 us in tiles of 64 and 57 in 32 or 96.
+// CU's workgroups share its matrix and vector units (us per tile for each that it gets; groups of 32
+// scale twice the sums), and a round of as many as its registers hold takes at least a wave's own
+// latencies; slices add the partial sums' way out and back and a second launch.  Fitted to 2937 timed
+// (shape, RI, S) of 33 to 2048 tokens, over half of them within 4% and 90% within 10%; what it picks
+// is 1% off the fastest on average, 11% at most.  1500 x 4096 -> 12288 takes 166 us in tiles of 96 rows
+// (exactly six workgroups a CU), 169 in 64 and 170 in 128; 512 x 5120 -> 17408 takes 119 us in tiles of 64
+// and 130 in 96 or 128.
+constexpr int gemm_workgroups(int ri, int GU) { return ri == 2 ? (GU < 4 ? 4 : 3) : ri == 4 && GU < 4 ? 3 : 2; }   // of a CU
 struct GemmPlan {
   int ri, S;
 };
-GemmPlan plan_gemm(int M, int NT, int KT) {
+GemmPlan plan_gemm(int M, int NT, int KT, int GU) {
   GemmPlan p{8, 1};
   double least = -1.0;
   for (int ri = 2; ri <= 8; ri += 2) {
     const int64_t tiles = (int64_t)((NT + 7) / 8) * ((M + 16 * ri - 1) / (16 * ri));
-    const int64_t slots = ri <= 4 ? 768 : 512;
+    const int64_t slots = 256 * gemm_workgroups(ri, GU);
     for (int S = 1; S <= std::min(KT, 16); ++S) {
       const int64_t w = tiles * S;
-      const double shared = (double)((w + 255) / 256) * (0.24 + 0.079 * ri);
-      const double alone = (double)((w + slots - 1) / slots) * (0.38 + 0.126 * ri);
-      const double c = ((KT + S - 1) / S) * std::max(shared, alone) + (S > 1 ? 2.75 + (double)S * M * NT * 128.0 / 6e6 : 0.0);
+      const double shared = (double)((w + 255) / 256) * (0.157 + (GU < 4 ? 0.1 : 0.132) * ri);
+      const double alone = (double)((w + slots - 1) / slots) * (0.294 + (GU < 4 ? 0.117 : 0.171) * ri);
+      const double c = ((KT + S - 1) / S) * std::max(shared, alone) + (S > 1 ? 2.97 + (double)S * M * NT * 128.0 / 6.26e6 : 0.0);
       if (least < 0.0 || c < least) {
         least = c;
         p = {ri, S};
@@ -657,7 +669,7 @@ extern "C" int64_t helm_int4_linear_workspace_bytes(int M, int N, int K, int gro
   if (M < 1 || N < 1 || K < 1 || N > (1 << 27) || K > (1 << 19)) return 0;
   if (group_size != 32 && group_size != 64 && group_size != 128) return 0;
   const int NT = (N + 15) / 16, KT = (K + 127) / 128;
-  const int S = M <= kGemvTokens ? plan_gemv(M, NT, KT, 128 / group_size).S : plan_gemm(M, NT, KT).S;
+  const int S = M <= kGemvTokens ? plan_gemv(M, NT, KT, 128 / group_size).S : plan_gemm(M, NT, KT, 128 / group_size).S;
   return S > 1 ? (int64_t)S * M * NT * 16 * (int64_t)sizeof(float) : 0;
 }
 
@@ -684,7 +696,7 @@ extern "C" int helm_int4_linear(const void* x, int64_t ldx, const void* qweight,
   a.NT = (N + 15) / 16; a.KT = (K + 127) / 128; a.np = a.NT * 16;
   const int GU = 128 / group_size;
   const GemvPlan gp = M <= kGemvTokens ? plan_gemv(M, a.NT, a.KT, GU) : GemvPlan{};
-  const GemmPlan mp = M <= kGemvTokens ? GemmPlan{} : plan_gemm(M, a.NT, a.KT);
+  const GemmPlan mp = M <= kGemvTokens ? GemmPlan{} : plan_gemm(M, a.NT, a.KT, GU);
   a.S = M <= kGemvTokens ? gp.S : mp.S;
   const int64_t need = a.S > 1 ? (int64_t)a.S * M * a.np * (int64_t)sizeof(float) : 0;
   HELM_CHECK_ARG(need == 0 || (workspace && helm::aligned16(workspace) && workspace_bytes >= need),

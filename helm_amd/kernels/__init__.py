@@ -371,9 +371,8 @@ def int4_linear(input: torch.Tensor, weight: Int4Weight, bias: Optional[torch.Te
     """y = fp16(input @ W.T + bias) with 4-bit weights W = codes * scale (one scale per
     output and group of inputs) on the GPU, fp32 accumulate.
 
-    input [..., K] fp16, weight an Int4Weight of [N, K], bias [N] fp16 or None.  Decode
-    (<= 32 tokens) scales each group's sum in fp32; above, the weights enter the product
-    as fp16(code * scale)."""
+    input [..., K] fp16, weight an Int4Weight of [N, K], bias [N] fp16 or None.  Scales
+    multiply sums of codes * x in fp32; y is rounded once."""
     q = weight.qweight
     index = _native.gpu_of("int4_linear", input, q, bias, out)
     N, K = weight.out_features, weight.in_features

@@ -136,8 +136,8 @@ int helm_int8_gemm_ws(const void* x, int64_t ldx, const int8_t* q, int64_t ldq,
 /*   y[m,n] = fp16( sum_g s[n,g] sum_{k in g} c[n,k] x[m,k]  (+ bias[n]) )  */
 /* ------------------------------------------------------------------------ */
 
-/* Any M >= 1: a matrix-core GEMV for 1-32 tokens, a tiled product above (whose weights
- * are fp16(c * s); the GEMV applies s in fp32).  c in [-8, 7], group_size 32, 64 or 128.
+/* Any M >= 1: a matrix-core GEMV for 1-32 tokens, a tiled product above; both apply s to
+ * sums in fp32.  c in [-8, 7], group_size 32, 64 or 128.
  *   x       [M, K] fp16, row stride ldx        y [M, N] fp16, row stride ldy
  *   qweight the codes in tiles of 16 outputs x 128 inputs, NT = ceil(N / 16) by
  *           KT = ceil(K / 128) of them: 32-bit word t (0..3) of lane l (0..63) of tile

@@ -1,0 +1,83 @@
+"""int4_linear against its definition in fp64 where the kernels' forms could part from it: one rounding
+whatever the number of tokens, scales of any size, infinite inputs, inputs of one sign, and every form that
+the shapes can take.
+
+Tolerance.  y = fp16(e + d) with e exact, so |y - e| <= |fp16(e) - e| + 2 |d| (the distance to the nearest
+fp16 number changes by no more than its argument does).  d sums fp32 errors, each at most 2^-23 (a matrix
+instruction may cut off instead of rounding) of a partial sum:
+  * sums over the codes themselves (17 tokens and more): up to 128 inputs of a group one after another, partial
+    sums no larger than sum |c x| of the group, then K / 32 groups, 16 waves or slices and the bias;
+  * up to 16 tokens: 32 additions of partial sums no larger than 300 sum |x| of the group (codes plus 8 behind an
+    offset of up to 256), the rest as above.
+As a whole d is far smaller: its signs are independent, and its norm below 2^-18 of e's norm.
+"""
+import numpy as np
+import pytest
+import torch
+
+from helm_amd import kernels as hk
+
+
+def make(n, k, gs, seed, big=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(-8, 8, (n, k), generator=g, dtype=torch.int8, device="cuda")
+    scale = ((0.5 + torch.rand(n, k // gs, generator=g, device="cuda")) * 0.006 * big).half()
+    return codes, scale
+
+
+def normal(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").half()
+
+
+def exact(x, codes, scale, bias=None):
+    """fp64 products, and the bounds' sums: sum |w x| and sum s |x|."""
+    gs = codes.shape[1] // scale.shape[1]
+    s = scale.double().repeat_interleave(gs, 1)
+    w, x64 = codes.double() * s, x.double()
+    e = x64 @ w.t().contiguous()
+    if bias is not None:
+        e += bias.double()
+    return e, x64.abs() @ w.abs().t().contiguous(), x64.abs() @ s.t().contiguous()
+
+
+def check(y, x, codes, scale, bias=None):
+    e, wx, sx = exact(x, codes, scale, bias)
+    k, m = codes.shape[1], x.shape[0]
+    d = (k / 32 + 16 + 20 + (0 if m <= 16 else 128)) * 2.0 ** -23 * wx + (32 * 2.0 ** -23 * 300 * sx if m <= 16 else 0)
+    if bias is not None:
+        d += 2.0 ** -23 * bias.double().abs()
+    nearest = (e.half().double() - e).abs()
+    err = (y.double() - e).abs()
+    assert (err <= nearest + 2 * d).all(), float((err - nearest - 2 * d).max())
+    if e.numel() >= 4000:
+        assert float(err.norm()) <= float(nearest.norm()) + 2.0 ** -17 * float(e.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gs", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 16, 17, 32, 33, 64, 65, 100, 250])
+@pytest.mark.parametrize("n,k", [(200, 256), (1000, 4096)])
+def test_one_rounding_at_any_number_of_tokens(cuda, m, gs, n, k):
+    codes, scale = make(n, k, gs, m)
+    x = normal(n + m, m, k)
+    bias = normal(5, n)
+    w = hk.Int4Weight.pack(codes, scale)
+    check(hk.int4_linear(x, w), x, codes, scale)
+    check(hk.int4_linear(x, w, bias), x, codes, scale, bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gs", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 20, 33, 100])
+def test_scales_whose_products_fp16_does_not_hold(cuda, m, gs):
+    """Scales up to 60000 and down to the smallest: code * scale is beyond fp16 or below its steps, y is not."""
+    n, k = 150, 384
+    codes, _ = make(n, k, gs, m)
+    scale = torch.full((n, k // gs), 60000.0, device=cuda).half()
+    scale[::2] = 2.0 ** -24
+    scale[::3] = 3 * 2.0 ** -24
+    x = normal(3, m, k) * 2.0 ** -6
+    x[:, ::5] = 0
+    for factor in (2.0 ** -3, 1.0):
+        xs = (x.float() * factor).half()
+        check(hk.int4_linear(xs, hk.Int4Weight.pack(codes, scale)), xs, codes, scale)
