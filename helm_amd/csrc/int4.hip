@@ -471,12 +471,14 @@ __global__ __launch_bounds__(kGThreads, RI <= 4 && (RI == 2 || GU < 4) ? 3 : 2) 
       for (int i = 0; i < kCopies; ++i) copy_to_lds(xb, aoff[i], base + i * 1024);
       return;
     }
-    // K ends inside the tile: chunks past it read the row's last one (weights there are zero)
+    // K ends inside the tile: zeros past it (against weights of 0 an infinity would give NaN)
     int c = wave * kCopies * 64 + lane;
     asm volatile("" : "+v"(c));         // (nothing of this is kept in registers around the loop)
 #pragma unroll 1
-    for (int i = 0; i < kCopies; ++i, c += 64)
-      copy_to_lds(xb, offset(c) - 2 * max(kt * 128 + chunk(c) * 8 - (K - 8), 0), base + i * 1024);
+    for (int i = 0; i < kCopies; ++i, c += 64) {
+      if (kt * 128 + chunk(c) * 8 < K) copy_to_lds(xb, offset(c), base + i * 1024);
+      else *reinterpret_cast<uint4*>(smem + stage * kStageBytes + c * 16) = uint4{};
+    }
   };
 
   // a tile's weights of this wave: words 2 kh, 2 kh + 1 and their scales

@@ -81,3 +81,40 @@ def test_scales_whose_products_fp16_does_not_hold(cuda, m, gs):
     for factor in (2.0 ** -3, 1.0):
         xs = (x.float() * factor).half()
         check(hk.int4_linear(xs, hk.Int4Weight.pack(codes, scale)), xs, codes, scale)
+
+
+def with_infinities(m, n, k, gs):
+    """x with infinities in three rows, and weights of which half of the outputs have no code of 0."""
+    codes, scale = make(n, k, gs, m + n)
+    half = codes[:(n + 1) // 2]
+    half[half == 0] = 3
+    x = normal(k, m, k)
+    clean = x.clone()
+    x[0, k // 3] = float("inf")
+    x[m // 2, k - 1] = float("-inf")                      # the last one: next to where K may end inside a tile
+    x[m - 1, 1] = float("inf")
+    x[m - 1, k - 9] = float("inf")
+    return x, clean, codes, scale
+
+
+def check_infinities(x, clean, codes, scale):
+    w = hk.Int4Weight.pack(codes, scale)
+    y, finite = hk.int4_linear(x, w).cpu(), hk.int4_linear(clean, w).cpu()
+    gs = codes.shape[1] // scale.shape[1]
+    e = x.cpu().double() @ (codes.cpu().double() * scale.cpu().double().repeat_interleave(gs, 1)).t()
+    rows = ~x.isfinite().all(-1).cpu()
+    assert torch.equal(y[~rows], finite[~rows])           # the other tokens keep their bits
+    got, want = y[rows].double(), e[rows]
+    assert not want.isfinite().any() and want.isinf().any()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(0.0, 1.0, -1.0), want.nan_to_num(0.0, 1.0, -1.0))
+
+
+INFINITE = [(40, 128, 128), (72, 160, 32), (100, 192, 64), (250, 1056, 32), (130, 17408, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,gs", INFINITE)
+@pytest.mark.parametrize("m", [33, 70, 90, 200])
+def test_infinite_inputs_of_a_prompt(cuda, m, n, k, gs):
+    check_infinities(*with_infinities(m, n, k, gs))
