@@ -117,16 +117,19 @@ __device__ __forceinline__ const void* uniform(const void* p) {
 // tiles per wave, and the scales of a row tile's share through another, waited for by count:
 // 96 KB on the way per CU, and no register holds any (two or three row tiles in registers
 // instead spilled, or kept less on the way: 4.2 TB/s; this streams 151936 x 4096, 321 MB, at
-// 6.1, and 5120 -> 34816, 92 MB in 20 us, at 4.6, of which 5 us are its start).  A tile is read
+// 6.1).  Where the shares are uneven the barriers wait: 5120 inputs are two tiles for half of the waves
+// and three for the others, and 34816 outputs nine row tiles for half of the workgroups and eight for
+// the others, so 0.79 of the places hold a tile: 92 MB in 20 us, 4.6 TB/s.  A tile is read
 // back as it lies, a 16-byte operand word group per lane.
-// The products run on b + u; the -sum((b + 8) x) that turns them into codes is the same for
-// every output, so it is computed once per wave and group (an MFMA with a constant operand)
-// and starts each accumulation: fp32 sums of numbers up to 264 |x| (2^-24 of them: 2^-13 of a
-// code's unit).  A group's sum is scaled by its outputs' scales in fp32.  The waves' partial
+// The products of up to 16 tokens run on b + u; the -sum((b + 8) x) that turns them into codes is the
+// same for every output, so it is computed once per wave and group (an MFMA with a constant operand)
+// and starts each accumulation.  Its partial sums are up to 300 sum |x| of the group, each rounded by
+// 2^-24 of that.  (Codes for every product, four more instructions a word: 151936 x 4096 at one token
+// 53 -> 61 us, 5120 -> 34816 20 -> 22.9.)  Infinite starts take a walk of their own.  A group's sum is scaled by its outputs' scales in fp32.  The waves' partial
 // tiles meet in LDS, one barrier per row tile, and take turns at the epilogue.
-// 17 to 32 tokens are two operands of each unpacked weight: 12288 x 4096 at 24 tokens 12.5 us
-// against the tiled product's 17.2, 4096 x 12288 at 32 16.5 against 17.3, 1.17 times as fast over
-// 12 shapes.
+// 17 to 32 tokens are two operands of each unpacked weight, here the codes themselves (two products share
+// the four instructions): 12288 x 4096 at 24 tokens 13.0 us, where the tiled product
+// takes 19 at 33.
 constexpr int kGemvTokens = 32;
 constexpr int kW = 16;
 constexpr int kMaxTiles = 64;         // row tiles a workgroup may walk (staged biases)
@@ -238,103 +241,120 @@ __global__ __launch_bounds__(kW * 64) void int4_gemv_kernel(Int4Args a) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
         if (u >= own || (u0 + u) * 128 + t * 32 >= a.K) xr[mb][u][t] = h8_t{};
-  // -sum((b + 8) x) of each group: every row of the product with a constant operand
+  // -sum((b + 8) x) of each group: every row of the product with a constant operand.  Where x holds an
+  // infinity it is one too, or NaN, and the sum that starts with it NaN.
   float nbias[MB][UW][GU];
-  {
+  bool inf = false;                     // of the lane's token
+  if constexpr (MB == 1) {
     const _Float16 p = (_Float16)-264.0f, q = (_Float16)-24.0f;
     const h8_t c = {p, p, q, q, p, p, q, q};
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
+    for (int u = 0; u < UW; ++u)
 #pragma unroll
-      for (int u = 0; u < UW; ++u)
+      for (int g = 0; g < GU; ++g) {
+        f4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int g = 0; g < GU; ++g) {
-          f4_t s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int t = 0; t < TG; ++t) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, xr[mb][u][g * TG + t], s, 0, 0, 0);
-          nbias[mb][u][g] = s[0];
-        }
+        for (int t = 0; t < TG; ++t) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(c, xr[0][u][g * TG + t], s, 0, 0, 0);
+        nbias[0][u][g] = s[0];
+        inf |= !(fabsf(s[0]) < INFINITY);
+      }
   }
   const Unpack unpack;
 
   const uint8_t* pw = &s_w[wave][0];  // slots read next
   const uint8_t* ps = &s_s[wave][0];
   const int total = T * UW;
-  for (int t = 0; t < T; ++t) {
-    f4_t acc[MB];
+  // inf_c: some token's group starts with an infinity; such sums run on the codes themselves, all others as ever
+  auto walk = [&](auto inf_c) {
+    for (int t = 0; t < T; ++t) {
+      f4_t acc[MB];
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) acc[mb] = f4_t{0.f, 0.f, 0.f, 0.f};
+      for (int mb = 0; mb < MB; ++mb) acc[mb] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < UW; ++u) {
-      // tile landed: at most the kDepth - 1 later tiles' copies are on the way, and those of
-      // the row tiles that begin among them (the stream's end, where fewer follow, waits for
-      // all)
-      constexpr auto later = [](int u_) {
-        int n = kDepth - 1;
-        for (int j = 1; j < kDepth; ++j) n += (u_ + j) % UW == 0;
-        return n;
-      };
-      if (t * UW + u + kDepth <= total) wait_vm_n(later(u));
-      else wait_vm<0>();
-      uint4 w = *reinterpret_cast<const uint4*>(pw + lane * 16);
-      uint2 sc[GU];
+      for (int u = 0; u < UW; ++u) {
+        // tile landed: at most the kDepth - 1 later tiles' copies are on the way, and those of
+        // the row tiles that begin among them (the stream's end, where fewer follow, waits for
+        // all)
+        constexpr auto later = [](int u_) {
+          int n = kDepth - 1;
+          for (int j = 1; j < kDepth; ++j) n += (u_ + j) % UW == 0;
+          return n;
+        };
+        if (t * UW + u + kDepth <= total) wait_vm_n(later(u));
+        else wait_vm<0>();
+        uint4 w = *reinterpret_cast<const uint4*>(pw + lane * 16);
+        uint2 sc[GU];
 #pragma unroll
-      for (int g = 0; g < GU; ++g) sc[g] = *reinterpret_cast<const uint2*>(ps + (u * GU + g) * 32 + grp * 8);
-      pw = pw + 1024 == &s_w[wave][kDepth * 1024] ? &s_w[wave][0] : pw + 1024;
-      // the slot is refilled once this wave's reads have returned
-      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w) :: "memory");
+        for (int g = 0; g < GU; ++g) sc[g] = *reinterpret_cast<const uint2*>(ps + (u * GU + g) * 32 + grp * 8);
+        pw = pw + 1024 == &s_w[wave][kDepth * 1024] ? &s_w[wave][0] : pw + 1024;
+        // the slot is refilled once this wave's reads have returned
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w) :: "memory");
 #pragma unroll
-      for (int g = 0; g < GU; ++g) asm volatile("" : "+v"(sc[g].x), "+v"(sc[g].y));
-      if (t + (u + kDepth) / UW < T) issue(t + (u + kDepth) / UW, (u + kDepth) % UW);
-      if (u >= own) continue;         // not this wave's (uniform)
-      const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
+        for (int g = 0; g < GU; ++g) asm volatile("" : "+v"(sc[g].x), "+v"(sc[g].y));
+        if (t + (u + kDepth) / UW < T) issue(t + (u + kDepth) / UW, (u + kDepth) % UW);
+        if (u >= own) continue;         // not this wave's (uniform)
+        const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int g = 0; g < GU; ++g) {
-        h8_t wf[TG];
+        for (int g = 0; g < GU; ++g) {
+          h8_t wf[TG];
 #pragma unroll
-        for (int q = 0; q < TG; ++q) wf[q] = __builtin_bit_cast(h8_t, unpack(wd[g * TG + q]));
+          for (int q = 0; q < TG; ++q)
+            wf[q] = MB == 1 ? __builtin_bit_cast(h8_t, unpack(wd[g * TG + q])) : word_codes(unpack, wd[g * TG + q]);
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-          float z = nbias[mb][u][g];
-          asm("" : "+v"(z));          // (or four copies of each would be kept)
-          f4_t c = {z, z, z, z};
+          for (int mb = 0; mb < MB; ++mb) {
+            float z = MB == 1 ? nbias[mb][u][g] : 0.f;
+            if constexpr (MB == 1) asm("" : "+v"(z));   // (or four copies of each would be kept)
+            f4_t c = {z, z, z, z};
 #pragma unroll
-          for (int q = 0; q < TG; ++q) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[q], xr[mb][u][g * TG + q], c, 0, 0, 0);
-          acc[mb][0] = fmaf(lo_h(sc[g].x), c[0], acc[mb][0]);
-          acc[mb][1] = fmaf(hi_h(sc[g].x), c[1], acc[mb][1]);
-          acc[mb][2] = fmaf(lo_h(sc[g].y), c[2], acc[mb][2]);
-          acc[mb][3] = fmaf(hi_h(sc[g].y), c[3], acc[mb][3]);
+            for (int q = 0; q < TG; ++q) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[q], xr[mb][u][g * TG + q], c, 0, 0, 0);
+            if constexpr (decltype(inf_c)::value) {
+              f4_t e = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int q = 0; q < TG; ++q)
+                e = __builtin_amdgcn_mfma_f32_16x16x32_f16(word_codes(unpack, wd[g * TG + q]), xr[mb][u][g * TG + q], e, 0, 0, 0);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) c[r] = fabsf(z) < INFINITY ? c[r] : e[r];
+            }
+            acc[mb][0] = fmaf(lo_h(sc[g].x), c[0], acc[mb][0]);
+            acc[mb][1] = fmaf(hi_h(sc[g].x), c[1], acc[mb][1]);
+            acc[mb][2] = fmaf(lo_h(sc[g].y), c[2], acc[mb][2]);
+            acc[mb][3] = fmaf(hi_h(sc[g].y), c[3], acc[mb][3]);
+          }
         }
       }
-    }
-    ps = ps + 256 == &s_s[wave][kScSlots * 256] ? &s_s[wave][0] : ps + 256;
+      ps = ps + 256 == &s_s[wave][kScSlots * 256] ? &s_s[wave][0] : ps + 256;
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) s_c[t & 1][mb][wave][lane] = acc[mb];
-    lds_barrier();      // buffer t & 1 is written again only after tile t + 1's barrier
+      for (int mb = 0; mb < MB; ++mb) s_c[t & 1][mb][wave][lane] = acc[mb];
+      lds_barrier();      // buffer t & 1 is written again only after tile t + 1's barrier
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      if (wave != ((t * MB + mb) & (kW - 1))) continue;
-      const f4_t(*sc)[64] = s_c[t & 1][mb];
-      f4_t v = sc[0][lane];
+      for (int mb = 0; mb < MB; ++mb) {
+        if (wave != ((t * MB + mb) & (kW - 1))) continue;
+        const f4_t(*sc)[64] = s_c[t & 1][mb];
+        f4_t v = sc[0][lane];
 #pragma unroll (UW * MB <= 2 ? 15 : 5)  // (as many reads on the way as registers are left: 57 -> 53 us at 151936 x 4096)
-      for (int w = 1; w < kW; ++w) {
-        const f4_t o = sc[w][lane];
+        for (int w = 1; w < kW; ++w) {
+          const f4_t o = sc[w][lane];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] += o[r];
-      }
-      const int n0 = (tb + t * nb) * 16 + grp * 4, m = mb * 16 + col;   // v[r]: output n0 + r of token m
-      if (m < M && n0 < a.N) {
-        if constexpr (PART) {
-          *reinterpret_cast<f4_t*>(a.part + ((int64_t)sl * M + m) * a.np + n0) = v;
-        } else {
-          uint16_t* yp = a.y + (int64_t)m * a.ldy + n0;
+          for (int r = 0; r < 4; ++r) v[r] += o[r];
+        }
+        const int n0 = (tb + t * nb) * 16 + grp * 4, m = mb * 16 + col;   // v[r]: output n0 + r of token m
+        if (m < M && n0 < a.N) {
+          if constexpr (PART) {
+            *reinterpret_cast<f4_t*>(a.part + ((int64_t)sl * M + m) * a.np + n0) = v;
+          } else {
+            uint16_t* yp = a.y + (int64_t)m * a.ldy + n0;
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n0 + r < a.N) yp[r] = f2h(v[r] + h2f(s_bias[t * 16 + grp * 4 + r]));
+            for (int r = 0; r < 4; ++r)
+              if (n0 + r < a.N) yp[r] = f2h(v[r] + h2f(s_bias[t * 16 + grp * 4 + r]));
+          }
         }
       }
     }
+  };
+  if constexpr (MB == 1) {
+    if (__builtin_expect(__any(inf), 0)) return walk(std::true_type{});
   }
+  walk(std::false_type{});
 }
 
 // Adds the S partial sums of four outputs of a token, and the bias.

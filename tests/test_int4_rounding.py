@@ -118,3 +118,22 @@ INFINITE = [(40, 128, 128), (72, 160, 32), (100, 192, 64), (250, 1056, 32), (130
 @pytest.mark.parametrize("m", [33, 70, 90, 200])
 def test_infinite_inputs_of_a_prompt(cuda, m, n, k, gs):
     check_infinities(*with_infinities(m, n, k, gs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,gs", INFINITE + [(1000, 4096, 64), (300, 5120, 128), (600, 2048, 128), (16400, 512, 32)])
+@pytest.mark.parametrize("m", [1, 5, 16, 17, 32])
+def test_infinite_inputs_of_a_few_tokens(cuda, m, n, k, gs):
+    check_infinities(*with_infinities(m, n, k, gs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gs", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 16, 17, 32, 33, 100])
+def test_inputs_of_one_sign(cuda, m, gs):
+    """Sums of codes plus an offset are far larger than the sums of codes that they stand for."""
+    n, k = 500, 4096
+    codes, scale = make(n, k, gs, m)
+    x = (2.0 + normal(m, m, k).float().abs()).half()
+    for signed in (x, -x):
+        check(hk.int4_linear(signed, hk.Int4Weight.pack(codes, scale)), signed, codes, scale)
