@@ -36,7 +36,7 @@ import torch
 
 from .. import _native
 from ..kernels import attention as ka
-from ..kernels import fused, int8_linear, quantize_per_channel
+from ..kernels import Int8Linear, fused, int8_linear, quantize_per_channel
 from .kv_allocator import KVAllocator
 from .kv_cache import KVCacheManager, perform_streaming_attention
 from .page_table import DevicePageTable, PinnedRing
@@ -129,7 +129,16 @@ class Int8Qwen3Weights:
         """Take the weights of a transformers Qwen3ForCausalLM whose linears were
         replaced by Int8Linear (helm_amd.kernels.patch_linears); q/k/v are packed
         into one buffer and the modules are re-pointed at views of it, so the
-        patched-forward path and the engine share storage."""
+        patched-forward path and the engine share storage.  Raises RuntimeError, with
+        every module as it was, where a projection is anything else (an Int4Linear has
+        buffers of the same names in another layout)."""
+        for i, layer in enumerate(model.model.layers):
+            for part in ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj",
+                         "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj"):
+                owner, name = part.split(".")
+                m = getattr(getattr(layer, owner), name)
+                if not isinstance(m, Int8Linear):
+                    raise RuntimeError(f"Int8Qwen3Weights: layer {i}'s {part} is {type(m).__name__}, not Int8Linear")
         cfg = model.config
         D = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
         shape = Qwen3Shape(cfg.hidden_size, cfg.num_attention_heads, cfg.num_key_value_heads, D,
