@@ -253,27 +253,29 @@ def alloc_blocked_sequences(n: int, num_kv_heads: int, cap: int, head_dim: int, 
 
 
 class AttnWorkspace:
-    """Reusable fp32 split-K workspace (part_o + part_ml), grown on demand."""
+    """Reusable fp32 split-K workspace (part_o + part_ml), grown on demand.  What it has outgrown
+    stays (a captured call goes on using its address); it grows twofold at least, so that this is
+    no more than it holds."""
 
     def __init__(self, device: torch.device):
         self.device = device
         self.buf = torch.empty(0, dtype=torch.float32, device=device)
         self._outgrown = []
 
+    def _grow(self, n: int) -> None:
+        if self.buf.numel() < n:
+            self._outgrown.append(self.buf)
+            self.buf = torch.empty(max(n, 2 * self.buf.numel()), dtype=torch.float32, device=self.device)
+
     def get(self, B: int, Hq: int, D: int, total_splits: int):
         n_o = B * Hq * total_splits * D
         n = n_o + B * Hq * total_splits * 2
-        if self.buf.numel() < n:
-            self.buf = torch.empty(n, dtype=torch.float32, device=self.device)
+        self._grow(n)
         return self.buf[:n_o], self.buf[n_o:n]
 
     def reserve(self, index: int, nbytes: int) -> int:
-        """Address of at least `nbytes`, for a call on GPU `index`.  What the workspace has
-        outgrown stays (a captured call goes on using its address); it grows twofold at least, so
-        that this is no more than it holds."""
-        if self.buf.numel() * 4 < nbytes:
-            self._outgrown.append(self.buf)
-            self.buf = torch.empty(max(-(-nbytes // 4), 2 * self.buf.numel()), dtype=torch.float32, device=self.device)
+        """Address of at least `nbytes`, for a call on GPU `index`."""
+        self._grow(-(-nbytes // 4))
         if self.buf.get_device() != index:
             raise RuntimeError(f"AttnWorkspace: on {self.buf.device}, the call on GPU {index}")
         return self.buf.data_ptr()
