@@ -10,17 +10,17 @@
 //   * pick: a workgroup per row finds the chunk that holds a border from those sums and
 //     resolves the key inside it from the few logits of that chunk, then the slice that
 //     holds the drawn token, then the token.
-// Weights of a chunk are summed in 2^-44 fixed point relative to the slice's largest:
-// sums of integers do not depend on their order, so atomics leave the result the same
-// from run to run.  All else is in 64 bits: a token next to a border decides a whole
+// Weights of a chunk are summed in 2^-44 fixed point relative to the slice's largest, those of
+// the border's chunk that stay in 2^-50 of what the chunk's stay below: sums of integers do not
+// depend on their order, so atomics leave the result the same from run to run.  All else is in 64 bits: a token next to a border decides a whole
 // number.
 // Bound by latency: the logits are read once by as many CUs as there are slices; then a
 // row has four dependent round trips to memory (sums, the border's chunk, the slice's
 // borders, its logits) and a scan after each.  Scans run over DPP, and every wave repeats
 // the small ones for itself instead of waiting at a barrier for another.  A row of 151936 with
-// top-k 20 and top-p 0.8 takes 16 us (5 of them the slices); 16 rows without filters 19, with
-// top-p alone 31 (every logit is listed, and the border's chunk holds a third of them); 64 rows of
-// 50257 with min-p 20.
+// top-k 20 and top-p 0.8 takes 16.5 us (5 of them the slices); 16 rows without filters 19, with
+// top-p alone 31.5 (every logit is listed, and the border's chunk holds a third of them); 64 rows of
+// 50257 with min-p 21.
 #include "helm_common.h"
 
 namespace {
@@ -78,6 +78,9 @@ __device__ __forceinline__ double exp2_neg(double y, const double* tab) {
   const double p = fma(fma(fma(fma(fma(r, 1.0 / 120, 1.0 / 24), r, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0);
   const int i = (int)fmax(n, -131072.0);
   return ldexp(p * tab[i & 63], i >> 6);
+}
+__device__ __forceinline__ double pow2(int e) {             // |e| < 1023
+  return __builtin_bit_cast(double, (unsigned long long)(1023 + e) << 52);
 }
 // weight of `key` against `top`, the largest; c = log2(e) / t
 __device__ __forceinline__ double weight(uint32_t key, uint32_t top, double c, const double* tab) {
@@ -325,6 +328,7 @@ __global__ __launch_bounds__(kPT) void sample_pick_kernel(SampleArgs a, bool vec
   __shared__ uint32_t s_pc[kPW][kChunks];
   __shared__ uint32_t s_hist[2][1024];                 // number of each key of a chunk
   __shared__ double s_wkey[1024];                      // weight of each key of the border's chunk
+  __shared__ unsigned long long s_wfix[1024];          // the same in fixed point
   __shared__ double s_sm[kMaxSlices];                  // kept weight of a slice, without border ties
   __shared__ uint32_t s_tie[kMaxSlices];
   __shared__ double s_wd[2][kPW];
@@ -533,7 +537,17 @@ __global__ __launch_bounds__(kPT) void sample_pick_kernel(SampleArgs a, bool vec
   bkey = (uint32_t)__builtin_amdgcn_readfirstlane((int)bkey);   // the same in every lane
   // kept weight of each slice: whole chunks above the border's, its own logit by logit
   const int bl = kChunks - 1 - (int)(bkey >> 10);
-  if (held != bl) s_wkey[1023 - tid] = weight((bkey & ~1023u) | (uint32_t)(1023 - tid), top, c, s_tab);
+  // (a list's order within a chunk is that of atomics: sums in fixed point, 2^-50 of what the chunk's
+  // weights stay below, do not depend on it; the largest of all is 1, so below 2^-900 they may be 0)
+  const uint32_t ctop = min(bkey | 1023u, top);
+  const float below = ((float)value_of(ctop) - (float)value_of(top)) * (float)c;
+  const int wexp = ctop == top ? 1 : (int)ceilf(fmaxf(below, -900.f)) + 1;
+  {
+    const double w = held == bl ? s_wkey[1023 - tid] : weight((bkey & ~1023u) | (uint32_t)(1023 - tid), top, c, s_tab);
+    // w 2^(50 - wexp) in the last places of a number from 2^52 on
+    s_wfix[1023 - tid] = __builtin_bit_cast(unsigned long long, fma(w, pow2(50 - wexp), 4503599627370496.0)) -
+                         __builtin_bit_cast(unsigned long long, 4503599627370496.0);
+  }
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
     const int n = (int)lane_of(cnt[i], bl);
@@ -543,15 +557,15 @@ __global__ __launch_bounds__(kPT) void sample_pick_kernel(SampleArgs a, bool vec
     }
   }
   __syncthreads();
-  double ms[kOwn];
+  unsigned long long part[kOwn];                       // of the border's chunk
   uint32_t tie[kOwn];
   auto count = [&](int i, uint32_t key) {
-    ms[i] += key > bkey ? s_wkey[key & 1023u] : 0.0;
+    part[i] += key > bkey ? s_wfix[key & 1023u] : 0ull;
     tie[i] += key == bkey;
   };
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
-    ms[i] = lane < bl ? mass[i] : 0.0;
+    part[i] = 0;
     tie[i] = 0;
     if (lane < (int)lane_of(cnt[i], bl)) count(i, el[i]);
   }
@@ -560,8 +574,12 @@ __global__ __launch_bounds__(kPT) void sample_pick_kernel(SampleArgs a, bool vec
   for (int i = 0; i < kOwn; ++i) {
     const int s = wave + kPW * i;
     if (s >= S) break;
-    const double sum = wave_total(ms[i]);
-    const uint32_t ties = wave_total(tie[i]);
+    double sum = wave_total(lane < bl ? mass[i] : 0.0);
+    uint32_t ties = 0;
+    if (lane_of(cnt[i], bl) > 0) {                     // listed in the border's chunk
+      sum += (double)wave_total(part[i]) * pow2(wexp - 50);
+      ties = wave_total(tie[i]);
+    }
     if (lane == 0) {
       s_sm[s] = sum;
       s_tie[s] = ties;
