@@ -62,6 +62,7 @@ _SIGNATURES = {
     "helm_fp16_gemv_rmsnorm": [_vp, _i64, _vp, _f32, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp],
     "helm_argmax_f16": [_vp, _i64, _i32, _i32, _vp, _vp],
     "helm_int4_linear": [_vp, _i64, _vp, _vp, _i32, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _i64, _vp],
+    "helm_int4_linear_form": [_i32, _i32, _i32, _i32, _vp],
     "helm_kv_append_q8": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp],
     "helm_qk_norm_rope_append_q8": [_vp, _i64, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _i32,
                                     _i32, _i32, _i32, _i32, _vp],

@@ -695,6 +695,27 @@ extern "C" int64_t helm_int4_linear_workspace_bytes(int M, int N, int K, int gro
   return S > 1 ? (int64_t)S * M * NT * 16 * (int64_t)sizeof(float) : 0;
 }
 
+extern "C" int helm_int4_linear_form(int M, int N, int K, int group_size, int32_t* form) {
+  HELM_CHECK_ARG(form, "helm_int4_linear_form: null pointer");
+  HELM_CHECK_ARG(M >= 1 && N >= 1 && K >= 1, "helm_int4_linear_form: M, N, K must be positive");
+  HELM_CHECK_SUPPORTED(N <= (1 << 27) && K <= (1 << 19) && M <= (1 << 22), "helm_int4_linear_form: shape too large");
+  HELM_CHECK_SUPPORTED((group_size == 32 || group_size == 64 || group_size == 128) && K % group_size == 0,
+                       "helm_int4_linear_form: group size must be 32, 64 or 128 and divide K");
+  const int NT = (N + 15) / 16, KT = (K + 127) / 128, GU = 128 / group_size;
+  if (M <= kGemvTokens) {
+    const GemvPlan p = plan_gemv(M, NT, KT, GU);
+    form[0] = M > 16 ? 2 : 1;
+    form[1] = p.uw;
+    form[2] = p.S;
+  } else {
+    const GemmPlan p = plan_gemm(M, NT, KT, GU);
+    form[0] = 0;
+    form[1] = 16 * p.ri;
+    form[2] = p.S;
+  }
+  return HELM_OK;
+}
+
 extern "C" int helm_int4_linear(const void* x, int64_t ldx, const void* qweight, const void* scale,
                                 int group_size, const void* bias, void* y, int64_t ldy, int M, int N, int K,
                                 void* workspace, int64_t workspace_bytes, void* stream) {

@@ -152,6 +152,10 @@ int helm_int8_gemm_ws(const void* x, int64_t ldx, const int8_t* q, int64_t ldq,
  * helm_int4_linear_workspace_bytes (0: may be NULL).  Beside helm_int8_gemv_ws and
  * helm_int8_gemm_ws, the counterparts of fp16_gemv.cpp:105-157. */
 int64_t helm_int4_linear_workspace_bytes(int M, int N, int K, int group_size);
+/* The kernel that helm_int4_linear picks at a shape, as three numbers: blocks of 16 tokens (1
+ * or 2) of the GEMV, or 0 for the tiled product; 128-input tiles a wave (GEMV) or rows a tile;
+ * workgroups that share the inputs of an output. */
+int helm_int4_linear_form(int M, int N, int K, int group_size, int32_t* form);
 int helm_int4_linear(const void* x, int64_t ldx, const void* qweight, const void* scale,
                      int group_size, const void* bias, void* y, int64_t ldy, int M, int N, int K,
                      void* workspace, int64_t workspace_bytes, void* stream);
