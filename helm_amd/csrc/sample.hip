@@ -12,8 +12,8 @@
 //     holds the drawn token, then the token.
 // Weights of a chunk are summed in 2^-44 fixed point relative to the slice's largest, those of
 // the border's chunk that stay in 2^-50 of what the chunk's stay below: sums of integers do not
-// depend on their order, so atomics leave the result the same from run to run.  All else is in 64 bits: a token next to a border decides a whole
-// number.
+// depend on their order, so atomics leave the result the same from run to run.  All else is in 64
+// bits: a token next to a border decides a whole number.
 // Bound by latency: the logits are read once by as many CUs as there are slices; then a
 // row has four dependent round trips to memory (sums, the border's chunk, the slice's
 // borders, its logits) and a scan after each.  Scans run over DPP, and every wave repeats
