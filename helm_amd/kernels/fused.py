@@ -266,8 +266,9 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
     by index), of these the shortest prefix, by weight, that holds a share top_p, of these
     the ones of at least min_p times the largest; then, in index order, the token at which
     the summed weight passes u times the sum of all.  temperature 0 is `argmax`.  Each
-    setting is a number, or a tensor with one per row (fp32, top_k int32).  NaN logits are
-    never drawn; a row with no logit above -inf gives 0.  N is at most 262144.  `workspace` from
+    setting is a number, or a tensor with one per row (fp32, top_k int32).  At a temperature
+    above 0 NaN logits are never drawn (`argmax` takes them as the largest) and a row with no
+    logit above -inf gives 0.  N is at most 262144.  `workspace` from
     sample_workspace, allocated here when not given."""
     tensors = [x for x in (temperature, top_k, top_p, min_p) if torch.is_tensor(x)]
     index = _native.gpu_of("sample", logits, u, out, workspace, *tensors)
