@@ -9,7 +9,8 @@
 // Output: V's codes turned into fp16 (exact), fp32 accumulation.
 //
 // Bound by streaming the pages once, with the vector ALU close behind: 16384 tokens of 8 heads, D
-// 128, 34 MB, take 10 us and 2.2 for the merge, 16 items of up to 12000 35 and 4.  One 256-thread
+// 128, 34 MB, take 10 us and 2.2 for the merge, 16 items of up to 12000 35 and 4 (with nothing in them
+// 21 together: 1024 workgroups in two rounds, whose first loads do not wait for a length).  One 256-thread
 // workgroup per (split, kv head, item), its four waves taking 64-token steps round robin.
 // Per step a wave computes
 //   S[64 tok x 16 col] = K . Q^T         four 16 x 16 tiles

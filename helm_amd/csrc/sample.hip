@@ -16,7 +16,8 @@
 // bits: a token next to a border decides a whole number.
 // Bound by latency: the logits are read once by as many CUs as there are slices; then a
 // row has four dependent round trips to memory (sums, the border's chunk, the slice's
-// borders, its logits) and a scan after each.  Scans run over DPP, and every wave repeats
+// borders, its logits) and a scan after each, and one more for u and for settings of its own, which are
+// read where they are needed.  Scans run over DPP, and every wave repeats
 // the small ones for itself instead of waiting at a barrier for another.  A row of 151936 with
 // top-k 20 and top-p 0.8 takes 16.5 us (5 of them the slices); 16 rows without filters 19, with
 // top-p alone 31.5 (every logit is listed, and the border's chunk holds a third of them); 64 rows of
