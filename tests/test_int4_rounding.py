@@ -137,3 +137,16 @@ def test_inputs_of_one_sign(cuda, m, gs):
     x = (2.0 + normal(m, m, k).float().abs()).half()
     for signed in (x, -x):
         check(hk.int4_linear(signed, hk.Int4Weight.pack(codes, scale)), signed, codes, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(33, 40), (130, 6144)])
+def test_rows_of_a_prompt_far_apart(cuda, m, n):
+    """The largest row stride that the tiled product takes (its offsets have 32 bits), and one beyond."""
+    k = 160
+    codes, scale = make(n, k, 32, m)
+    w = hk.Int4Weight.pack(codes, scale)
+    for ldx in (1 << 23, (1 << 23) + 8):
+        x = torch.empty((m - 1) * ldx + k, dtype=torch.float16, device=cuda).as_strided((m, k), (ldx, 1))
+        x.copy_(normal(m, m, k))
+        check(hk.int4_linear(x, w), x.contiguous(), codes, scale)
