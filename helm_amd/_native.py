@@ -66,6 +66,16 @@ _SIGNATURES = {
     "helm_kv_append_q8": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp],
     "helm_qk_norm_rope_append_q8": [_vp, _i64, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _i32,
                                     _i32, _i32, _i32, _i32, _vp],
+    "helm_chunk_attn": [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32,
+                        _i32, _i32, _i32, _i32, _f32, _vp, _i64, _i64, _vp, _i64, _vp],
+    "helm_rope_append": [_vp, _i64, _vp, _vp, _f32, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _f32,
+                         _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp],
+    "helm_copy_pages": [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp],
+    "helm_copy_pages_q8": [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp],
+    "helm_fork_pages": [_vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32,
+                        _vp],
+    "helm_fork_pages_q8": [_vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32,
+                           _vp],
     "helm_dequantize_pages": [_vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp],
     "helm_paged_decode_attn_q8": [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32,
                                   _i32, _i32, _f32, _i32, _vp, _i64, _vp],
@@ -81,6 +91,7 @@ _OTHER = {
     "helm_paged_attn_noalloc_max_floats": ([], _i64),
     "helm_int4_linear_workspace_bytes": ([_i32, _i32, _i32, _i32], _i64),
     "helm_paged_attn_q8_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32, _i32, _i32], _i64),
+    "helm_chunk_attn_workspace_bytes": ([_i32] * 10, _i64),
     "helm_sample_workspace_bytes": ([_i32, _i32], _i64),
     "helm_argmax_workspace_bytes": ([_i32], _i64),
     "helm_prefill_attn_workspace_bytes": ([_i32, _i32, _i32, _i32, _i32], _i64),

@@ -1,0 +1,877 @@
+// chunk_attention.hip — attention of a ragged batch of new tokens over a paged cache,
+// with a sliding window and first tokens that stay visible.
+//
+// Sequence b has rows q_starts[b] .. q_starts[b + 1] - 1 of q, its n newest tokens; its
+// t-th row stands at p = seq_lens[b] - n + t and sees key j where j <= p and (no window,
+// or j > p - window, or j < sinks).  out = softmax(scale q . K^T) V over those keys.
+//
+// All lengths are on the device, so what a workgroup does is found on the device too (the
+// plan): each sequence's rows (token, head of the kv head's group; token-major) are cut into
+// row tiles, each tile's keys into the sequence's number of pieces, and workgroup x of a
+// kv head takes the x-th (sequence, tile, piece).  Pieces are sized so that a launch has a
+// few more workgroups than the chip has places, whatever the lengths are; sequences of one
+// piece write their output, the others fp32 partials that a second kernel merges.  The
+// grid and the workspace depend on bounds that the host knows (plan_of).
+//
+// Two kernels share the sequences by their number of rows:
+//   few_attn_kernel   up to 16 or 32 rows (decode, drafts): bound by streaming K and V
+//                     once; the four waves of a workgroup take key steps in turn
+//   tile_attn_kernel  more (prompts): bound by the matrix cores; the waves take rows and
+//                     share K and V through LDS
+// Both run S^T = K . Q^T and O^T += V^T . P^T on v_mfma_f32_16x16x32_f16 with the keys of the
+// score tiles permuted so that each lane holds the probabilities of the 8 consecutive keys
+// whose V^T it feeds to the second product, and an online softmax in the log2 domain whose
+// maximum is raised only when it is passed by kLazy.
+#include <algorithm>
+#include <type_traits>
+
+#include "helm_common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr float kLazy = 8.f;            // lazy-rescale slack of the running maximum (log2)
+constexpr int kMaxPieces = 64;          // of a tile's keys
+
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+// How one of the two kernels cuts the sequences it takes.
+struct Form {
+  int lo, hi;          // it takes sequences of lo < rows <= hi
+  int tile;            // rows of a tile
+  int step;            // keys of a step
+  int min_steps;       // least steps of a piece
+  int want;            // pieces of a kv head that fill the chip
+  int items;           // workgroups of a kv head that the grid has
+};
+
+struct ChunkArgs {
+  const uint16_t* q;
+  int64_t q_st, q_sh;                   // query element (t, h, d): t*q_st + h*q_sh + d
+  uint16_t* out;
+  int64_t o_st, o_sh;
+  const uint16_t* k;
+  int64_t k_ss, k_hs;
+  const uint16_t* v;
+  int64_t v_ss, v_hs, v_ds;
+  int64_t num_slots;
+  const int32_t* page_table;
+  int64_t pt_stride;
+  const int32_t* seq_lens;
+  const int32_t* q_starts;              // null: one row per sequence
+  int N, B, Hq, Hkv, G, P, max_pages, max_new;
+  int window, sinks;                    // window 0: none
+  int covered;                          // tokens that the table has room for
+  float qk_scale_log2;
+  Form f;
+  float* part_o;                        // [Hkv][split items][tile rows][D] sums, not normalised
+  float* part_ml;                       // [Hkv][split items][tile rows][2] running maximum, sum
+  int split_items;                      // of a kv head
+};
+
+struct Seq {
+  int start, n, rows, len;              // first row, new tokens, rows (token, head) to do, tokens
+  int tiles, steps;
+};
+
+__device__ __forceinline__ Seq seq_of(const ChunkArgs& a, int i) {
+  Seq s{0, 0, 0, 0, 0, 0};
+  if (i >= a.B) return s;
+  int s0 = i, e = i + 1;
+  if (a.q_starts) {
+    s0 = a.q_starts[i];
+    e = a.q_starts[i + 1];
+  }
+  s.len = a.seq_lens[i];
+  s.start = min(max(s0, 0), a.N);
+  s.n = max(min(e, a.N) - s.start, 0);
+  s.rows = min(s.n, a.max_new) * a.G;
+  if (s.rows <= a.f.lo || s.rows > a.f.hi) {
+    s.rows = 0;
+    return s;
+  }
+  s.tiles = (s.rows + a.f.tile - 1) / a.f.tile;
+  int keys = min(max(s.len, 0), a.covered);
+  // (at most: a tile's window begins at its first row's and ends at its last row)
+  if (a.window) keys = (int)min((int64_t)keys, (int64_t)a.window + a.sinks + a.f.tile / a.G + 2 * a.f.step);
+  s.steps = max((keys + a.f.step - 1) / a.f.step, 1);
+  return s;
+}
+
+// Sum over a workgroup's threads, to all of them, and this thread's exclusive prefix.
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t& before, uint64_t* s_wave) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t inc = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint64_t o = __shfl_up(inc, off, 64);
+    if (lane >= off) inc += o;
+  }
+  __syncthreads();
+  if (lane == 63) s_wave[wave] = inc;
+  __syncthreads();
+  uint64_t total = 0, base = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) base += s_wave[w];
+    total += s_wave[w];
+  }
+  before = base + inc - v;
+  return total;
+}
+
+struct Item {
+  int seq, start, n, rows, len;         // the sequence: index, first row, new tokens, rows to do, tokens
+  int tile, piece, pieces;
+  int part;                             // partial of its tile's piece 0
+};
+
+// The want-th (tile, piece) of a kv head, or with MERGE the want-th tile of more than one
+// piece; false where there are fewer.  Pieces of a sequence: its steps over the mean number
+// of steps of a place, rounded.  W = sum of tiles x steps and m = ceil(W / want) give at most
+// W / m + tiles <= want + tiles items, and at most 4/3 want in sequences of several pieces
+// (those have steps >= 3/2 m).
+template <bool MERGE>
+__device__ __forceinline__ bool find_item(const ChunkArgs& a, int want, Item& it) {
+  __shared__ uint64_t s_wave[kWaves];
+  __shared__ Item s_item;
+  const int tid = threadIdx.x;
+  uint64_t work = 0, unused;
+  Seq s = seq_of(a, tid);
+  for (int i = tid; i < a.B; i += kThreads) {
+    if (i != tid) s = seq_of(a, i);
+    work += (uint64_t)s.tiles * (uint64_t)s.steps;
+  }
+  if (a.B > kThreads) s = seq_of(a, tid);
+  const uint64_t W = block_scan(work, unused, s_wave);
+  const uint64_t mean = (W + a.f.want - 1) / a.f.want;
+  const int m = (int)min(max(mean, (uint64_t)a.f.min_steps), (uint64_t)1 << 30);
+  if (tid == 0) s_item.pieces = 0;
+  uint64_t base = 0;                    // low half: items before, high half: partials before
+  for (int i0 = 0; i0 < a.B; i0 += kThreads) {
+    if (i0 > 0) s = seq_of(a, i0 + tid);
+    const int pieces = min(max((s.steps + m / 2) / m, 1), kMaxPieces);
+    const uint32_t parts = pieces > 1 ? (uint32_t)(s.tiles * pieces) : 0u;
+    const uint32_t mine = MERGE ? (pieces > 1 ? (uint32_t)s.tiles : 0u) : (uint32_t)(s.tiles * pieces);
+    uint64_t before;
+    const uint64_t total = block_scan((uint64_t)mine | (uint64_t)parts << 32, before, s_wave);
+    before += base;
+    const int at = want - (int)(uint32_t)before;
+    if (s.tiles > 0 && at >= 0 && at < (int)mine) {
+      const int per = MERGE ? 1 : pieces;
+      const int tile = s.tiles - 1 - at / per;          // the tiles with the most keys first
+      s_item = Item{i0 + tid, s.start, s.n, s.rows, s.len, tile, at % per, pieces,
+                    (int)(before >> 32) + tile * pieces};
+    }
+    base += total;
+    if ((int)(uint32_t)base > want) break;              // (uniform)
+  }
+  __syncthreads();
+  it.seq = __builtin_amdgcn_readfirstlane(s_item.seq);
+  it.start = __builtin_amdgcn_readfirstlane(s_item.start);
+  it.n = __builtin_amdgcn_readfirstlane(s_item.n);
+  it.rows = __builtin_amdgcn_readfirstlane(s_item.rows);
+  it.len = __builtin_amdgcn_readfirstlane(s_item.len);
+  it.tile = __builtin_amdgcn_readfirstlane(s_item.tile);
+  it.piece = __builtin_amdgcn_readfirstlane(s_item.piece);
+  it.pieces = __builtin_amdgcn_readfirstlane(s_item.pieces);
+  it.part = __builtin_amdgcn_readfirstlane(s_item.part);
+  return it.pieces > 0;
+}
+
+// The keys that rows at positions p0 .. p1 see, in steps: those of the sinks, then those of
+// the window.  Step j covers the keys from at(j) * step on.
+struct Steps {
+  int sink, first, count;               // steps of the sinks; first step of the window; all
+  int end;                              // no row sees a key from end on,
+  int open;                             // nor one in [sinks, open)
+  __device__ __forceinline__ int at(int j) const { return j < sink ? j : first + j - sink; }
+};
+__device__ __forceinline__ Steps steps_of(const ChunkArgs& a, int p0, int p1, int len, int step) {
+  Steps s{0, 0, 0, 0, 0};
+  s.end = max(min(min(p1 + 1, len), a.covered), 0);
+  const int last = (s.end + step - 1) / step;
+  s.count = last;
+  if (a.window) {
+    s.open = max(p0 - a.window + 1, 0);
+    s.first = s.open / step;
+    s.sink = min((min(a.sinks, s.end) + step - 1) / step, s.first);
+    s.count = s.sink + max(last - s.first, 0);
+  }
+  return s;
+}
+
+// the few-row kernel reads q and K and V once (non-temporal)
+__device__ __forceinline__ h8_t ld_h8_nt(const uint16_t* p) {
+  return __builtin_bit_cast(h8_t, __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p)));
+}
+__device__ __forceinline__ h8_t ld_h8(const uint16_t* p) {
+  return __builtin_bit_cast(h8_t, *reinterpret_cast<const u32x4_t*>(p));
+}
+
+// The bits of the pair of keys 2 q, 2 q + 1 past `key` that some row may see.
+__device__ __forceinline__ uint32_t pair_bits(const ChunkArgs& a, const Steps& s, int key, int q) {
+  auto seen = [&](int k) { return k < s.end && (k >= s.open || k < a.sinks); };
+  return (seen(key + 2 * q) ? 0x0000ffffu : 0u) | (seen(key + 2 * q + 1) ? 0xffff0000u : 0u);
+}
+__device__ __forceinline__ u32x4_t seen_only(const ChunkArgs& a, const Steps& s, int key, bool page_ok, u32x4_t w) {
+  w.x &= page_ok ? pair_bits(a, s, key, 0) : 0u;
+  w.y &= page_ok ? pair_bits(a, s, key, 1) : 0u;
+  w.z &= page_ok ? pair_bits(a, s, key, 2) : 0u;
+  w.w &= page_ok ? pair_bits(a, s, key, 3) : 0u;
+  return w;
+}
+
+// ── few rows ─────────────────────────────────────────────────────────────────
+
+// NC tiles of 16 rows.  Steps of 32 keys, one wave each, round robin; K's and V's registers
+// are filled again as soon as they have been read.  P is split into fp16 hi + lo parts, so
+// that the product keeps fp32's accuracy (the matrix cores wait for memory anyway).
+template <int D, int P, int NC>
+__global__ __launch_bounds__(kThreads, 2) void few_attn_kernel(ChunkArgs a) {
+  constexpr int KT = D / 32;
+  constexpr int DT = D / 16;
+  constexpr int kStep = 32;
+  __shared__ float s_m[kWaves][16 * NC], s_l[kWaves][16 * NC];
+  __shared__ __attribute__((aligned(16))) float s_o[kWaves][16 * NC][D];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int col = lane & 15, grp = lane >> 4;
+  const int hk = (int)(blockIdx.x % (unsigned)a.Hkv);
+  Item it;
+  if (!find_item<false>(a, (int)(blockIdx.x / (unsigned)a.Hkv), it)) return;
+  const int G = a.G;
+  const int p0 = it.len - it.n, p1 = p0 + it.rows / G - 1;      // (one tile a sequence)
+  const Steps steps = steps_of(a, p0, p1, it.len, kStep);
+  const int lo = (int)((int64_t)steps.count * it.piece / it.pieces);
+  const int hi = (int)((int64_t)steps.count * (it.piece + 1) / it.pieces);
+  const int mine = hi - lo > wave ? (hi - lo - 1 - wave) / kWaves + 1 : 0;
+  const int32_t* ptab = a.page_table + (int64_t)it.seq * a.pt_stride;
+  auto tok = [&](int i) { return steps.at(min(lo + wave + i * kWaves, hi - 1)) * kStep; };
+  // slots of this lane's K rows (keys 8 (col / 4) + 4 t + col % 4 of a step) and V keys (8 grp ..)
+  auto slot = [&](int key) {
+    const int s = ptab[min(key / P, a.max_pages - 1)];
+    return s >= 0 && s < a.num_slots ? s : -1;
+  };
+  int nk = -1, nv = -1;
+  if (mine > 0) {
+    nk = slot(tok(0) + (col >> 2) * 8);
+    nv = slot(tok(0) + grp * 8);
+  }
+  const bool two = NC > 1 && it.rows > 16;
+  int pos[NC];
+  h8_t qb[NC][KT];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int row = min(c * 16 + col, it.rows - 1);
+    const int t = row / G;
+    pos[c] = p0 + t;
+    const uint16_t* qp = a.q + (int64_t)(it.start + t) * a.q_st + (int64_t)(hk * G + row - t * G) * a.q_sh + grp * 8;
+#pragma unroll
+    for (int kk = 0; kk < KT; ++kk) qb[c][kk] = ld_h8(qp + kk * 32);
+  }
+  const uint16_t* kbase = a.k + (int64_t)hk * a.k_hs + grp * 8;
+  const uint16_t* vbase = a.v + (int64_t)hk * a.v_hs + (int64_t)col * a.v_ds;
+  h8_t kb[2][KT], vb[DT];
+  auto load_k = [&](int s, int t0) {
+    const uint16_t* kp = kbase + (int64_t)max(s, 0) * a.k_ss + ((t0 + (col >> 2) * 8) % P + (col & 3)) * D;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int kk = 0; kk < KT; ++kk) kb[t][kk] = ld_h8_nt(kp + t * 4 * D + kk * 32);
+  };
+  auto load_v = [&](int s, int t0) {
+    const uint16_t* vp = vbase + (int64_t)max(s, 0) * a.v_ss + (t0 + grp * 8) % P;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) vb[d] = ld_h8_nt(vp + (int64_t)d * 16 * a.v_ds);
+  };
+
+  float m_run[NC], l_run[NC];
+  f4_t o[NC][DT];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    m_run[c] = -INFINITY;
+    l_run[c] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[c][d] = f4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  bool ok = nv >= 0;
+  if (mine > 0) {
+    load_k(nk, tok(0));
+    load_v(nv, tok(0));
+    nk = slot(tok(1) + (col >> 2) * 8);
+    nv = slot(tok(1) + grp * 8);
+  }
+  auto step = [&](int i, auto more) {
+    constexpr bool kMore = decltype(more)::value;
+    const int t0 = tok(i), tv = t0 + grp * 8;
+    const bool whole = __all(ok) && t0 + kStep - 1 <= p0 && t0 + kStep <= steps.end &&
+                       (!a.window || t0 > p1 - a.window || t0 + kStep <= a.sinks);
+    float sv[NC][8];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (c && !two) break;
+      f4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < KT; ++kk) {
+        s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[0][kk], qb[c][kk], s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[1][kk], qb[c][kk], s1, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sv[c][r] = s0[r];
+        sv[c][4 + r] = s1[r];
+      }
+    }
+    if constexpr (kMore) load_k(nk, tok(i + 1));
+    if (!whole) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        vb[d] = __builtin_bit_cast(h8_t, seen_only(a, steps, tv, ok, __builtin_bit_cast(u32x4_t, vb[d])));
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (c && !two) break;
+      if (!whole) {
+        const int top = ok ? min(pos[c], steps.end - 1) : -1;
+        const int low = a.window ? pos[c] - a.window + 1 : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          sv[c][j] = tv + j <= top && (tv + j >= low || tv + j < a.sinks) ? sv[c][j] : -INFINITY;
+      }
+      const float mx = fmaxf(fmaxf(fmaxf(sv[c][0], sv[c][1]), fmaxf(sv[c][2], sv[c][3])),
+                             fmaxf(fmaxf(sv[c][4], sv[c][5]), fmaxf(sv[c][6], sv[c][7]))) * a.qk_scale_log2;
+      if (__ballot(mx > m_run[c] + kLazy)) {
+        float m = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const float m_new = fmaxf(m_run[c], m);
+        const float alpha = __builtin_amdgcn_exp2f(m_run[c] - (m_new == -INFINITY ? 0.f : m_new));
+        l_run[c] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[c][d] *= alpha;
+        m_run[c] = m_new;
+      }
+      const float ref = m_run[c] == -INFINITY ? 0.f : -m_run[c];
+      h8_t ph, pl;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[c][j], a.qk_scale_log2, ref));
+        sum += p;
+        ph[j] = (_Float16)p;
+        pl[j] = (_Float16)(p - (float)ph[j]);
+      }
+      l_run[c] += sum;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[d], ph, o[c][d], 0, 0, 0);
+        o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[d], pl, o[c][d], 0, 0, 0);
+      }
+    }
+    if constexpr (kMore) {
+      load_v(nv, tok(i + 1));
+      ok = nv >= 0;
+      nk = slot(tok(i + 2) + (col >> 2) * 8);
+      nv = slot(tok(i + 2) + grp * 8);
+    }
+  };
+  if (mine > 0) {
+    for (int i = 0; i + 1 < mine; ++i) step(i, std::true_type{});
+    step(mine - 1, std::false_type{});
+  }
+
+  // the lane groups' sums, then (through LDS) the waves
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    float l = l_run[c];
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f4_t*>(&s_o[wave][c * 16 + col][d * 16 + grp * 4]) = o[c][d];
+    if (grp == 0) {
+      s_m[wave][c * 16 + col] = m_run[c];
+      s_l[wave][c * 16 + col] = l;
+    }
+  }
+  __syncthreads();
+  for (int idx = tid; idx < it.rows * (D / 4); idx += kThreads) {
+    const int row = idx / (D / 4), d = (idx - row * (D / 4)) * 4;
+    float m = s_m[0][row];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_m[w][row]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    f4_t n = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(s_m[w][row] - ref);
+      l = fmaf(f, s_l[w][row], l);
+      const f4_t x = *reinterpret_cast<const f4_t*>(&s_o[w][row][d]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) n[e] = fmaf(f, x[e], n[e]);
+    }
+    if (it.pieces > 1) {
+      const int64_t at = ((int64_t)hk * a.split_items + it.part + it.piece) * a.f.tile + row;
+      *reinterpret_cast<f4_t*>(a.part_o + at * D + d) = n;
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.f / l;       // (a row that sees nothing: zeros; NaN stays)
+      const int t = row / G;
+      *reinterpret_cast<uint2*>(a.out + (int64_t)(it.start + t) * a.o_st + (int64_t)(hk * G + row - t * G) * a.o_sh + d) =
+          make_uint2(pack_h2(n[0] * inv, n[1] * inv), pack_h2(n[2] * inv, n[3] * inv));
+    }
+  }
+}
+
+// ── many rows ────────────────────────────────────────────────────────────────
+
+constexpr int kNC = 2;                   // 16-row tiles of a wave
+constexpr int kTile = kWaves * 16 * kNC; // rows of a workgroup
+constexpr int kKeys = 64;                // keys of a step
+
+// Workgroup barrier for the K / V stages: this wave's copies into LDS have landed and its
+// LDS reads have returned (s_waitcnt vmcnt(0) lgkmcnt(0)), then s_barrier.
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (0 << 8));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// One wave's 1 KiB global -> LDS copy: lane l moves 16 bytes from base + off to LDS byte lds +
+// 16 l.  Inline assembly, so that the compiler does not make a step's operand reads wait for
+// the copies of the next one; the step's barrier waits.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // m0 is named as clobbered on purpose
+__device__ __forceinline__ void copy_to_lds(const uint16_t* base, uint32_t off, uint32_t lds) {
+  const uint64_t p = (uint64_t)(uintptr_t)base;
+  const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)p) |
+                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32)) << 32;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(at)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// XOR swizzle of K chunk columns: the 16 rows of an operand read differ in it
+template <int CPR>
+__device__ __forceinline__ int kswz(int r) {
+  return ((r & 3) | (((r >> 3) & 3) << 2)) & (CPR - 1);
+}
+
+template <int D, int P>
+__global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
+  constexpr int NC = kNC;
+  constexpr int KT = D / 32;
+  constexpr int DT = D / 16;
+  constexpr int CPR = D / 8;                        // 16-byte chunks of a K row
+  constexpr int kKC = kKeys * CPR;                  // chunks of a stage's K, and of its V
+  constexpr int kI = kKC / kThreads;                // copies of a thread for each
+  constexpr int UPP = kKeys / P;                    // pages of a step
+  __shared__ __attribute__((aligned(16))) u32x4_t s_kv[2][2 * kKC];
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63;
+  const int col = lane & 15, grp = lane >> 4;
+  const int hk = (int)(blockIdx.x % (unsigned)a.Hkv);
+  Item it;
+  if (!find_item<false>(a, (int)(blockIdx.x / (unsigned)a.Hkv), it)) return;
+  const int G = a.G;
+  const int r0 = it.tile * kTile, rw = r0 + wave * 16 * NC;       // first row of the tile, of this wave
+  const int base = it.len - it.n;                                 // position of the sequence's first row
+  const Steps steps = steps_of(a, base + r0 / G, base + (min(r0 + kTile, it.rows) - 1) / G, it.len, kKeys);
+  const int lo = (int)((int64_t)steps.count * it.piece / it.pieces);
+  const int hi = (int)((int64_t)steps.count * (it.piece + 1) / it.pieces);
+  // positions of this wave's rows (none: no key is below its last one)
+  const int pw0 = base + rw / G, pw1 = rw < it.rows ? base + (min(rw + 16 * NC, it.rows) - 1) / G : -1;
+
+  int pos[NC];
+  h8_t qb[NC][KT];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int row = min(rw + c * 16 + col, it.rows - 1);
+    const int t = row / G;
+    pos[c] = base + t;
+    const uint16_t* qp = a.q + (int64_t)(it.start + t) * a.q_st + (int64_t)(hk * G + row - t * G) * a.q_sh + grp * 8;
+#pragma unroll
+    for (int kk = 0; kk < KT; ++kk) qb[c][kk] = ld_h8(qp + kk * 32);
+  }
+
+  // The table is read through scalar loads: a step's slots are the same for all lanes
+  typedef const __attribute__((address_space(4))) int32_t cint_t;
+  cint_t* ptab = (cint_t*)(uintptr_t)(a.page_table + (int64_t)it.seq * a.pt_stride);
+  int slot[UPP];                                    // of the step whose copies go out next
+  auto look_up = [&](int j) {
+    const int pg = steps.at(min(j, hi - 1)) * UPP;
+#pragma unroll
+    for (int u = 0; u < UPP; ++u) slot[u] = ptab[min(pg + u, a.max_pages - 1)];
+  };
+  auto valid = [&](int s) { return s >= 0 && s < a.num_slots; };
+  uint32_t k_off[kI], v_off[kI];                    // bytes of this thread's chunks from their page's start
+#pragma unroll
+  for (int i = 0; i < kI; ++i) {
+    const int pc = i * kThreads + tid, row = pc / CPR;
+    k_off[i] = (uint32_t)((row % P) * D + ((pc % CPR) ^ kswz<CPR>(row)) * 8) * 2;
+    const int vi = i * kWaves + wave, kp = vi / (D / 32), dim = vi % (D / 32) * 32 + (lane & 31);
+    v_off[i] = ((uint32_t)dim * (uint32_t)a.v_ds + (uint32_t)((kp * 16) % P + (lane >> 5) * 8)) * 2;
+  }
+  const uint16_t* kbase = a.k + (int64_t)hk * a.k_hs;
+  const uint16_t* vbase = a.v + (int64_t)hk * a.v_hs;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)&s_kv[0][0];
+  // Copies of the looked-up step into stage b: one copy instruction is 1 KiB of K rows or 32
+  // dims x 16 keys of V, of one page.  Slots outside the pool read slot 0 (masked later).
+  auto issue = [&](int b) {
+    auto of = [&](int u) {
+      int s = slot[0];
+#pragma unroll
+      for (int x = 1; x < UPP; ++x) s = u == x ? slot[x] : s;
+      return (int64_t)(valid(s) ? s : 0);
+    };
+#pragma unroll
+    for (int i = 0; i < kI; ++i) {
+      const int row = (i * kThreads + wave * 64) / CPR, vi = i * kWaves + wave, kp = vi / (D / 32);
+      copy_to_lds(kbase + of(row / P) * a.k_ss, k_off[i], lds0 + (uint32_t)((b * 2 * kKC + i * kThreads + wave * 64) * 16));
+      copy_to_lds(vbase + of(kp * 16 / P) * a.v_ss, v_off[i], lds0 + (uint32_t)((b * 2 * kKC + kKC + vi * 64) * 16));
+    }
+  };
+
+  float m_run[NC];
+  f4_t o[NC][DT], l_acc[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    m_run[c] = -INFINITY;
+    l_acc[c] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[c][d] = f4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  h8_t ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = (_Float16)1.f;
+
+  uint32_t bad = 0, bad_next = 0;                   // invalid pages of the step, of the next one
+  auto bad_of = [&]() {
+    uint32_t x = 0;
+#pragma unroll
+    for (int u = 0; u < UPP; ++u) x |= valid(slot[u]) ? 0u : 1u << u;
+    return x;
+  };
+  if (lo < hi) {
+    look_up(lo);
+    bad_next = bad_of();
+    issue(0);
+    look_up(lo + 1);
+  }
+  for (int j = lo; j < hi; ++j) {
+    const int b = (j - lo) & 1;
+    stage_barrier();                                // the step is in its stage; the other one is no longer read
+    bad = bad_next;
+    if (j + 1 < hi) {
+      bad_next = bad_of();
+      issue(b ^ 1);
+      look_up(j + 2);
+    }
+    const int key0 = steps.at(j) * kKeys;
+    // V of keys that no row sees may hold anything: zero (uniform over the workgroup; the first
+    // and last steps of a tile)
+    if (bad || key0 + kKeys > steps.end || (key0 < steps.open && key0 + kKeys > a.sinks)) {
+#pragma unroll
+      for (int i = 0; i < kI; ++i) {
+        const int vi = i * kWaves + wave, key = vi / (D / 32) * 16 + (lane >> 5) * 8;
+        u32x4_t* x = &s_kv[b][kKC + vi * 64 + lane];
+        *x = seen_only(a, steps, key0 + key, !((bad >> (key / P)) & 1), *x);
+      }
+      lds_barrier();
+    }
+#pragma unroll
+    for (int u = 0; u < kKeys / 32; ++u) {
+      const int k0 = key0 + u * 32, tv = k0 + grp * 8;
+      // nothing of these 32 keys is visible to this wave's rows
+      if (k0 > pw1 || k0 >= steps.end || (a.window && k0 + 31 <= pw0 - a.window && k0 >= a.sinks)) continue;
+      const bool whole = !bad && k0 + 31 <= pw0 && k0 + 32 <= steps.end &&
+                         (!a.window || k0 > pw1 - a.window || k0 + 32 <= a.sinks);
+      float sv[NC][8];
+      h8_t kf[2][KT];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int row = u * 32 + (col >> 2) * 8 + t * 4 + (col & 3);
+#pragma unroll
+        for (int kk = 0; kk < KT; ++kk)
+          kf[t][kk] = __builtin_bit_cast(h8_t, s_kv[b][row * CPR + ((kk * 4 + grp) ^ kswz<CPR>(row))]);
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        f4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < KT; ++kk) {
+          s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0][kk], qb[c][kk], s0, 0, 0, 0);
+          s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[1][kk], qb[c][kk], s1, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          sv[c][r] = s0[r];
+          sv[c][4 + r] = s1[r];
+        }
+      }
+      if (!whole) {
+        const bool ok = !((bad >> ((u * 32 + grp * 8) / P)) & 1);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int top = ok ? min(pos[c], steps.end - 1) : -1;
+          const int low = a.window ? pos[c] - a.window + 1 : 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            sv[c][e] = tv + e <= top && (tv + e >= low || tv + e < a.sinks) ? sv[c][e] : -INFINITY;
+        }
+      }
+      h8_t vf[DT];
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const int kp = u * 2 + (grp >> 1);
+        vf[d] = __builtin_bit_cast(
+            h8_t, s_kv[b][kKC + (kp * (D / 32) + (d >> 1)) * 64 + (grp & 1) * 32 + (d & 1) * 16 + col]);
+      }
+      float mx[NC];
+      bool raise = false;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        mx[c] = fmaxf(fmaxf(fmaxf(sv[c][0], sv[c][1]), fmaxf(sv[c][2], sv[c][3])),
+                      fmaxf(fmaxf(sv[c][4], sv[c][5]), fmaxf(sv[c][6], sv[c][7]))) * a.qk_scale_log2;
+        raise |= mx[c] > m_run[c] + kLazy;
+      }
+      if (__ballot(raise)) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          float m = fmaxf(mx[c], __shfl_xor(mx[c], 16, 64));
+          m = fmaxf(m, __shfl_xor(m, 32, 64));
+          const float m_new = fmaxf(m_run[c], m);
+          const float alpha = __builtin_amdgcn_exp2f(m_run[c] - (m_new == -INFINITY ? 0.f : m_new));
+          l_acc[c] *= alpha;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[c][d] *= alpha;
+          m_run[c] = m_new;
+        }
+      }
+      // P enters the product rounded to fp16, and so do the sums (a product with ones): the
+      // rounding of a probability then moves numerator and denominator alike
+      h8_t ph[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const float ref = m_run[c] == -INFINITY ? 0.f : -m_run[c];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          ph[c][e] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(sv[c][e], a.qk_scale_log2, ref));
+      }
+#pragma unroll
+      for (int c = 0; c < NC; ++c) l_acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[c], l_acc[c], 0, 0, 0);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], ph[c], o[c][d], 0, 0, 0);
+    }
+  }
+
+  // o[c][d][r] = O^T[dim d*16 + grp*4 + r][row col of tile c]
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int row = rw + c * 16 + col;
+    if (row >= it.rows) continue;
+    const float l = l_acc[c][0];
+    if (it.pieces > 1) {
+      const int64_t at = ((int64_t)hk * a.split_items + it.part + it.piece) * kTile + (row - r0);
+      float* dst = a.part_o + at * D + grp * 4;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) *reinterpret_cast<f4_t*>(dst + d * 16) = o[c][d];
+      if (grp == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_run[c], l);
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int t = row / G;
+      uint16_t* dst = a.out + (int64_t)(it.start + t) * a.o_st + (int64_t)(hk * G + row - t * G) * a.o_sh + grp * 4;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        *reinterpret_cast<uint2*>(dst + d * 16) = make_uint2(pack_h2(o[c][d][0] * inv, o[c][d][1] * inv),
+                                                             pack_h2(o[c][d][2] * inv, o[c][d][3] * inv));
+    }
+  }
+}
+
+// ── joining the pieces ───────────────────────────────────────────────────────
+
+constexpr int kMergeRows = 32;           // of a workgroup
+
+// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over a tile's pieces, four dims a thread;
+// bound by reading the partials once.
+template <int D>
+__global__ __launch_bounds__(kThreads) void chunk_merge_kernel(ChunkArgs a) {
+  const int hk = (int)(blockIdx.x % (unsigned)a.Hkv);
+  Item it;
+  if (!find_item<true>(a, (int)(blockIdx.x / (unsigned)a.Hkv), it)) return;
+  const int r0 = it.tile * a.f.tile;
+  const int rows = min(it.rows - r0, a.f.tile);
+  const int64_t base = (int64_t)hk * a.split_items + it.part;
+  for (int idx = threadIdx.x; idx < kMergeRows * (D / 4); idx += kThreads) {
+    const int row = blockIdx.y * kMergeRows + idx / (D / 4), d = idx % (D / 4) * 4;
+    if (row >= rows) break;
+    const float* ml = a.part_ml + (base * a.f.tile + row) * 2;
+    const float* po = a.part_o + (base * a.f.tile + row) * D + d;
+    const int64_t stride = a.f.tile;
+    float m = -INFINITY;
+    for (int p = 0; p < it.pieces; ++p) m = fmaxf(m, ml[p * stride * 2]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    f4_t n = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    for (int p = 0; p < it.pieces; ++p) {
+      const float2 x = *reinterpret_cast<const float2*>(ml + p * stride * 2);
+      const f4_t y = *reinterpret_cast<const f4_t*>(po + p * stride * D);
+      const float f = __builtin_amdgcn_exp2f(x.x - ref);
+      l = fmaf(f, x.y, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) n[e] = fmaf(f, y[e], n[e]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int t = (r0 + row) / a.G;
+    *reinterpret_cast<uint2*>(a.out + (int64_t)(it.start + t) * a.o_st + (int64_t)(hk * a.G + r0 + row - t * a.G) * a.o_sh + d) =
+        make_uint2(pack_h2(n[0] * inv, n[1] * inv), pack_h2(n[2] * inv, n[3] * inv));
+  }
+}
+
+// ── host ─────────────────────────────────────────────────────────────────────
+
+// How a call's sequences are shared between the two kernels and cut, from what the host knows.
+struct Plan {
+  Form few, tile;                       // items 0: not launched
+  int few_nc;
+  int few_parts, tile_parts;            // partials of a kv head (0: no sequence can have two pieces)
+};
+
+Form form_of(int lo, int hi, int tile, int step, int min_steps, int want, int64_t tiles) {
+  return {lo, hi, tile, step, min_steps, want, (int)std::min<int64_t>(tiles + want, 1 << 28)};
+}
+int parts_of(const Form& f, int64_t keys) {
+  const int64_t steps = (keys + f.step - 1) / f.step;
+  return f.items > 0 && 2 * steps >= 3 * (int64_t)f.min_steps ? (4 * f.want + 2) / 3 : 0;
+}
+
+Plan plan_of(int N, int B, int Hq, int Hkv, int P, int max_pages, int max_new, int window, int sinks) {
+  Plan p{};
+  const int G = Hq / Hkv;
+  const int64_t most = (int64_t)std::min(max_new, N) * G;         // rows of a sequence
+  const int seqs = std::min(B, N);
+  const int few = G > 32 || (B == 1 && most > 32) ? 0 : most <= 16 ? 16 : 32;
+  p.few_nc = few / 16;
+  int64_t keys = (int64_t)max_pages * P;
+  auto bound = [&](const Form& f) {
+    return window ? std::min<int64_t>(keys, (int64_t)window + sinks + f.tile / G + 2 * f.step) : keys;
+  };
+  if (few) {
+    p.few = form_of(0, few, few, 32, 4, std::max(1, 512 / Hkv), seqs);
+    p.few_parts = parts_of(p.few, bound(p.few));
+  }
+  if (most > few) {
+    p.tile = form_of(few, 1 << 30, kTile, kKeys, 4, std::max(1, 512 / Hkv), (int64_t)N * G / kTile + seqs);
+    p.tile_parts = parts_of(p.tile, bound(p.tile));
+  }
+  return p;
+}
+int64_t part_floats(const Form& f, int parts, int Hkv, int D) { return (int64_t)Hkv * parts * f.tile * (D + 2); }
+
+template <int D, int P>
+void launch(ChunkArgs a, const Plan& p, float* ws, hipStream_t s) {
+  auto run = [&](const Form& f, int parts, auto kernel) {
+    a.f = f;
+    a.split_items = parts;
+    a.part_o = ws;
+    a.part_ml = ws + (int64_t)a.Hkv * parts * f.tile * D;
+    ws += part_floats(f, parts, a.Hkv, D);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)f.items * (unsigned)a.Hkv), dim3(kThreads), 0, s, a);
+    if (parts)
+      hipLaunchKernelGGL((chunk_merge_kernel<D>),
+                         dim3((unsigned)(parts / 2 + 1) * (unsigned)a.Hkv, (f.tile + kMergeRows - 1) / kMergeRows),
+                         dim3(kThreads), 0, s, a);
+  };
+  if (p.tile.items) run(p.tile, p.tile_parts, tile_attn_kernel<D, P>);
+  if (p.few.items) {
+    if (p.few_nc == 1) run(p.few, p.few_parts, few_attn_kernel<D, P, 1>);
+    else run(p.few, p.few_parts, few_attn_kernel<D, P, 2>);
+  }
+}
+
+}  // namespace
+
+extern "C" int64_t helm_chunk_attn_workspace_bytes(int N, int B, int Hq, int Hkv, int D, int P, int max_pages,
+                                                   int max_new, int window, int sinks) {
+  if (N < 1 || B < 1 || Hkv < 1 || Hq < Hkv || Hq % Hkv || D < 1 || P < 1 || max_pages < 1 || max_new < 1 ||
+      window < 0 || sinks < 0)
+    return 0;
+  const Plan p = plan_of(N, B, Hq, Hkv, P, max_pages, max_new, window, sinks);
+  return (part_floats(p.few, p.few_parts, Hkv, D) + part_floats(p.tile, p.tile_parts, Hkv, D)) * (int64_t)sizeof(float);
+}
+
+extern "C" int helm_chunk_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const helm_kv_pool* pool,
+                               const int32_t* page_table, int64_t pt_stride, const int32_t* seq_lens,
+                               const int32_t* q_starts, int N, int B, int Hq, int Hkv, int D, int P, int max_pages,
+                               int max_new, int window, int sinks, float scale, void* out, int64_t out_stride_t,
+                               int64_t out_stride_h, void* workspace, int64_t workspace_bytes, void* stream) {
+  const std::string f("helm_chunk_attn");
+  HELM_CHECK_ARG(q && pool && pool->k && pool->v && page_table && seq_lens && out, f + ": null pointer");
+  HELM_CHECK_ARG(N >= 1 && B >= 1 && Hq >= 1 && Hkv >= 1 && max_pages >= 1 && max_new >= 1,
+                 f + ": sizes must be positive");
+  HELM_CHECK_ARG(window >= 0 && sinks >= 0, f + ": window and sinks must not be negative");
+  HELM_CHECK_ARG(q_starts || N == B, f + ": without q_starts there is one row per sequence");
+  HELM_CHECK_ARG(Hq % Hkv == 0, f + ": Hq must be a multiple of Hkv");
+  HELM_CHECK_ARG(scale > 0.f && scale < INFINITY, f + ": scale must be positive and finite");
+  HELM_CHECK_SUPPORTED(D == 64 || D == 128, f + ": head_dim must be 64 or 128");
+  HELM_CHECK_SUPPORTED(P == 16 || P == 32 || P == 64, f + ": page size must be 16, 32 or 64");
+  HELM_CHECK_SUPPORTED((int64_t)N * (Hq / Hkv) < (1 << 30) && Hq <= 65535, f + ": too many rows or heads");
+  HELM_CHECK_SUPPORTED((int64_t)max_pages * P <= (int64_t)1 << 30 && window <= 1 << 30 && sinks <= 1 << 30,
+                       f + ": more than 2^30 keys");
+  HELM_CHECK_ARG(B == 1 || pt_stride >= max_pages, f + ": page-table stride < max_pages");
+  HELM_CHECK_ARG(pool->num_slots >= 1 && pool->k_head_stride >= (int64_t)P * D && pool->v_dim_stride >= P &&
+                     pool->v_head_stride >= (int64_t)P,
+                 f + ": pool strides too small for the page");
+  HELM_CHECK_SUPPORTED(pool->v_dim_stride * D < (1ll << 30), f + ": V dim stride too large (in-page offsets are 32-bit)");
+  HELM_CHECK_SUPPORTED(q_stride_t % 8 == 0 && q_stride_h % 8 == 0 && out_stride_t % 4 == 0 && out_stride_h % 4 == 0 &&
+                           pool->k_slot_stride % 8 == 0 && pool->k_head_stride % 8 == 0 &&
+                           pool->v_slot_stride % 8 == 0 && pool->v_head_stride % 8 == 0 && pool->v_dim_stride % 8 == 0,
+                       f + ": strides must be multiples of 8 (q, pool) / 4 (out) elements");
+  HELM_CHECK_SUPPORTED(helm::aligned16(q) && helm::aligned16(pool->k) && helm::aligned16(pool->v) &&
+                           (reinterpret_cast<uintptr_t>(out) & 7u) == 0,
+                       f + ": q and pools must be 16-byte aligned, out 8-byte aligned");
+  const Plan p = plan_of(N, B, Hq, Hkv, P, max_pages, max_new, window, sinks);
+  const int64_t need = helm_chunk_attn_workspace_bytes(N, B, Hq, Hkv, D, P, max_pages, max_new, window, sinks);
+  HELM_CHECK_ARG(need == 0 || (workspace && helm::aligned16(workspace) && workspace_bytes >= need),
+                 f + ": this call needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
+  HELM_CHECK_SUPPORTED((int64_t)std::max(p.few.items, p.tile.items) * Hkv < (1ll << 31), f + ": too many workgroups");
+  ChunkArgs a{};
+  a.q = static_cast<const uint16_t*>(q); a.q_st = q_stride_t; a.q_sh = q_stride_h;
+  a.out = static_cast<uint16_t*>(out); a.o_st = out_stride_t; a.o_sh = out_stride_h;
+  a.k = static_cast<const uint16_t*>(pool->k); a.k_ss = pool->k_slot_stride; a.k_hs = pool->k_head_stride;
+  a.v = static_cast<const uint16_t*>(pool->v);
+  a.v_ss = pool->v_slot_stride; a.v_hs = pool->v_head_stride; a.v_ds = pool->v_dim_stride;
+  a.num_slots = pool->num_slots;
+  a.page_table = page_table; a.pt_stride = pt_stride; a.seq_lens = seq_lens; a.q_starts = q_starts;
+  a.N = N; a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.P = P; a.max_pages = max_pages;
+  a.max_new = std::min(max_new, N);
+  a.window = window; a.sinks = window ? sinks : 0;
+  a.covered = max_pages * P;
+  a.qk_scale_log2 = scale * kLog2e;
+  float* ws = static_cast<float*>(workspace);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  auto by_page = [&](auto d_tag) {
+    constexpr int Dc = decltype(d_tag)::value;
+    if (P == 16) launch<Dc, 16>(a, p, ws, s);
+    else if (P == 32) launch<Dc, 32>(a, p, ws, s);
+    else launch<Dc, 64>(a, p, ws, s);
+  };
+  if (D == 64) by_page(std::integral_constant<int, 64>{});
+  else by_page(std::integral_constant<int, 128>{});
+  HELM_CHECK_LAUNCH("helm_chunk_attn launch");
+  return HELM_OK;
+}

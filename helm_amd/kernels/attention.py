@@ -2,7 +2,9 @@
 
 Thin typed wrappers over helm_paged_decode_attn / helm_paged_attn_reduce /
 helm_kv_append / helm_stage_pages_h2d, and the same over pages held in 8 bits
-(Q8PoolView: paged_decode_attention_q8, kv_append_q8, dequantize_pages).
+(Q8PoolView: paged_decode_attention_q8, kv_append_q8, dequantize_pages); attention of
+ragged batches of new tokens with sliding windows (chunk_attention,
+window_decode_attention), and pages moved inside a pool (copy_pages, fork_pages).
 
 KV layout.  A page of the reference is a pair of (1, Hkv, P, D) tensors
 (helm/runtime/kv_allocator.py:26-28).  Here every page is a slot of a pool: K is
@@ -563,6 +565,221 @@ def dequantize_pages(pool: Q8PoolView, pages: torch.Tensor) -> PoolView:
         _native.call_on(index, "helm_dequantize_pages", pool.c_ref(), pages.data_ptr(), n, k.data_ptr(), v.data_ptr(),
                         Hkv, D, P, _native.raw_stream(index))
     return PoolView(k, v, page, P * D, page, P * D, P, n, Hkv)
+
+
+# ── ragged batches of new tokens ─────────────────────────────────────────────
+
+@functools.lru_cache(maxsize=4096)
+def chunk_workspace_bytes(N: int, B: int, Hq: int, Hkv: int, D: int, P: int, max_pages: int, max_new: int,
+                          window: int, sinks: int) -> int:
+    """Workspace of helm_chunk_attn (0: none)."""
+    return int(_native.lib().helm_chunk_attn_workspace_bytes(N, B, Hq, Hkv, D, P, max_pages, max_new, window, sinks))
+
+
+def _check_table(what: str, page_table: torch.Tensor, seq_lens: torch.Tensor, B: Optional[int] = None) -> Tuple[int, int]:
+    """(columns, row stride) of an int32 page table [B, max_pages] with its lengths [B]."""
+    if (page_table.dtype != torch.int32 or page_table.dim() != 2 or (B is not None and page_table.shape[0] != B)
+            or (page_table.stride(1) != 1 and page_table.shape[1] > 1)):
+        raise RuntimeError(f"{what}: page_table must be int32 [B, max_pages], row-major")
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != page_table.shape[:1] or not seq_lens.is_contiguous():
+        raise RuntimeError(f"{what}: seq_lens must be int32 [B], contiguous")
+    rows, cols = page_table.shape
+    if rows > 1 and page_table.stride(0) < cols:
+        raise RuntimeError(f"{what}: the rows of page_table overlap")
+    return cols, page_table.stride(0) if rows > 1 else cols
+
+
+def _check_fp16_pool(what: str, pool: PoolView, page_size: int) -> Tuple[int, int]:
+    """(kv heads, head_dim) of an fp16 pool whose pages hold page_size tokens."""
+    if not isinstance(pool, PoolView) or pool.k.dtype != torch.float16 or pool.v.dtype != torch.float16:
+        raise RuntimeError(f"{what}: the pool must be a PoolView of fp16 pages")
+    if page_size not in (16, 32, 64):
+        raise RuntimeError(f"{what}: the page size must be 16, 32 or 64")
+    if pool.k_head_stride < page_size * pool.k.shape[-1] or pool.v_dim_stride < page_size:
+        raise RuntimeError(f"{what}: the pool's pages do not hold {page_size} tokens")
+    return pool.num_kv_heads, pool.k.shape[-1]
+
+
+def _chunk(what: str, q: torch.Tensor, pool: PoolView, page_table: torch.Tensor, seq_lens: torch.Tensor,
+           q_starts: Optional[torch.Tensor], page_size: int, window: int, sinks: int, scale: Optional[float],
+           max_new: Optional[int], workspace: Optional[AttnWorkspace], out: Optional[torch.Tensor]) -> torch.Tensor:
+    index = _native.gpu_of(what, q, pool.k, pool.v, page_table, seq_lens, q_starts, out)
+    if q.dtype != torch.float16 or q.dim() != 3 or (q.stride(2) != 1 and q.shape[2] > 1):
+        raise RuntimeError(f"{what}: q must be fp16 [N, Hq, D] with unit stride on D")
+    N, Hq, D = q.shape
+    Hkv, Dp = _check_fp16_pool(what, pool, page_size)
+    if D != Dp or D not in (64, 128):
+        raise RuntimeError(f"{what}: q has head_dim {D}, the pool {Dp} (64 or 128 are supported)")
+    if Hq % Hkv:
+        raise RuntimeError(f"{what}: {Hq} query heads are no multiple of the pool's {Hkv}")
+    max_pages, pts = _check_table(what, page_table, seq_lens, N if q_starts is None else None)
+    B = page_table.shape[0]
+    if q_starts is not None and (q_starts.dtype != torch.int32 or q_starts.shape != (B + 1,)
+                                 or not q_starts.is_contiguous()):
+        raise RuntimeError(f"{what}: q_starts must be int32 [B + 1] = [{B + 1}], contiguous")
+    if window < 0 or sinks < 0:
+        raise RuntimeError(f"{what}: window and sinks must not be negative")
+    if max_new is None:
+        max_new = N
+    elif max_new < 1:
+        raise RuntimeError(f"{what}: max_new must be positive")
+    if scale is None:
+        scale = D ** -0.5
+    elif not 0.0 < scale < math.inf:
+        raise RuntimeError(f"{what}: scale must be positive and finite")
+    if out is None:
+        out = q.new_empty((N, Hq, D))
+    elif (out.dtype != torch.float16 or out.shape != (N, Hq, D) or out.stride(2) != 1 or out.stride(0) % 4
+          or out.stride(1) % 4 or out.data_ptr() % 8):
+        raise RuntimeError(f"{what}: out must be fp16 [N, Hq, D], unit stride on D, rows 8-byte aligned")
+    if N == 0 or B == 0:
+        return out
+    if max_pages == 0:
+        raise RuntimeError(f"{what}: the page table has no columns")
+    st, sh, _ = q.stride()
+    if st % 8 or sh % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+        st, sh, _ = q.stride()
+    max_new = min(int(max_new), N)
+    # (what no key reaches is no window)
+    window = 0 if window >= max_pages * page_size else int(window)
+    sinks = min(int(sinks), max_pages * page_size) if window else 0
+    need = chunk_workspace_bytes(N, B, Hq, Hkv, D, page_size, max_pages, max_new, window, sinks)
+    ws = None
+    if need:
+        if workspace is None:
+            workspace = AttnWorkspace(q.device)
+        ws = workspace.reserve(index, need)
+    _native.call_on(index, "helm_chunk_attn", q.data_ptr(), st, sh, pool.c_ref(), page_table.data_ptr(), pts,
+                    seq_lens.data_ptr(), _native.ptr(q_starts), N, B, Hq, Hkv, D, page_size, max_pages, max_new,
+                    window, sinks, scale, out.data_ptr(), out.stride(0), out.stride(1), ws, need,
+                    _native.raw_stream(index))
+    return out
+
+
+def chunk_attention(q: torch.Tensor, pool: PoolView, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                    q_starts: torch.Tensor, page_size: int, window: int = 0, sinks: int = 0,
+                    scale: Optional[float] = None, max_new: Optional[int] = None,
+                    workspace: Optional[AttnWorkspace] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of a ragged batch of new tokens over a paged cache that holds them
+    already: whole prompts, chunks of prompts, drafted tokens and single ones, in any mix
+    (helm_chunk_attn).
+
+    Sequence b has rows q_starts[b] .. q_starts[b + 1] - 1 of q [N, Hq, D] fp16, its newest
+    tokens; seq_lens[b] counts them and its cached ones, page_table [B, max_pages] holds its
+    slots (all int32).  The token at position p sees keys j <= p; with a `window` of w > 0 only
+    j > p - w, and the first `sinks` tokens: pages that no new token sees may be freed (-1 in
+    the table).  A token that sees no key gives zeros.  Rows before q_starts[0] and from
+    q_starts[B] on are not written, so a batch may be padded.
+
+    max_new bounds the new tokens of a sequence (any longer one has its first max_new rows
+    written): the smaller, the fewer kernels run.  Lengths are read on the device: a captured
+    call takes other lengths of the same tensors at each replay.  How a sequence's keys are
+    cut depends on the batch, and with it the last bits of its rows.  `workspace` is allocated
+    here when not given; calls that overlap, or two graphs that may replay at once, need one
+    each.  Returns out [N, Hq, D] fp16."""
+    if q_starts is None:
+        raise RuntimeError("chunk_attention: q_starts is missing")
+    return _chunk("chunk_attention", q, pool, page_table, seq_lens, q_starts, page_size, window, sinks, scale, max_new,
+                  workspace, out)
+
+
+def window_decode_attention(q: torch.Tensor, pool: PoolView, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                            page_size: int, window: int, sinks: int = 0, scale: Optional[float] = None,
+                            workspace: Optional[AttnWorkspace] = None,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_decode_attention with a sliding window: the newest token of each sequence, q
+    [B, Hq, D] fp16, attends its last `window` tokens (itself among them; 0: all) and its first
+    `sinks` (chunk_attention of one row per sequence).  Zeros for a sequence of length 0."""
+    return _chunk("window_decode_attention", q, pool, page_table, seq_lens, None, page_size, window, sinks, scale, 1,
+                  workspace, out)
+
+
+# ── pages moved inside a pool ────────────────────────────────────────────────
+
+def _page_layout(what: str, pool, page_size: Optional[int]) -> int:
+    if isinstance(pool, Q8PoolView):
+        return pool._check_page_size(page_size, what)
+    if page_size is None:
+        raise RuntimeError(f"{what}: a PoolView needs its page size")
+    _check_fp16_pool(what, pool, page_size)
+    return page_size
+
+
+def copy_pages(pool, src: torch.Tensor, dst: torch.Tensor, page_size: Optional[int] = None) -> None:
+    """Page dst[i] <- page src[i] of a pool (a PoolView, or a Q8PoolView with its scales), for
+    int32 slots src, dst [n] on the device: what compaction moves, or copies of a shared page
+    before it is written.  Pairs with a slot outside the pool are skipped.  A slot that is
+    written must be named by no other pair (what those pages hold then is not defined)."""
+    what = "copy_pages"
+    P = _page_layout(what, pool, page_size)
+    index = _native.gpu_of(what, pool.k, pool.v, src, dst)
+    for t in (src, dst):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape != src.shape or not t.is_contiguous():
+            raise RuntimeError(f"{what}: src and dst must be contiguous int32 vectors of one length")
+    if src.shape[0] == 0:
+        return
+    D = pool.k.shape[-1]
+    if isinstance(pool, Q8PoolView):
+        _native.call_on(index, "helm_copy_pages_q8", pool.c_ref(), src.data_ptr(), dst.data_ptr(), src.shape[0],
+                        pool.num_kv_heads, D, P, _native.raw_stream(index))
+    else:
+        _native.call_on(index, "helm_copy_pages", pool.c_ref(), src.data_ptr(), dst.data_ptr(), src.shape[0],
+                        pool.num_kv_heads, D, P, _native.raw_stream(index))
+
+
+def fork_pages(pool, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, fresh: torch.Tensor,
+               page_size: Optional[int] = None, table_out: Optional[torch.Tensor] = None,
+               lens_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Children that go on where other sequences stand (beams, samples of one prompt), as one
+    launch: rows of a new page table and their lengths, (table_out [n, max_pages], lens_out
+    [n]).  Child i continues row p = parents[i] of page_table [B, max_pages], seq_lens [B]:
+
+      fresh[i] >= 0   it shares p's full pages, and its next token goes to slot fresh[i], to
+                      which p's last page is copied where it is not full; -1 after it
+      fresh[i] < 0    p's row as it is (the one child that goes on in p's own last page)
+
+    parents and fresh are int32 [n]; a parent outside [0, B) gives a row of -1 and length 0.  A
+    length past the table counts as the table's.  Slots in `fresh` are in the pool, in use
+    nowhere, and named once.  The rows of several layers go in one call as rows of one table.
+    The outputs must not overlap the inputs."""
+    what = "fork_pages"
+    P = _page_layout(what, pool, page_size)
+    index = _native.gpu_of(what, pool.k, pool.v, page_table, seq_lens, parents, fresh, table_out, lens_out)
+    cols, pts = _check_table(what, page_table, seq_lens)
+    for t in (parents, fresh):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape != parents.shape or not t.is_contiguous():
+            raise RuntimeError(f"{what}: parents and fresh must be contiguous int32 vectors of one length")
+    n = parents.shape[0]
+    if table_out is None:
+        table_out = page_table.new_empty((n, cols))
+    if lens_out is None:
+        lens_out = seq_lens.new_empty((n,))
+    if table_out.shape != (n, cols):
+        raise RuntimeError(f"{what}: table_out must be int32 [{n}, {cols}], row-major")
+    _, ots = _check_table(what, table_out, lens_out, n)
+    for a, b in ((table_out, page_table), (lens_out, seq_lens), (table_out, seq_lens), (lens_out, page_table),
+                 (table_out, parents), (table_out, fresh), (lens_out, parents), (lens_out, fresh)):
+        if _overlap(a, b):
+            raise RuntimeError(f"{what}: the outputs must not overlap the inputs")
+    if n == 0:
+        return table_out, lens_out
+    if cols == 0:
+        raise RuntimeError(f"{what}: the page table has no columns")
+    _native.call_on(index, "helm_fork_pages_q8" if isinstance(pool, Q8PoolView) else "helm_fork_pages", pool.c_ref(),
+                    page_table.data_ptr(), pts, seq_lens.data_ptr(), page_table.shape[0], parents.data_ptr(),
+                    fresh.data_ptr(), table_out.data_ptr(), ots, lens_out.data_ptr(), n, cols, pool.num_kv_heads,
+                    pool.k.shape[-1], P, _native.raw_stream(index))
+    return table_out, lens_out
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """True when the bytes from a's first to its last element meet those of b."""
+    def span(t):
+        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
 
 
 def stage_pages_h2d(host_pool: torch.Tensor, dev_staging: torch.Tensor, host_slots,

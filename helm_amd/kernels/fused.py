@@ -8,13 +8,14 @@ projection, and q/k-norm + RoPE + the paged KV write into one kernel.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Union
 
 import torch
 
 from .. import _native
 from . import gemv_split_bytes
-from .attention import _check_places
+from .attention import _check_fp16_pool, _check_places, _check_table
 
 
 def _check_fp16(*ts):
@@ -123,6 +124,54 @@ def rope_inv_freq(head_dim: int, theta: float, device=None) -> torch.Tensor:
         device=device, dtype=torch.float) / head_dim))).float()
 
 
+def rope_scaled_inv_freq(rotary_dim: int, theta: float, kind: str, factor: float,
+                         original_context: Optional[int] = None, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                         device=None):
+    """(inv_freq fp32 [rotary_dim / 2], rope_scale) for contexts `factor` times as long as the
+    one trained on, for rope_append:
+
+      "linear"   every frequency divided by `factor`
+      "theta"    theta raised to theta * factor^(r / (r - 2)): the fastest frequency stays, the
+                 slowest is divided by `factor`
+      "bands"    by how often a frequency turns in the original context, c inv / 2 pi: above
+                 beta_fast turns it stays, below beta_slow it is divided by `factor`, between
+                 them its turns weigh the two linearly
+      "yarn"     the same two ends with weights linear in the dim's index between those of
+                 beta_fast (rounded down) and beta_slow (rounded up) turns, and q and k both times
+                 0.1 ln(factor) + 1 (arXiv 2309.00071)"""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise RuntimeError(f"rope_scaled_inv_freq: rotary_dim must be even and positive (got {rotary_dim})")
+    if not factor >= 1.0:
+        raise RuntimeError(f"rope_scaled_inv_freq: factor must be at least 1 (got {factor})")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    inv, scale = theta ** -i, 1.0
+    if kind in ("bands", "yarn"):
+        if original_context is None or original_context < 1:
+            raise RuntimeError(f"rope_scaled_inv_freq: {kind} needs the original context's length")
+        if not beta_fast > beta_slow > 0.0:
+            raise RuntimeError("rope_scaled_inv_freq: beta_fast must be above beta_slow, and that above 0")
+    if kind == "linear":
+        inv = inv / factor
+    elif kind == "theta":
+        if rotary_dim > 2:
+            inv = (theta * factor ** (rotary_dim / (rotary_dim - 2))) ** -i
+    elif kind == "bands":
+        stay = ((original_context * inv / (2 * math.pi) - beta_slow) / (beta_fast - beta_slow)).clamp(0.0, 1.0)
+        inv = inv * stay + inv / factor * (1.0 - stay)
+    elif kind == "yarn":
+        def index(turns):               # of the dim pair that turns so often in the original context
+            return rotary_dim * math.log(original_context / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        low = max(math.floor(index(beta_fast)), 0)
+        high = min(math.ceil(index(beta_slow)), rotary_dim - 1)
+        at = torch.arange(rotary_dim // 2, dtype=torch.float64)
+        stay = 1.0 - ((at - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        inv = inv * stay + inv / factor * (1.0 - stay)
+        scale = 0.1 * math.log(factor) + 1.0
+    else:
+        raise RuntimeError(f"rope_scaled_inv_freq: kind must be linear, theta, bands or yarn (got {kind!r})")
+    return inv.float().to(device) if device is not None else inv.float(), scale
+
+
 def qk_norm_rope_append(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor,
                         eps: float, positions: torch.Tensor, inv_freq: torch.Tensor,
                         q_out: torch.Tensor, pool, slots: torch.Tensor, offsets: torch.Tensor,
@@ -183,6 +232,69 @@ def qk_norm_rope_append_q8(qkv: torch.Tensor, q_norm_w: Optional[torch.Tensor],
     _native.call_on(index, "helm_qk_norm_rope_append_q8", qkv.data_ptr(), stride, _native.ptr(q_norm_w),
                     _native.ptr(k_norm_w), eps, positions.data_ptr(), inv_freq.data_ptr(), q_out.data_ptr(),
                     pool.c_ref(), slots.data_ptr(), offsets.data_ptr(), B, Hq, Hkv, D, P, _native.raw_stream(index))
+    return q_out
+
+
+def rope_append(qkv: torch.Tensor, pool, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                q_starts: Optional[torch.Tensor], page_size: int, inv_freq: torch.Tensor, num_q_heads: int,
+                num_kv_heads: int, head_dim: int, interleaved: bool = False, rope_scale: float = 1.0,
+                q_norm_w: Optional[torch.Tensor] = None, k_norm_w: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                positions: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions of a ragged batch and its K/V into pages, what chunk_attention reads
+    (helm_rope_append): beside qk_norm_rope_append for other layouts of the rotation, and with
+    the places of the tokens found in the page table.
+
+    Sequence b has rows q_starts[b] .. q_starts[b + 1] - 1 of the fused projection qkv [N,
+    (Hq + 2 Hkv) * D] fp16, the last of its seq_lens[b] tokens (None: one row each); the token
+    at position p goes to slot page_table[b, p // P] at p % P (a place outside the table or the
+    pool is not written).  Per q and k head: RMSNorm where the norm weights are given, then the
+    first 2 len(inv_freq) dims turn by the angle p * inv_freq[i] (in 64 bits), pairs (i, i + r/2)
+    of the r rotated dims, or with `interleaved` (2 i, 2 i + 1), times rope_scale; the other
+    dims pass.  All in fp32, q and k rounded once; v's bits are copied.  `positions` (int32 [N])
+    gives angles of their own, places stay those of the cache.  inv_freq is fp32:
+    rope_inv_freq, or rope_scaled_inv_freq for long contexts.
+
+    Rows outside q_starts are neither kept nor written in q_out [N, Hq, D], which is returned."""
+    what = "rope_append"
+    index = _native.gpu_of(what, qkv, pool.k, pool.v, page_table, seq_lens, q_starts, inv_freq, q_norm_w, k_norm_w,
+                           positions, q_out)
+    _check_fp16(qkv, q_norm_w, k_norm_w, q_out)
+    Hq, Hkv, D = num_q_heads, num_kv_heads, head_dim
+    if qkv.dim() != 2 or qkv.shape[1] != (Hq + 2 * Hkv) * D or qkv.stride(1) != 1:
+        raise RuntimeError(f"{what}: qkv must be [N, (Hq + 2 Hkv) * D] with unit stride")
+    if _check_fp16_pool(what, pool, page_size) != (Hkv, D):
+        raise RuntimeError(f"{what}: {Hkv} heads of {D} do not fit the pool's {pool.num_kv_heads} of {pool.k.shape[-1]}")
+    N, width = qkv.shape
+    cols, pts = _check_table(what, page_table, seq_lens, N if q_starts is None else None)
+    B = page_table.shape[0]
+    if q_starts is not None and (q_starts.dtype != torch.int32 or q_starts.shape != (B + 1,)
+                                 or not q_starts.is_contiguous()):
+        raise RuntimeError(f"{what}: q_starts must be int32 [B + 1] = [{B + 1}], contiguous")
+    if (inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous()
+            or 2 * inv_freq.shape[0] > D):
+        raise RuntimeError(f"{what}: inv_freq must be fp32 [r / 2], contiguous, with r <= {D} rotated dims")
+    if positions is not None and (positions.dtype != torch.int32 or positions.shape != (N,)
+                                  or not positions.is_contiguous()):
+        raise RuntimeError(f"{what}: positions must be int32 [{N}], contiguous")
+    if (q_norm_w is None) != (k_norm_w is None):
+        raise RuntimeError(f"{what}: give both q / k norm weights or neither")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.shape != (D,) or not w.is_contiguous()):
+            raise RuntimeError(f"{what}: norm weights must be [D], contiguous")
+    if q_out is None:
+        q_out = qkv.new_empty((N, Hq, D))
+    elif q_out.shape != (N, Hq, D) or not q_out.is_contiguous():
+        raise RuntimeError(f"{what}: q_out must be [N, Hq, D], contiguous")
+    if N == 0 or B == 0:
+        return q_out
+    stride = qkv.stride(0) if N > 1 else width
+    if stride % 8 or stride < width or qkv.data_ptr() % 16:
+        qkv, stride = qkv.clone(memory_format=torch.contiguous_format), width
+    _native.call_on(index, "helm_rope_append", qkv.data_ptr(), stride, _native.ptr(q_norm_w), _native.ptr(k_norm_w),
+                    eps, page_table.data_ptr(), pts, cols, seq_lens.data_ptr(), _native.ptr(q_starts),
+                    _native.ptr(positions), inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(bool(interleaved)),
+                    rope_scale, q_out.data_ptr(), pool.c_ref(), N, B, Hq, Hkv, D, page_size,
+                    _native.raw_stream(index))
     return q_out
 
 

@@ -309,6 +309,36 @@ int helm_prefill_attn_mask(const void* q, int64_t q_stride_t, int64_t q_stride_h
                            const void* mask, int64_t mask_stride_h, int64_t mask_stride_t,
                            const int32_t* key_end, void* out, int64_t out_stride_t, int64_t out_stride_h, void* stream);
 
+/* Attention of a ragged batch of new tokens over a paged cache, with a sliding window.
+ * Sequence b of B has the rows q_starts[b] .. q_starts[b + 1] - 1 of q [N, Hq, D] (strides
+ * q_stride_t, q_stride_h), its n newest tokens, at positions seq_lens[b] - n ..
+ * seq_lens[b] - 1; their K/V already lie in the pages page_table[b, 0 .. max_pages) of
+ * `pool`.  The row at position p sees the keys j <= p with window == 0, or j > p - window,
+ * or j < sinks; out = softmax(scale * q . K^T) V, row for row in out [N, Hq, D] fp16 (strides
+ * out_stride_t, out_stride_h).  q_starts [B + 1] ascending; null: one row per sequence (N ==
+ * B).  All lengths may change between replays of a captured call.
+ *   - A row that sees no key (an empty table, a negative position) gives zeros; rows of q
+ *     before q_starts[0] or from q_starts[B] on are not written.
+ *   - Table entries outside [0, num_slots) contribute no keys, and are not needed for pages
+ *     that no row sees (those behind the window may be freed); keys past max_pages * P do
+ *     not exist.  K and V of places that no row sees may hold anything.
+ *   - max_new: the most new tokens of a sequence that the call is prepared for (N: any);
+ *     a sequence with more has only its first max_new rows written.
+ *   - workspace (16-byte aligned, contents on entry do not matter) of at least
+ *     helm_chunk_attn_workspace_bytes for the same numbers; 0: may be NULL.
+ * The keys of sequences are cut by what else is in the batch, so a row's last bits can
+ * depend on it; a call's bits do not change from run to run.  scale > 0; D 64 or 128; P 16,
+ * 32 or 64; any Hq / Hkv.  The prefill SDPA of kv_offload.py:253-265 and the decode one of
+ * :126,160 for several sequences at once. */
+int64_t helm_chunk_attn_workspace_bytes(int N, int B, int Hq, int Hkv, int D, int P, int max_pages,
+                                        int max_new, int window, int sinks);
+int helm_chunk_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const helm_kv_pool* pool,
+                    const int32_t* page_table, int64_t pt_stride, const int32_t* seq_lens,
+                    const int32_t* q_starts, int N, int B, int Hq, int Hkv, int D, int P,
+                    int max_pages, int max_new, int window, int sinks, float scale, void* out,
+                    int64_t out_stride_t, int64_t out_stride_h, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+
 /* Largest number of page-table entries one split of helm_paged_decode_attn may
  * stage. */
 int helm_paged_attn_max_split_pages(void);
@@ -380,6 +410,35 @@ int helm_gather_pages_h2d(const void* host_k, const void* host_v, void* dev_k, v
 int helm_stage_pages_h2d(const void* host_pool, void* dev_staging,
                          const int32_t* host_slots, int n, int64_t dev_first_slot,
                          size_t page_bytes, void* copy_stream, void* done_event);
+
+/* Pages moved inside a pool: page dst[i] <- page src[i], K and V whole, for device arrays of n
+ * int32 slots.  Pairs with a slot outside [0, num_slots) are skipped; a slot that is written
+ * must be named by no other pair (what those pages hold then is not defined).  The _q8 form
+ * moves codes and scales of a helm_kv_pool_q8 (declared below).  What move_page
+ * (helm/runtime/kv_allocator.py:95-144) does between tiers, inside one. */
+struct helm_kv_pool_q8;
+int helm_copy_pages(const helm_kv_pool* pool, const int32_t* src, const int32_t* dst, int n, int Hkv,
+                    int D, int P, void* stream);
+int helm_copy_pages_q8(const struct helm_kv_pool_q8* pool, const int32_t* src, const int32_t* dst, int n,
+                       int Hkv, int D, int P, void* stream);
+
+/* Sequences that continue others: row i of table_out [n, max_pages] (row stride out_stride) and
+ * lens_out[i] from row p = parents[i] of page_table [B, max_pages] (row stride pt_stride) and
+ * seq_lens[p] (at most the table's tokens; a parent outside [0, B): a row of -1, length 0).
+ *   fresh[i] <  0: p's row as it is
+ *   fresh[i] >= 0: p's full pages, then fresh[i], then -1; where p's last page is not full it is
+ *                  copied to slot fresh[i] (K and V whole)
+ * Slots in fresh are in use nowhere and named once; outputs do not overlap inputs; tables of
+ * at most 2^30 tokens.  Follows the page lists of helm/runtime/kv_cache.py:30-113, of which the
+ * reference keeps one per sequence and shares none. */
+int helm_fork_pages(const helm_kv_pool* pool, const int32_t* page_table, int64_t pt_stride,
+                    const int32_t* seq_lens, int B, const int32_t* parents, const int32_t* fresh,
+                    int32_t* table_out, int64_t out_stride, int32_t* lens_out, int n, int max_pages,
+                    int Hkv, int D, int P, void* stream);
+int helm_fork_pages_q8(const struct helm_kv_pool_q8* pool, const int32_t* page_table, int64_t pt_stride,
+                       const int32_t* seq_lens, int B, const int32_t* parents, const int32_t* fresh,
+                       int32_t* table_out, int64_t out_stride, int32_t* lens_out, int n, int max_pages,
+                       int Hkv, int D, int P, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* KV pages held in 8 bits                                                  */
@@ -467,6 +526,24 @@ int helm_qk_norm_rope_append(const void* qkv, const void* q_norm_w, const void* 
                              void* q_out, const helm_kv_pool* pool,
                              const int32_t* slots, const int32_t* offsets,
                              int B, int Hq, int Hkv, int D, int P, void* stream);
+
+/* Rotary positions of a ragged batch and its K/V into pages.  Row `row` of qkv [N, (Hq + 2 Hkv)
+ * * D] fp16 (q | k | v, row stride qkv_stride_t) of sequence b (q_starts[b] <= row < q_starts[b
+ * + 1]; q_starts [B + 1] ascending, null: row b) is token p = seq_lens[b] - (q_starts[b + 1] -
+ * row) of it and goes to slot page_table[b, p / P] at offset p % P (not written where that is
+ * outside the table [B, max_pages] or the pool).  Per q / k head: x rsqrt(mean(x^2) + eps) w
+ * where q_norm_w and k_norm_w [D] are given, then of the first r = rotary_dim dims the pairs (i,
+ * i + r/2), with `interleaved` (2 i, 2 i + 1), turn by positions[row] * inv_freq[i] (positions
+ * null: p; the angle in 64 bits) times rope_scale.  fp32 throughout, one rounding; q to q_out
+ * [N, Hq, D] (rows of no sequence are not written), v's bits are copied.  Rows of qkv, norm
+ * weights and q_out 16-byte aligned.  Follows helm/runtime/kv_offload.py:244-249 and
+ * kv_cache.py:55-113. */
+int helm_rope_append(const void* qkv, int64_t qkv_stride_t, const void* q_norm_w, const void* k_norm_w,
+                     float eps, const int32_t* page_table, int64_t pt_stride, int max_pages,
+                     const int32_t* seq_lens, const int32_t* q_starts, const int32_t* positions,
+                     const float* inv_freq, int rotary_dim, int interleaved, float rope_scale,
+                     void* q_out, const helm_kv_pool* pool, int N, int B, int Hq, int Hkv, int D,
+                     int P, void* stream);
 
 /* The q / k half of helm_qk_norm_rope_append for callers that hold the model's
  * own RoPE tables (the patched attention forward of the drop-in path): per-head
