@@ -57,7 +57,7 @@ struct ChunkArgs {
   int64_t k_ss, k_hs;
   const uint16_t* v;
   int64_t v_ss, v_hs, v_ds;
-  int64_t num_slots;
+  int32_t num_slots;
   const int32_t* page_table;
   int64_t pt_stride;
   const int32_t* seq_lens;
@@ -459,13 +459,15 @@ __device__ __forceinline__ void copy_to_lds(const uint16_t* base, uint32_t off, 
 }
 #pragma clang diagnostic pop
 
-// XOR swizzle of K chunk columns: the 16 rows of an operand read differ in it
+// XOR swizzle of K chunk columns: the 16 rows (col >> 2) * 8 + t * 4 + (col & 3) of an operand
+// read have the swizzles col
 template <int CPR>
 __device__ __forceinline__ int kswz(int r) {
   return ((r & 3) | (((r >> 3) & 3) << 2)) & (CPR - 1);
 }
 
-template <int D, int P>
+// WIN: there is a window.
+template <int D, int P, bool WIN>
 __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
   constexpr int NC = kNC;
   constexpr int KT = D / 32;
@@ -474,6 +476,7 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
   constexpr int kKC = kKeys * CPR;                  // chunks of a stage's K, and of its V
   constexpr int kI = kKC / kThreads;                // copies of a thread for each
   constexpr int UPP = kKeys / P;                    // pages of a step
+  constexpr uint32_t kStage = 2 * kKC * 16;         // bytes of a stage
   __shared__ __attribute__((aligned(16))) u32x4_t s_kv[2][2 * kKC];
 
   const int tid = threadIdx.x;
@@ -483,23 +486,23 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
   const int hk = (int)(blockIdx.x % (unsigned)a.Hkv);
   Item it;
   if (!find_item<false>(a, (int)(blockIdx.x / (unsigned)a.Hkv), it)) return;
-  const int G = a.G;
   const int r0 = it.tile * kTile, rw = r0 + wave * 16 * NC;       // first row of the tile, of this wave
   const int base = it.len - it.n;                                 // position of the sequence's first row
-  const Steps steps = steps_of(a, base + r0 / G, base + (min(r0 + kTile, it.rows) - 1) / G, it.len, kKeys);
+  const Steps steps = steps_of(a, base + r0 / a.G, base + (min(r0 + kTile, it.rows) - 1) / a.G, it.len, kKeys);
   const int lo = (int)((int64_t)steps.count * it.piece / it.pieces);
   const int hi = (int)((int64_t)steps.count * (it.piece + 1) / it.pieces);
-  // positions of this wave's rows (none: no key is below its last one)
-  const int pw0 = base + rw / G, pw1 = rw < it.rows ? base + (min(rw + 16 * NC, it.rows) - 1) / G : -1;
+  // positions of this wave's rows (none: every key is behind its last one)
+  const int pw0 = base + rw / a.G, pw1 = rw < it.rows ? base + (min(rw + 16 * NC, it.rows) - 1) / a.G : -1;
 
   int pos[NC];
   h8_t qb[NC][KT];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int row = min(rw + c * 16 + col, it.rows - 1);
-    const int t = row / G;
+    const int t = row / a.G;
     pos[c] = base + t;
-    const uint16_t* qp = a.q + (int64_t)(it.start + t) * a.q_st + (int64_t)(hk * G + row - t * G) * a.q_sh + grp * 8;
+    const uint16_t* qp =
+        a.q + (int64_t)(it.start + t) * a.q_st + (int64_t)(hk * a.G + row - t * a.G) * a.q_sh + grp * 8;
 #pragma unroll
     for (int kk = 0; kk < KT; ++kk) qb[c][kk] = ld_h8(qp + kk * 32);
   }
@@ -513,8 +516,8 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
 #pragma unroll
     for (int u = 0; u < UPP; ++u) slot[u] = ptab[min(pg + u, a.max_pages - 1)];
   };
-  auto valid = [&](int s) { return s >= 0 && s < a.num_slots; };
-  uint32_t k_off[kI], v_off[kI];                    // bytes of this thread's chunks from their page's start
+  // bytes of this thread's chunks from their page's start
+  uint32_t k_off[kI], v_off[kI];
 #pragma unroll
   for (int i = 0; i < kI; ++i) {
     const int pc = i * kThreads + tid, row = pc / CPR;
@@ -524,29 +527,47 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
   }
   const uint16_t* kbase = a.k + (int64_t)hk * a.k_hs;
   const uint16_t* vbase = a.v + (int64_t)hk * a.v_hs;
+  const uint32_t k_ss = (uint32_t)a.k_ss, v_ss = (uint32_t)a.v_ss;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_t*)&s_kv[0][0];
-  // Copies of the looked-up step into stage b: one copy instruction is 1 KiB of K rows or 32
-  // dims x 16 keys of V, of one page.  Slots outside the pool read slot 0 (masked later).
-  auto issue = [&](int b) {
-    auto of = [&](int u) {
-      int s = slot[0];
+  // Copies of the looked-up step into the stage at LDS byte `to`; its invalid pages, one bit
+  // each (they read slot 0).  Copy i of a wave is 1 KiB of K rows and 32 dims x 16 keys of V,
+  // both of the step's 16 keys i (D = 128) or 2 i + wave / 2.
+  auto issue = [&](uint32_t to) {
+    uint32_t bad = 0;
+    int s[UPP];
 #pragma unroll
-      for (int x = 1; x < UPP; ++x) s = u == x ? slot[x] : s;
-      return (int64_t)(valid(s) ? s : 0);
-    };
+    for (int u = 0; u < UPP; ++u) {
+      const bool ok = (uint32_t)slot[u] < (uint32_t)a.num_slots;
+      s[u] = ok ? slot[u] : 0;
+      bad |= ok ? 0u : 1u << u;
+    }
 #pragma unroll
     for (int i = 0; i < kI; ++i) {
-      const int row = (i * kThreads + wave * 64) / CPR, vi = i * kWaves + wave, kp = vi / (D / 32);
-      copy_to_lds(kbase + of(row / P) * a.k_ss, k_off[i], lds0 + (uint32_t)((b * 2 * kKC + i * kThreads + wave * 64) * 16));
-      copy_to_lds(vbase + of(kp * 16 / P) * a.v_ss, v_off[i], lds0 + (uint32_t)((b * 2 * kKC + kKC + vi * 64) * 16));
+      uint32_t x = (uint32_t)s[D == 128 ? i * 16 / P : i * 32 / P];
+      if (D == 64 && P == 16) x = wave >> 1 ? (uint32_t)s[(2 * i + 1) % UPP] : x;
+      copy_to_lds(kbase + (uint64_t)x * k_ss, k_off[i], to + (uint32_t)(i * kThreads + wave * 64) * 16);
+      copy_to_lds(vbase + (uint64_t)x * v_ss, v_off[i], to + (uint32_t)(kKC + (i * kWaves + wave) * 64) * 16);
     }
+    return bad;
   };
 
-  float m_run[NC];
+  // LDS bytes of this lane's operands in the stage that is read: K row (col >> 2) * 8 + (col &
+  // 3), chunk (4 kk + grp) ^ col, and V key group grp, dim col
+  uint32_t k_at[KT], v_at;
+#pragma unroll
+  for (int kk = 0; kk < KT; ++kk)
+    k_at[kk] = (uint32_t)(((col >> 2) * 8 + (col & 3)) * CPR + ((kk * 4 + grp) ^ (col & (CPR - 1)))) * 16;
+  v_at = (uint32_t)(kKC + (grp >> 1) * (D / 32) * 64 + (grp & 1) * 32 + col) * 16;
+  auto lds_h8 = [&](uint32_t at) { return *reinterpret_cast<const h8_t*>(reinterpret_cast<const char*>(&s_kv[0][0]) + at); };
+
+  // m_run: what a column's scores are relative to (0 until it has met a key), thr: how far a
+  // score may pass it (a column that has met no key takes any)
+  float m_run[NC], thr[NC];
   f4_t o[NC][DT], l_acc[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    m_run[c] = -INFINITY;
+    m_run[c] = 0.f;
+    thr[c] = -3.4e38f;
     l_acc[c] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[c][d] = f4_t{0.f, 0.f, 0.f, 0.f};
@@ -555,56 +576,46 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = (_Float16)1.f;
 
-  uint32_t bad = 0, bad_next = 0;                   // invalid pages of the step, of the next one
-  auto bad_of = [&]() {
-    uint32_t x = 0;
-#pragma unroll
-    for (int u = 0; u < UPP; ++u) x |= valid(slot[u]) ? 0u : 1u << u;
-    return x;
-  };
+  uint32_t bad_next = 0, stage = 0;
   if (lo < hi) {
     look_up(lo);
-    bad_next = bad_of();
-    issue(0);
+    bad_next = issue(lds0);
     look_up(lo + 1);
   }
   for (int j = lo; j < hi; ++j) {
-    const int b = (j - lo) & 1;
     stage_barrier();                                // the step is in its stage; the other one is no longer read
-    bad = bad_next;
+    const uint32_t bad = bad_next, cur = stage;
+    stage ^= kStage;
     if (j + 1 < hi) {
-      bad_next = bad_of();
-      issue(b ^ 1);
+      bad_next = issue(lds0 + stage);
       look_up(j + 2);
     }
     const int key0 = steps.at(j) * kKeys;
     // V of keys that no row sees may hold anything: zero (uniform over the workgroup; the first
     // and last steps of a tile)
-    if (bad || key0 + kKeys > steps.end || (key0 < steps.open && key0 + kKeys > a.sinks)) {
-#pragma unroll
+    if (bad || key0 + kKeys > steps.end || (WIN && key0 < steps.open && key0 + kKeys > a.sinks)) {
+#pragma unroll 1
       for (int i = 0; i < kI; ++i) {
         const int vi = i * kWaves + wave, key = vi / (D / 32) * 16 + (lane >> 5) * 8;
-        u32x4_t* x = &s_kv[b][kKC + vi * 64 + lane];
+        u32x4_t* x = reinterpret_cast<u32x4_t*>(reinterpret_cast<char*>(&s_kv[0][0]) + cur) + kKC + vi * 64 + lane;
         *x = seen_only(a, steps, key0 + key, !((bad >> (key / P)) & 1), *x);
       }
       lds_barrier();
     }
+    // nothing of the step is visible to this wave's rows
+    if (key0 > pw1 || (WIN && key0 + kKeys - 1 <= pw0 - a.window && key0 >= a.sinks)) continue;
+    const bool whole = !bad && key0 + kKeys - 1 <= pw0 && key0 + kKeys <= steps.end &&
+                       (!WIN || key0 > pw1 - a.window || key0 + kKeys <= a.sinks);
+
+    // scores of keys key0 + 32 u + 8 grp + e
+    float t[2][NC][8];
 #pragma unroll
-    for (int u = 0; u < kKeys / 32; ++u) {
-      const int k0 = key0 + u * 32, tv = k0 + grp * 8;
-      // nothing of these 32 keys is visible to this wave's rows
-      if (k0 > pw1 || k0 >= steps.end || (a.window && k0 + 31 <= pw0 - a.window && k0 >= a.sinks)) continue;
-      const bool whole = !bad && k0 + 31 <= pw0 && k0 + 32 <= steps.end &&
-                         (!a.window || k0 > pw1 - a.window || k0 + 32 <= a.sinks);
-      float sv[NC][8];
+    for (int u = 0; u < 2; ++u) {
       h8_t kf[2][KT];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int row = u * 32 + (col >> 2) * 8 + t * 4 + (col & 3);
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int kk = 0; kk < KT; ++kk)
-          kf[t][kk] = __builtin_bit_cast(h8_t, s_kv[b][row * CPR + ((kk * 4 + grp) ^ kswz<CPR>(row))]);
-      }
+        for (int kk = 0; kk < KT; ++kk) kf[y][kk] = lds_h8(cur + k_at[kk] + (uint32_t)(u * 32 + y * 4) * CPR * 16);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         f4_t s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
@@ -615,66 +626,78 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          sv[c][r] = s0[r];
-          sv[c][4 + r] = s1[r];
+          t[u][c][r] = s0[r];
+          t[u][c][4 + r] = s1[r];
         }
       }
-      if (!whole) {
+    }
+    if (!whole) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int tv = key0 + u * 32 + grp * 8;
         const bool ok = !((bad >> ((u * 32 + grp * 8) / P)) & 1);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          const int top = ok ? min(pos[c], steps.end - 1) : -1;
-          const int low = a.window ? pos[c] - a.window + 1 : 0;
+          const int n = ok ? min(pos[c], steps.end - 1) - tv : -1;             // last visible e
+          const int f = WIN ? pos[c] - a.window + 1 - tv : 0, g = WIN ? a.sinks - tv : 0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            sv[c][e] = tv + e <= top && (tv + e >= low || tv + e < a.sinks) ? sv[c][e] : -INFINITY;
+          for (int e = 0; e < 8; ++e) {
+            const bool see = (e <= n) & (!WIN | (e >= f) | (e < g));
+            t[u][c][e] = see ? t[u][c][e] : -INFINITY;
+          }
         }
       }
-      h8_t vf[DT];
+    }
+    bool raise = false;
+    float mx[NC];
 #pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const int kp = u * 2 + (grp >> 1);
-        vf[d] = __builtin_bit_cast(
-            h8_t, s_kv[b][kKC + (kp * (D / 32) + (d >> 1)) * 64 + (grp & 1) * 32 + (d & 1) * 16 + col]);
-      }
-      float mx[NC];
-      bool raise = false;
+    for (int c = 0; c < NC; ++c) {
+      mx[c] = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          t[u][c][e] = __builtin_fmaf(t[u][c][e], a.qk_scale_log2, -m_run[c]);
+          mx[c] = fmaxf(mx[c], t[u][c][e]);
+        }
+      raise |= mx[c] > thr[c];
+    }
+    if (__ballot(raise)) {
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        mx[c] = fmaxf(fmaxf(fmaxf(sv[c][0], sv[c][1]), fmaxf(sv[c][2], sv[c][3])),
-                      fmaxf(fmaxf(sv[c][4], sv[c][5]), fmaxf(sv[c][6], sv[c][7]))) * a.qk_scale_log2;
-        raise |= mx[c] > m_run[c] + kLazy;
-      }
-      if (__ballot(raise)) {
+        float m = fmaxf(mx[c], __shfl_xor(mx[c], 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const bool up = m > thr[c];
+        const float by = up ? m : 0.f;
+        const float alpha = up ? (thr[c] == kLazy ? __builtin_amdgcn_exp2f(-by) : 0.f) : 1.f;
+        m_run[c] += by;
+        thr[c] = up ? kLazy : thr[c];
+        l_acc[c] *= alpha;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          float m = fmaxf(mx[c], __shfl_xor(mx[c], 16, 64));
-          m = fmaxf(m, __shfl_xor(m, 32, 64));
-          const float m_new = fmaxf(m_run[c], m);
-          const float alpha = __builtin_amdgcn_exp2f(m_run[c] - (m_new == -INFINITY ? 0.f : m_new));
-          l_acc[c] *= alpha;
+        for (int d = 0; d < DT; ++d) o[c][d] *= alpha;
 #pragma unroll
-          for (int d = 0; d < DT; ++d) o[c][d] *= alpha;
-          m_run[c] = m_new;
-        }
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) t[u][c][e] -= by;
       }
-      // P enters the product rounded to fp16, and so do the sums (a product with ones): the
-      // rounding of a probability then moves numerator and denominator alike
+    }
+    // P enters the product rounded to fp16, and so do the sums (a product with ones): the
+    // rounding of a probability then moves numerator and denominator alike
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
       h8_t ph[NC];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const float ref = m_run[c] == -INFINITY ? 0.f : -m_run[c];
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          ph[c][e] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(sv[c][e], a.qk_scale_log2, ref));
-      }
+        for (int e = 0; e < 8; ++e) ph[c][e] = (_Float16)__builtin_amdgcn_exp2f(t[u][c][e]);
 #pragma unroll
       for (int c = 0; c < NC; ++c) l_acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[c], l_acc[c], 0, 0, 0);
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d) {
+        const h8_t vf = lds_h8(cur + v_at + (uint32_t)(u * 2 * (D / 32) * 64 + (d >> 1) * 64 + (d & 1) * 16) * 16);
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-          o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], ph[c], o[c][d], 0, 0, 0);
+        for (int c = 0; c < NC; ++c) o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[c], o[c][d], 0, 0, 0);
+      }
     }
   }
 
@@ -689,11 +712,11 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
       float* dst = a.part_o + at * D + grp * 4;
 #pragma unroll
       for (int d = 0; d < DT; ++d) *reinterpret_cast<f4_t*>(dst + d * 16) = o[c][d];
-      if (grp == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_run[c], l);
+      if (grp == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(thr[c] == kLazy ? m_run[c] : -INFINITY, l);
     } else {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int t = row / G;
-      uint16_t* dst = a.out + (int64_t)(it.start + t) * a.o_st + (int64_t)(hk * G + row - t * G) * a.o_sh + grp * 4;
+      const float inv = l == 0.f ? 0.f : 1.f / l;       // (a row that sees nothing: zeros; NaN stays)
+      const int tt = row / a.G;
+      uint16_t* dst = a.out + (int64_t)(it.start + tt) * a.o_st + (int64_t)(hk * a.G + row - tt * a.G) * a.o_sh + grp * 4;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
         *reinterpret_cast<uint2*>(dst + d * 16) = make_uint2(pack_h2(o[c][d][0] * inv, o[c][d][1] * inv),
@@ -796,7 +819,10 @@ void launch(ChunkArgs a, const Plan& p, float* ws, hipStream_t s) {
                          dim3((unsigned)(parts / 2 + 1) * (unsigned)a.Hkv, (f.tile + kMergeRows - 1) / kMergeRows),
                          dim3(kThreads), 0, s, a);
   };
-  if (p.tile.items) run(p.tile, p.tile_parts, tile_attn_kernel<D, P>);
+  if (p.tile.items) {
+    if (a.window) run(p.tile, p.tile_parts, tile_attn_kernel<D, P, true>);
+    else run(p.tile, p.tile_parts, tile_attn_kernel<D, P, false>);
+  }
   if (p.few.items) {
     if (p.few_nc == 1) run(p.few, p.few_parts, few_attn_kernel<D, P, 1>);
     else run(p.few, p.few_parts, few_attn_kernel<D, P, 2>);
@@ -837,6 +863,9 @@ extern "C" int helm_chunk_attn(const void* q, int64_t q_stride_t, int64_t q_stri
                      pool->v_head_stride >= (int64_t)P,
                  f + ": pool strides too small for the page");
   HELM_CHECK_SUPPORTED(pool->v_dim_stride * D < (1ll << 30), f + ": V dim stride too large (in-page offsets are 32-bit)");
+  HELM_CHECK_SUPPORTED(pool->k_slot_stride >= 0 && pool->k_slot_stride < (1ll << 32) && pool->v_slot_stride >= 0 &&
+                           pool->v_slot_stride < (1ll << 32),
+                       f + ": slot strides must be below 2^32 elements");
   HELM_CHECK_SUPPORTED(q_stride_t % 8 == 0 && q_stride_h % 8 == 0 && out_stride_t % 4 == 0 && out_stride_h % 4 == 0 &&
                            pool->k_slot_stride % 8 == 0 && pool->k_head_stride % 8 == 0 &&
                            pool->v_slot_stride % 8 == 0 && pool->v_head_stride % 8 == 0 && pool->v_dim_stride % 8 == 0,
@@ -855,7 +884,7 @@ extern "C" int helm_chunk_attn(const void* q, int64_t q_stride_t, int64_t q_stri
   a.k = static_cast<const uint16_t*>(pool->k); a.k_ss = pool->k_slot_stride; a.k_hs = pool->k_head_stride;
   a.v = static_cast<const uint16_t*>(pool->v);
   a.v_ss = pool->v_slot_stride; a.v_hs = pool->v_head_stride; a.v_ds = pool->v_dim_stride;
-  a.num_slots = pool->num_slots;
+  a.num_slots = (int32_t)std::min<int64_t>(pool->num_slots, 0x7fffffff);   // (slots are int32)
   a.page_table = page_table; a.pt_stride = pt_stride; a.seq_lens = seq_lens; a.q_starts = q_starts;
   a.N = N; a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.P = P; a.max_pages = max_pages;
   a.max_new = std::min(max_new, N);
