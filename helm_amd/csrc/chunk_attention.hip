@@ -38,14 +38,20 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void_t;
 
-// How one of the two kernels cuts the sequences it takes.
+// How one of the two kernels cuts the sequences it takes, and its partials: sums [Hkv][parts]
+// [tile rows][D], not normalised, then [Hkv][parts][tile rows][2] running maximum and sum.
 struct Form {
   int lo, hi;          // it takes sequences of lo < rows <= hi
-  int tile;            // rows of a tile
-  int step;            // keys of a step
+  int tile, step;      // log2 of the rows of a tile, of the keys of a step
   int min_steps;       // least steps of a piece
   int want;            // pieces of a kv head that fill the chip
-  int items;           // workgroups of a kv head that the grid has
+  float per_want;      // 1 / want and a little, so that work * per_want is not below work / want
+  int most_keys;       // that a tile can see
+  int items;           // workgroups of a kv head that the grid has (0: not launched)
+  int parts;           // partials of a kv head (0: no sequence can have two pieces)
+  int cut_tiles;       // tiles of several pieces, at most
+  float* part_o;
+  float* part_ml;
 };
 
 struct ChunkArgs {
@@ -66,61 +72,49 @@ struct ChunkArgs {
   int window, sinks;                    // window 0: none
   int covered;                          // tokens that the table has room for
   float qk_scale_log2;
-  Form f;
-  float* part_o;                        // [Hkv][split items][tile rows][D] sums, not normalised
-  float* part_ml;                       // [Hkv][split items][tile rows][2] running maximum, sum
-  int split_items;                      // of a kv head
+  Form f[2];                            // few rows, many rows
 };
+constexpr int kFew = 0, kMany = 1;
 
 struct Seq {
   int start, n, rows, len;              // first row, new tokens, rows (token, head) to do, tokens
-  int tiles, steps;
+  int tiles, steps;                     // 0: not this form's
 };
 
-__device__ __forceinline__ Seq seq_of(const ChunkArgs& a, int i) {
-  Seq s{0, 0, 0, 0, 0, 0};
-  if (i >= a.B) return s;
-  int s0 = i, e = i + 1;
+__device__ __forceinline__ Seq seq_of(const ChunkArgs& a, const Form& f, int i) {
+  const int j = min(i, a.B - 1);
+  int s0 = j, e = j + 1;
+  const int len = a.seq_lens[j];
   if (a.q_starts) {
-    s0 = a.q_starts[i];
-    e = a.q_starts[i + 1];
+    s0 = a.q_starts[j];
+    e = a.q_starts[j + 1];
   }
-  s.len = a.seq_lens[i];
+  Seq s;
+  s.len = len;
   s.start = min(max(s0, 0), a.N);
   s.n = max(min(e, a.N) - s.start, 0);
   s.rows = min(s.n, a.max_new) * a.G;
-  if (s.rows <= a.f.lo || s.rows > a.f.hi) {
-    s.rows = 0;
-    return s;
-  }
-  s.tiles = (s.rows + a.f.tile - 1) / a.f.tile;
-  int keys = min(max(s.len, 0), a.covered);
-  // (at most: a tile's window begins at its first row's and ends at its last row)
-  if (a.window) keys = (int)min((int64_t)keys, (int64_t)a.window + a.sinks + a.f.tile / a.G + 2 * a.f.step);
-  s.steps = max((keys + a.f.step - 1) / a.f.step, 1);
+  const bool mine = i < a.B && s.rows > f.lo && s.rows <= f.hi;
+  s.tiles = mine ? (s.rows + (1 << f.tile) - 1) >> f.tile : 0;
+  s.steps = mine ? max((min(max(len, 0), f.most_keys) + (1 << f.step) - 1) >> f.step, 1) : 0;
   return s;
 }
 
-// Sum over a workgroup's threads, to all of them, and this thread's exclusive prefix.
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t& before, uint64_t* s_wave) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t inc = v;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t o = __shfl_up(inc, off, 64);
-    if (lane >= off) inc += o;
-  }
-  __syncthreads();
-  if (lane == 63) s_wave[wave] = inc;
-  __syncthreads();
-  uint64_t total = 0, base = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) base += s_wave[w];
-    total += s_wave[w];
-  }
-  before = base + inc - v;
-  return total;
+// Wave-wide sums by DPP moves: the total, and the sum up to and with a lane.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = dpp_add<0x111, 0xF>(v);           // row_shr 1, 2, 4, 8: within rows of 16
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);           // row_bcast 15: rows 1 and 3 take the row before
+  return dpp_add<0x143, 0xC>(v);        // row_bcast 31: rows 2 and 3 take the first half
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 
 struct Item {
@@ -129,57 +123,103 @@ struct Item {
   int part;                             // partial of its tile's piece 0
 };
 
-// The want-th (tile, piece) of a kv head, or with MERGE the want-th tile of more than one
-// piece; false where there are fewer.  Pieces of a sequence: its steps over the mean number
-// of steps of a place, rounded.  W = sum of tiles x steps and m = ceil(W / want) give at most
-// W / m + tiles <= want + tiles items, and at most 4/3 want in sequences of several pieces
-// (those have steps >= 3/2 m).
-template <bool MERGE>
-__device__ __forceinline__ bool find_item(const ChunkArgs& a, int want, Item& it) {
-  __shared__ uint64_t s_wave[kWaves];
-  __shared__ Item s_item;
-  const int tid = threadIdx.x;
-  uint64_t work = 0, unused;
-  Seq s = seq_of(a, tid);
-  for (int i = tid; i < a.B; i += kThreads) {
-    if (i != tid) s = seq_of(a, i);
-    work += (uint64_t)s.tiles * (uint64_t)s.steps;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_of(float v, float none) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ float dpp_sum(float v) {      // of a wave, the same in all lanes
+  v += dpp_of<0x111, 0xF>(v, 0.f);
+  v += dpp_of<0x112, 0xF>(v, 0.f);
+  v += dpp_of<0x114, 0xF>(v, 0.f);
+  v += dpp_of<0x118, 0xF>(v, 0.f);
+  v += dpp_of<0x142, 0xA>(v, 0.f);
+  v += dpp_of<0x143, 0xC>(v, 0.f);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+__device__ __forceinline__ float dpp_max(float v) {
+  v = fmaxf(v, dpp_of<0x111, 0xF>(v, v));
+  v = fmaxf(v, dpp_of<0x112, 0xF>(v, v));
+  v = fmaxf(v, dpp_of<0x114, 0xF>(v, v));
+  v = fmaxf(v, dpp_of<0x118, 0xF>(v, v));
+  v = fmaxf(v, dpp_of<0x142, 0xA>(v, v));
+  v = fmaxf(v, dpp_of<0x143, 0xC>(v, v));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// Pieces of a tile of so many steps, at most m each.
+__device__ __forceinline__ int pieces_of(int steps, float inv_m) {
+  return min(max((int)ceilf((float)steps * inv_m), 1), kMaxPieces);
+}
+
+// Most steps of a piece, 1 / m returned: with W the sum of tiles x steps of a kv head, the least m
+// of W / want x 1, 1.25, 1.5, 2 whose pieces find places all at once (a second round of
+// workgroups would cost as much as the first, and more pieces more partials); with more tiles than
+// places only what is twice as long as the mean is cut.  So there are at most want + tiles items,
+// and at most want in tiles of several pieces.
+__device__ __forceinline__ float inv_steps(const ChunkArgs& a, const Form& f, const Seq& first) {
+  const int lane = threadIdx.x & 63;
+  float work = (float)first.tiles * (float)first.steps, tiles = (float)first.tiles;
+  for (int i = 64; i < a.B; i += 64) {
+    const Seq s = seq_of(a, f, i + lane);
+    work += (float)s.tiles * (float)s.steps;
+    tiles += (float)s.tiles;
   }
-  if (a.B > kThreads) s = seq_of(a, tid);
-  const uint64_t W = block_scan(work, unused, s_wave);
-  const uint64_t mean = (W + a.f.want - 1) / a.f.want;
-  const int m = (int)min(max(mean, (uint64_t)a.f.min_steps), (uint64_t)1 << 30);
-  if (tid == 0) s_item.pieces = 0;
-  uint64_t base = 0;                    // low half: items before, high half: partials before
-  for (int i0 = 0; i0 < a.B; i0 += kThreads) {
-    if (i0 > 0) s = seq_of(a, i0 + tid);
-    const int pieces = min(max((s.steps + m / 2) / m, 1), kMaxPieces);
-    const uint32_t parts = pieces > 1 ? (uint32_t)(s.tiles * pieces) : 0u;
-    const uint32_t mine = MERGE ? (pieces > 1 ? (uint32_t)s.tiles : 0u) : (uint32_t)(s.tiles * pieces);
-    uint64_t before;
-    const uint64_t total = block_scan((uint64_t)mine | (uint64_t)parts << 32, before, s_wave);
-    before += base;
-    const int at = want - (int)(uint32_t)before;
-    if (s.tiles > 0 && at >= 0 && at < (int)mine) {
-      const int per = MERGE ? 1 : pieces;
-      const int tile = s.tiles - 1 - at / per;          // the tiles with the most keys first
-      s_item = Item{i0 + tid, s.start, s.n, s.rows, s.len, tile, at % per, pieces,
-                    (int)(before >> 32) + tile * pieces};
+  const float mean = dpp_sum(work) * f.per_want;
+  float m = 2.f * mean;
+  if (m > (float)f.min_steps && dpp_sum(tiles) < (float)f.want) {
+#pragma unroll 1
+    for (float by = 1.f; by < 2.f; by += 0.25f) {
+      const float inv = 1.f / fmaxf(mean * by, (float)f.min_steps);
+      float n = (float)(first.tiles * pieces_of(first.steps, inv));
+      for (int i = 64; i < a.B; i += 64) {
+        const Seq s = seq_of(a, f, i + lane);
+        n += (float)(s.tiles * pieces_of(s.steps, inv));
+      }
+      if (dpp_sum(n) <= (float)f.want) {
+        m = mean * by;
+        break;
+      }
     }
-    base += total;
-    if ((int)(uint32_t)base > want) break;              // (uniform)
   }
-  __syncthreads();
-  it.seq = __builtin_amdgcn_readfirstlane(s_item.seq);
-  it.start = __builtin_amdgcn_readfirstlane(s_item.start);
-  it.n = __builtin_amdgcn_readfirstlane(s_item.n);
-  it.rows = __builtin_amdgcn_readfirstlane(s_item.rows);
-  it.len = __builtin_amdgcn_readfirstlane(s_item.len);
-  it.tile = __builtin_amdgcn_readfirstlane(s_item.tile);
-  it.piece = __builtin_amdgcn_readfirstlane(s_item.piece);
-  it.pieces = __builtin_amdgcn_readfirstlane(s_item.pieces);
-  it.part = __builtin_amdgcn_readfirstlane(s_item.part);
-  return it.pieces > 0;
+  return 1.f / fmaxf(m, (float)f.min_steps);
+}
+
+// The want-th (tile, piece) of a kv head, or with MERGE the want-th tile of more than one
+// piece; false where there are fewer.  Every wave finds it by itself, a lane per sequence.
+template <bool FEW, bool MERGE>
+__device__ __forceinline__ bool find_item(const ChunkArgs& a, int want, Item& it) {
+  const Form& f = a.f[FEW ? kFew : kMany];
+  const int lane = threadIdx.x & 63;
+  const Seq first = seq_of(a, f, lane);
+  const float inv = inv_steps(a, f, first);
+  uint32_t items = 0, parts = 0;        // of the sequences before
+  for (int i0 = 0; i0 < a.B; i0 += 64) {
+    const Seq s = i0 == 0 ? first : seq_of(a, f, i0 + lane);
+    const int pieces = pieces_of(s.steps, inv);
+    const uint32_t own_parts = pieces > 1 ? (uint32_t)(s.tiles * pieces) : 0u;
+    const uint32_t mine = MERGE ? (pieces > 1 ? (uint32_t)s.tiles : 0u) : (uint32_t)(s.tiles * pieces);
+    const uint32_t upto = items + wave_scan(mine), parts_upto = parts + wave_scan(own_parts);
+    const uint64_t hit = __ballot(upto > (uint32_t)want);
+    if (hit) {                          // the first sequence that reaches it
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      it.seq = i0 + l;
+      it.pieces = (int)lane_of((uint32_t)pieces, l);
+      it.start = (int)lane_of((uint32_t)s.start, l);
+      it.n = (int)lane_of((uint32_t)s.n, l);
+      it.rows = (int)lane_of((uint32_t)s.rows, l);
+      it.len = (int)lane_of((uint32_t)s.len, l);
+      const int at = want - (int)(lane_of(upto, l) - lane_of(mine, l));
+      const int per = MERGE ? 1 : it.pieces;
+      const int t = (int)((uint32_t)at / (uint32_t)per);
+      it.tile = (int)lane_of((uint32_t)s.tiles, l) - 1 - t;      // the tiles with the most keys first
+      it.piece = at - t * per;
+      it.part = (int)(lane_of(parts_upto, l) - lane_of(own_parts, l)) + it.tile * it.pieces;
+      return true;
+    }
+    items = lane_of(upto, 63);
+    parts = lane_of(parts_upto, 63);
+  }
+  return false;
 }
 
 // The keys that rows at positions p0 .. p1 see, in steps: those of the sinks, then those of
@@ -212,16 +252,14 @@ __device__ __forceinline__ h8_t ld_h8(const uint16_t* p) {
   return __builtin_bit_cast(h8_t, *reinterpret_cast<const u32x4_t*>(p));
 }
 
-// The bits of the pair of keys 2 q, 2 q + 1 past `key` that some row may see.
-__device__ __forceinline__ uint32_t pair_bits(const ChunkArgs& a, const Steps& s, int key, int q) {
-  auto seen = [&](int k) { return k < s.end && (k >= s.open || k < a.sinks); };
-  return (seen(key + 2 * q) ? 0x0000ffffu : 0u) | (seen(key + 2 * q + 1) ? 0xffff0000u : 0u);
-}
-__device__ __forceinline__ u32x4_t seen_only(const ChunkArgs& a, const Steps& s, int key, bool page_ok, u32x4_t w) {
-  w.x &= page_ok ? pair_bits(a, s, key, 0) : 0u;
-  w.y &= page_ok ? pair_bits(a, s, key, 1) : 0u;
-  w.z &= page_ok ? pair_bits(a, s, key, 2) : 0u;
-  w.w &= page_ok ? pair_bits(a, s, key, 3) : 0u;
+// Of eight keys from `key` on, in an operand's words: the bits of those that some row may see.
+__device__ __forceinline__ u32x4_t seen_bits(const ChunkArgs& a, const Steps& s, int key, bool page_ok) {
+  u32x4_t w;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    auto seen = [&](int k) { return page_ok & (k < s.end) & ((k >= s.open) | (k < a.sinks)); };
+    w[q] = (seen(key + 2 * q) ? 0x0000ffffu : 0u) | (seen(key + 2 * q + 1) ? 0xffff0000u : 0u);
+  }
   return w;
 }
 
@@ -230,21 +268,28 @@ __device__ __forceinline__ u32x4_t seen_only(const ChunkArgs& a, const Steps& s,
 // NC tiles of 16 rows.  Steps of 32 keys, one wave each, round robin; K's and V's registers
 // are filled again as soon as they have been read.  P is split into fp16 hi + lo parts, so
 // that the product keeps fp32's accuracy (the matrix cores wait for memory anyway).
+template <int D, int NC>
+struct FewLds {
+  float o[kWaves][16 * NC][D];
+  float m[kWaves][16 * NC], l[kWaves][16 * NC];
+};
+
 template <int D, int P, int NC>
-__global__ __launch_bounds__(kThreads, 2) void few_attn_kernel(ChunkArgs a) {
+__device__ __forceinline__ void few_body(const ChunkArgs& a, int hk, int item, FewLds<D, NC>& lds) {
   constexpr int KT = D / 32;
   constexpr int DT = D / 16;
   constexpr int kStep = 32;
-  __shared__ float s_m[kWaves][16 * NC], s_l[kWaves][16 * NC];
-  __shared__ __attribute__((aligned(16))) float s_o[kWaves][16 * NC][D];
+  auto& s_m = lds.m;
+  auto& s_l = lds.l;
+  auto& s_o = lds.o;
+  const Form& f = a.f[kFew];
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int col = lane & 15, grp = lane >> 4;
-  const int hk = (int)(blockIdx.x % (unsigned)a.Hkv);
   Item it;
-  if (!find_item<false>(a, (int)(blockIdx.x / (unsigned)a.Hkv), it)) return;
+  if (!find_item<true, false>(a, item, it)) return;
   const int G = a.G;
   const int p0 = it.len - it.n, p1 = p0 + it.rows / G - 1;      // (one tile a sequence)
   const Steps steps = steps_of(a, p0, p1, it.len, kStep);
@@ -330,9 +375,9 @@ __global__ __launch_bounds__(kThreads, 2) void few_attn_kernel(ChunkArgs a) {
     }
     if constexpr (kMore) load_k(nk, tok(i + 1));
     if (!whole) {
+      const u32x4_t bits = seen_bits(a, steps, tv, ok);
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-        vb[d] = __builtin_bit_cast(h8_t, seen_only(a, steps, tv, ok, __builtin_bit_cast(u32x4_t, vb[d])));
+      for (int d = 0; d < DT; ++d) vb[d] = __builtin_bit_cast(h8_t, __builtin_bit_cast(u32x4_t, vb[d]) & bits);
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -342,7 +387,7 @@ __global__ __launch_bounds__(kThreads, 2) void few_attn_kernel(ChunkArgs a) {
         const int low = a.window ? pos[c] - a.window + 1 : 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          sv[c][j] = tv + j <= top && (tv + j >= low || tv + j < a.sinks) ? sv[c][j] : -INFINITY;
+          sv[c][j] = (tv + j <= top) & ((tv + j >= low) | (tv + j < a.sinks)) ? sv[c][j] : -INFINITY;
       }
       const float mx = fmaxf(fmaxf(fmaxf(sv[c][0], sv[c][1]), fmaxf(sv[c][2], sv[c][3])),
                              fmaxf(fmaxf(sv[c][4], sv[c][5]), fmaxf(sv[c][6], sv[c][7]))) * a.qk_scale_log2;
@@ -416,9 +461,9 @@ __global__ __launch_bounds__(kThreads, 2) void few_attn_kernel(ChunkArgs a) {
       for (int e = 0; e < 4; ++e) n[e] = fmaf(f, x[e], n[e]);
     }
     if (it.pieces > 1) {
-      const int64_t at = ((int64_t)hk * a.split_items + it.part + it.piece) * a.f.tile + row;
-      *reinterpret_cast<f4_t*>(a.part_o + at * D + d) = n;
-      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+      const int64_t at = ((int64_t)hk * f.parts + it.part + it.piece) * (16 * NC) + row;
+      *reinterpret_cast<f4_t*>(f.part_o + at * D + d) = n;
+      if (d == 0) *reinterpret_cast<float2*>(f.part_ml + at * 2) = make_float2(m, l);
     } else {
       const float inv = l == 0.f ? 0.f : 1.f / l;       // (a row that sees nothing: zeros; NaN stays)
       const int t = row / G;
@@ -466,9 +511,14 @@ __device__ __forceinline__ int kswz(int r) {
   return ((r & 3) | (((r >> 3) & 3) << 2)) & (CPR - 1);
 }
 
+template <int D>
+struct TileLds {
+  u32x4_t kv[2][2 * kKeys * D / 8];
+};
+
 // WIN: there is a window.
 template <int D, int P, bool WIN>
-__global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
+__device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, TileLds<D>& lds) {
   constexpr int NC = kNC;
   constexpr int KT = D / 32;
   constexpr int DT = D / 16;
@@ -477,15 +527,15 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
   constexpr int kI = kKC / kThreads;                // copies of a thread for each
   constexpr int UPP = kKeys / P;                    // pages of a step
   constexpr uint32_t kStage = 2 * kKC * 16;         // bytes of a stage
-  __shared__ __attribute__((aligned(16))) u32x4_t s_kv[2][2 * kKC];
+  auto& s_kv = lds.kv;
+  const Form& f = a.f[kMany];
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int col = lane & 15, grp = lane >> 4;
-  const int hk = (int)(blockIdx.x % (unsigned)a.Hkv);
   Item it;
-  if (!find_item<false>(a, (int)(blockIdx.x / (unsigned)a.Hkv), it)) return;
+  if (!find_item<false, false>(a, item, it)) return;
   const int r0 = it.tile * kTile, rw = r0 + wave * 16 * NC;       // first row of the tile, of this wave
   const int base = it.len - it.n;                                 // position of the sequence's first row
   const Steps steps = steps_of(a, base + r0 / a.G, base + (min(r0 + kTile, it.rows) - 1) / a.G, it.len, kKeys);
@@ -598,7 +648,7 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
       for (int i = 0; i < kI; ++i) {
         const int vi = i * kWaves + wave, key = vi / (D / 32) * 16 + (lane >> 5) * 8;
         u32x4_t* x = reinterpret_cast<u32x4_t*>(reinterpret_cast<char*>(&s_kv[0][0]) + cur) + kKC + vi * 64 + lane;
-        *x = seen_only(a, steps, key0 + key, !((bad >> (key / P)) & 1), *x);
+        *x &= seen_bits(a, steps, key0 + key, !((bad >> (key / P)) & 1));
       }
       lds_barrier();
     }
@@ -639,10 +689,10 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const int n = ok ? min(pos[c], steps.end - 1) - tv : -1;             // last visible e
-          const int f = WIN ? pos[c] - a.window + 1 - tv : 0, g = WIN ? a.sinks - tv : 0;
+          const int w0 = WIN ? pos[c] - a.window + 1 - tv : 0, sk = WIN ? a.sinks - tv : 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const bool see = (e <= n) & (!WIN | (e >= f) | (e < g));
+            const bool see = (e <= n) & (!WIN | (e >= w0) | (e < sk));
             t[u][c][e] = see ? t[u][c][e] : -INFINITY;
           }
         }
@@ -708,11 +758,11 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
     if (row >= it.rows) continue;
     const float l = l_acc[c][0];
     if (it.pieces > 1) {
-      const int64_t at = ((int64_t)hk * a.split_items + it.part + it.piece) * kTile + (row - r0);
-      float* dst = a.part_o + at * D + grp * 4;
+      const int64_t at = ((int64_t)hk * f.parts + it.part + it.piece) * kTile + (row - r0);
+      float* dst = f.part_o + at * D + grp * 4;
 #pragma unroll
       for (int d = 0; d < DT; ++d) *reinterpret_cast<f4_t*>(dst + d * 16) = o[c][d];
-      if (grp == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(thr[c] == kLazy ? m_run[c] : -INFINITY, l);
+      if (grp == 0) *reinterpret_cast<float2*>(f.part_ml + at * 2) = make_float2(thr[c] == kLazy ? m_run[c] : -INFINITY, l);
     } else {
       const float inv = l == 0.f ? 0.f : 1.f / l;       // (a row that sees nothing: zeros; NaN stays)
       const int tt = row / a.G;
@@ -725,43 +775,101 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
   }
 }
 
-// ── joining the pieces ───────────────────────────────────────────────────────
+// ── the kernels ──────────────────────────────────────────────────────────────
 
-constexpr int kMergeRows = 32;           // of a workgroup
-
-// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over a tile's pieces, four dims a thread;
-// bound by reading the partials once.
-template <int D>
-__global__ __launch_bounds__(kThreads) void chunk_merge_kernel(ChunkArgs a) {
+template <int D, int P, int NC>
+__global__ __launch_bounds__(kThreads, NC == 1 ? 3 : 2) void few_attn_kernel(ChunkArgs a) {
+  __shared__ __attribute__((aligned(16))) FewLds<D, NC> lds;
+  few_body<D, P, NC>(a, (int)(blockIdx.x % (unsigned)a.Hkv), (int)(blockIdx.x / (unsigned)a.Hkv), lds);
+}
+template <int D, int P, bool WIN>
+__global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
+  __shared__ __attribute__((aligned(16))) TileLds<D> lds;
+  tile_body<D, P, WIN>(a, (int)(blockIdx.x % (unsigned)a.Hkv), (int)(blockIdx.x / (unsigned)a.Hkv), lds);
+}
+// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over a tile's pieces.  Bound by latency: the
+// plan, the maxima, the partials.  A workgroup takes R rows (grid.y of them a tile, the tiles of
+// few rows first); its threads are 4 dims of a row each, and where those are fewer than 256, groups
+// that take the pieces in turn.
+template <int D, int R>
+__global__ __launch_bounds__(kThreads) void chunk_merge_kernel(ChunkArgs a, int few_tiles) {
+  constexpr int S = R * (D / 4);        // threads of a group
+  constexpr int PG = S < kThreads ? kThreads / S : 1;
+  constexpr int U = S < kThreads ? 1 : S / kThreads;     // (row, 4 dims) of a thread
+  __shared__ float s_w[R][kMaxPieces], s_inv[R];
+  __shared__ __attribute__((aligned(16))) f4_t s_n[PG][S];
+  const int tid = threadIdx.x;
   const int hk = (int)(blockIdx.x % (unsigned)a.Hkv);
+  int want = (int)(blockIdx.x / (unsigned)a.Hkv);
+  const bool few = want < few_tiles;
+  if (!few) want -= few_tiles;
+  const Form& f = a.f[few ? kFew : kMany];
   Item it;
-  if (!find_item<true>(a, (int)(blockIdx.x / (unsigned)a.Hkv), it)) return;
-  const int r0 = it.tile * a.f.tile;
-  const int rows = min(it.rows - r0, a.f.tile);
-  const int64_t base = (int64_t)hk * a.split_items + it.part;
-  for (int idx = threadIdx.x; idx < kMergeRows * (D / 4); idx += kThreads) {
-    const int row = blockIdx.y * kMergeRows + idx / (D / 4), d = idx % (D / 4) * 4;
-    if (row >= rows) break;
-    const float* ml = a.part_ml + (base * a.f.tile + row) * 2;
-    const float* po = a.part_o + (base * a.f.tile + row) * D + d;
-    const int64_t stride = a.f.tile;
-    float m = -INFINITY;
-    for (int p = 0; p < it.pieces; ++p) m = fmaxf(m, ml[p * stride * 2]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    f4_t n = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    for (int p = 0; p < it.pieces; ++p) {
-      const float2 x = *reinterpret_cast<const float2*>(ml + p * stride * 2);
-      const f4_t y = *reinterpret_cast<const f4_t*>(po + p * stride * D);
-      const float f = __builtin_amdgcn_exp2f(x.x - ref);
-      l = fmaf(f, x.y, l);
+  if (!(few ? find_item<true, true>(a, want, it) : find_item<false, true>(a, want, it))) return;
+  const int r0 = it.tile << f.tile, y0 = (int)blockIdx.y * R;
+  const int rows = min(it.rows - r0, 1 << f.tile) - y0;       // of this workgroup and on
+  if (rows <= 0) return;
+  const int64_t base = ((int64_t)hk * f.parts + it.part) << f.tile;
+  // lane p of a wave: piece p of a row
+  for (int r = tid >> 6; r < min(rows, R); r += kWaves) {
+    const int p = tid & 63;
+    float2 x = make_float2(-INFINITY, 0.f);
+    if (p < it.pieces)
+      x = *reinterpret_cast<const float2*>(f.part_ml + (base + ((int64_t)p << f.tile) + y0 + r) * 2);
+    const float m = dpp_max(x.x);
+    const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.x - m);
+    const float l = dpp_sum(w * x.y);
+    s_w[r][p] = w;
+    if (p == 0) s_inv[r] = l == 0.f ? 0.f : 1.f / l;    // (a row that sees nothing: zeros; NaN stays)
+  }
+  __syncthreads();
+  const int pg = tid / S;
+  // each thread's U rows together: their loads do not wait for one another
+  const float* po[U];
+  f4_t n[U];
+  int at[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) n[e] = fmaf(f, y[e], n[e]);
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int t = (r0 + row) / a.G;
-    *reinterpret_cast<uint2*>(a.out + (int64_t)(it.start + t) * a.o_st + (int64_t)(hk * a.G + r0 + row - t * a.G) * a.o_sh + d) =
-        make_uint2(pack_h2(n[0] * inv, n[1] * inv), pack_h2(n[2] * inv, n[3] * inv));
+  for (int u = 0; u < U; ++u) {
+    at[u] = tid % S + u * kThreads;
+    po[u] = f.part_o + (base + y0 + min(at[u] / (D / 4), rows - 1)) * D + at[u] % (D / 4) * 4;
+    n[u] = f4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  const int64_t stride = (int64_t)D << f.tile;
+  constexpr int L = 8 / U;              // pieces at a time
+  for (int p0 = pg; p0 < it.pieces; p0 += L * PG) {
+    f4_t y[L][U];
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      if (p0 + i * PG < it.pieces) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) y[i][u] = *reinterpret_cast<const f4_t*>(po[u] + (p0 + i * PG) * stride);
+      }
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      if (p0 + i * PG < it.pieces) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float w = s_w[min(at[u] / (D / 4), rows - 1)][p0 + i * PG];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) n[u][e] = fmaf(w, y[i][u][e], n[u][e]);
+        }
+      }
+  }
+  if constexpr (PG > 1) {
+    s_n[pg][at[0]] = n[0];
+    __syncthreads();
+    if (pg > 0) return;
+#pragma unroll
+    for (int g = 1; g < PG; ++g) n[0] += s_n[g][at[0]];
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int r = at[u] / (D / 4), d = at[u] % (D / 4) * 4;
+    if (r >= rows) break;
+    const float inv = s_inv[r];
+    const int row = r0 + y0 + r, t = row / a.G;
+    *reinterpret_cast<uint2*>(a.out + (int64_t)(it.start + t) * a.o_st + (int64_t)(hk * a.G + row - t * a.G) * a.o_sh + d) =
+        make_uint2(pack_h2(n[u][0] * inv, n[u][1] * inv), pack_h2(n[u][2] * inv, n[u][3] * inv));
   }
 }
 
@@ -769,17 +877,20 @@ __global__ __launch_bounds__(kThreads) void chunk_merge_kernel(ChunkArgs a) {
 
 // How a call's sequences are shared between the two kernels and cut, from what the host knows.
 struct Plan {
-  Form few, tile;                       // items 0: not launched
-  int few_nc;
-  int few_parts, tile_parts;            // partials of a kv head (0: no sequence can have two pieces)
+  Form f[2];
+  int few_nc;                           // 16-row tiles of the few-row kernel
 };
 
-Form form_of(int lo, int hi, int tile, int step, int min_steps, int want, int64_t tiles) {
-  return {lo, hi, tile, step, min_steps, want, (int)std::min<int64_t>(tiles + want, 1 << 28)};
-}
-int parts_of(const Form& f, int64_t keys) {
-  const int64_t steps = (keys + f.step - 1) / f.step;
-  return f.items > 0 && 2 * steps >= 3 * (int64_t)f.min_steps ? (4 * f.want + 2) / 3 : 0;
+Form form_of(int lo, int hi, int tile, int step, int min_steps, int want, int64_t tiles, int64_t keys) {
+  Form f{};
+  f.lo = lo; f.hi = hi; f.tile = tile; f.step = step; f.min_steps = min_steps; f.want = want;
+  f.per_want = 1.00002f / (float)want;
+  f.most_keys = (int)keys;
+  const int64_t steps = (keys + (1 << step) - 1) >> step;
+  f.items = (int)std::min<int64_t>(tiles + (steps > min_steps ? want + 1 : 0), 1 << 28);
+  f.parts = steps > min_steps ? (int)std::min<int64_t>(want + 2, tiles * kMaxPieces) : 0;
+  f.cut_tiles = (int)std::min<int64_t>(f.parts / 2, tiles);
+  return f;
 }
 
 Plan plan_of(int N, int B, int Hq, int Hkv, int P, int max_pages, int max_new, int window, int sinks) {
@@ -787,46 +898,50 @@ Plan plan_of(int N, int B, int Hq, int Hkv, int P, int max_pages, int max_new, i
   const int G = Hq / Hkv;
   const int64_t most = (int64_t)std::min(max_new, N) * G;         // rows of a sequence
   const int seqs = std::min(B, N);
-  const int few = G > 32 || (B == 1 && most > 32) ? 0 : most <= 16 ? 16 : 32;
+  const int few = G > 32 || (B == 1 && most > 32) ? 0 : most <= 16 ? 16 : most <= 32 || G > 16 ? 32 : 16;
   p.few_nc = few / 16;
-  int64_t keys = (int64_t)max_pages * P;
-  auto bound = [&](const Form& f) {
-    return window ? std::min<int64_t>(keys, (int64_t)window + sinks + f.tile / G + 2 * f.step) : keys;
+  // keys that a tile of so many rows can see: its window begins at its first row's and ends at
+  // its last row, both rounded to steps
+  auto keys = [&](int rows, int step) {
+    const int64_t all = (int64_t)max_pages * P;
+    return window ? std::min<int64_t>(all, (int64_t)window + sinks + rows / G + 2 * step) : all;
   };
-  if (few) {
-    p.few = form_of(0, few, few, 32, 4, std::max(1, 512 / Hkv), seqs);
-    p.few_parts = parts_of(p.few, bound(p.few));
-  }
-  if (most > few) {
-    p.tile = form_of(few, 1 << 30, kTile, kKeys, 4, std::max(1, 512 / Hkv), (int64_t)N * G / kTile + seqs);
-    p.tile_parts = parts_of(p.tile, bound(p.tile));
-  }
+  const int want = std::max(1, 512 / Hkv);
+  if (few) p.f[kFew] = form_of(0, few, few == 16 ? 4 : 5, 5, 4, want, seqs, keys(few, 32));
+  if (most > few)
+    p.f[kMany] = form_of(few, 1 << 30, 7, 6, 4, want, (int64_t)N * G / kTile + seqs, keys(kTile, kKeys));
   return p;
 }
-int64_t part_floats(const Form& f, int parts, int Hkv, int D) { return (int64_t)Hkv * parts * f.tile * (D + 2); }
+int64_t part_floats(const Form& f, int Hkv, int D) { return ((int64_t)Hkv * f.parts << f.tile) * (D + 2); }
 
 template <int D, int P>
 void launch(ChunkArgs a, const Plan& p, float* ws, hipStream_t s) {
-  auto run = [&](const Form& f, int parts, auto kernel) {
-    a.f = f;
-    a.split_items = parts;
-    a.part_o = ws;
-    a.part_ml = ws + (int64_t)a.Hkv * parts * f.tile * D;
-    ws += part_floats(f, parts, a.Hkv, D);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)f.items * (unsigned)a.Hkv), dim3(kThreads), 0, s, a);
-    if (parts)
-      hipLaunchKernelGGL((chunk_merge_kernel<D>),
-                         dim3((unsigned)(parts / 2 + 1) * (unsigned)a.Hkv, (f.tile + kMergeRows - 1) / kMergeRows),
-                         dim3(kThreads), 0, s, a);
+  for (int w = 0; w < 2; ++w) {
+    a.f[w] = p.f[w];
+    a.f[w].part_o = ws;
+    a.f[w].part_ml = ws + ((int64_t)a.Hkv * p.f[w].parts << p.f[w].tile) * D;
+    ws += part_floats(p.f[w], a.Hkv, D);
+  }
+  const Form &few = p.f[kFew], &many = p.f[kMany];
+  auto run = [&](auto kernel, int items) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)items * (unsigned)a.Hkv), dim3(kThreads), 0, s, a);
   };
-  if (p.tile.items) {
-    if (a.window) run(p.tile, p.tile_parts, tile_attn_kernel<D, P, true>);
-    else run(p.tile, p.tile_parts, tile_attn_kernel<D, P, false>);
+  if (many.items) {
+    if (a.window) run(tile_attn_kernel<D, P, true>, many.items);
+    else run(tile_attn_kernel<D, P, false>, many.items);
   }
-  if (p.few.items) {
-    if (p.few_nc == 1) run(p.few, p.few_parts, few_attn_kernel<D, P, 1>);
-    else run(p.few, p.few_parts, few_attn_kernel<D, P, 2>);
+  if (few.items) {
+    if (p.few_nc == 1) run(few_attn_kernel<D, P, 1>, few.items);
+    else run(few_attn_kernel<D, P, 2>, few.items);
   }
+  const int few_tiles = few.cut_tiles, tiles = few_tiles + many.cut_tiles;
+  if (tiles == 0) return;
+  if (many.parts)
+    hipLaunchKernelGGL((chunk_merge_kernel<D, 32>), dim3((unsigned)tiles * (unsigned)a.Hkv, kTile / 32), dim3(kThreads), 0,
+                       s, a, few_tiles);
+  else
+    hipLaunchKernelGGL((chunk_merge_kernel<D, 2>), dim3((unsigned)tiles * (unsigned)a.Hkv, (1 << few.tile) / 2),
+                       dim3(kThreads), 0, s, a, few_tiles);
 }
 
 }  // namespace
@@ -837,7 +952,7 @@ extern "C" int64_t helm_chunk_attn_workspace_bytes(int N, int B, int Hq, int Hkv
       window < 0 || sinks < 0)
     return 0;
   const Plan p = plan_of(N, B, Hq, Hkv, P, max_pages, max_new, window, sinks);
-  return (part_floats(p.few, p.few_parts, Hkv, D) + part_floats(p.tile, p.tile_parts, Hkv, D)) * (int64_t)sizeof(float);
+  return (part_floats(p.f[kFew], Hkv, D) + part_floats(p.f[kMany], Hkv, D)) * (int64_t)sizeof(float);
 }
 
 extern "C" int helm_chunk_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, const helm_kv_pool* pool,
@@ -877,7 +992,7 @@ extern "C" int helm_chunk_attn(const void* q, int64_t q_stride_t, int64_t q_stri
   const int64_t need = helm_chunk_attn_workspace_bytes(N, B, Hq, Hkv, D, P, max_pages, max_new, window, sinks);
   HELM_CHECK_ARG(need == 0 || (workspace && helm::aligned16(workspace) && workspace_bytes >= need),
                  f + ": this call needs " + std::to_string(need) + " bytes of 16-byte aligned workspace");
-  HELM_CHECK_SUPPORTED((int64_t)std::max(p.few.items, p.tile.items) * Hkv < (1ll << 31), f + ": too many workgroups");
+  HELM_CHECK_SUPPORTED(((int64_t)p.f[kFew].items + p.f[kMany].items) * Hkv < (1ll << 31), f + ": too many workgroups");
   ChunkArgs a{};
   a.q = static_cast<const uint16_t*>(q); a.q_st = q_stride_t; a.q_sh = q_stride_h;
   a.out = static_cast<uint16_t*>(out); a.o_st = out_stride_t; a.o_sh = out_stride_h;
