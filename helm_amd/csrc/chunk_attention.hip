@@ -100,23 +100,6 @@ __device__ __forceinline__ Seq seq_of(const ChunkArgs& a, const Form& f, int i) 
   return s;
 }
 
-// Wave-wide sums by DPP moves: the total, and the sum up to and with a lane.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
-  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  v = dpp_add<0x111, 0xF>(v);           // row_shr 1, 2, 4, 8: within rows of 16
-  v = dpp_add<0x112, 0xF>(v);
-  v = dpp_add<0x114, 0xF>(v);
-  v = dpp_add<0x118, 0xF>(v);
-  v = dpp_add<0x142, 0xA>(v);           // row_bcast 15: rows 1 and 3 take the row before
-  return dpp_add<0x143, 0xC>(v);        // row_bcast 31: rows 2 and 3 take the first half
-}
-__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
-  return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
-}
-
 struct Item {
   int seq, start, n, rows, len;         // the sequence: index, first row, new tokens, rows to do, tokens
   int tile, piece, pieces;
@@ -222,22 +205,27 @@ __device__ __forceinline__ bool find_item(const ChunkArgs& a, int want, Item& it
   return false;
 }
 
-// The keys that rows at positions p0 .. p1 see, in steps: those of the sinks, then those of
-// the window.  Step j covers the keys from at(j) * step on.
+// The keys that a tile's rows, at positions p0 .. p1, see, in steps: those of the sinks, then those
+// of the window.  Step j covers the keys from at(j) * step on.
 struct Steps {
   int sink, first, count;               // steps of the sinks; first step of the window; all
-  int end;                              // no row sees a key from end on,
-  int open;                             // nor one in [sinks, open)
+  int end;                              // the tile sees no key from end on
+  // No row of the sequence sees a key in [sinks, open) or from close on: their V may be anything.
+  // (V of other keys that a row does not see meets a probability of 0.)
+  int open, close;
   __device__ __forceinline__ int at(int j) const { return j < sink ? j : first + j - sink; }
 };
-__device__ __forceinline__ Steps steps_of(const ChunkArgs& a, int p0, int p1, int len, int step) {
-  Steps s{0, 0, 0, 0, 0};
-  s.end = max(min(min(p1 + 1, len), a.covered), 0);
+__device__ __forceinline__ Steps steps_of(const ChunkArgs& a, const Item& it, int p0, int p1, int step) {
+  Steps s{0, 0, 0, 0, 0, 0};
+  const int base = it.len - it.n;       // position of the sequence's first row
+  const int all = min(it.len, a.covered);
+  s.end = max(min(p1 + 1, all), 0);
+  s.close = max(min(base + (int)((uint32_t)it.rows / (uint32_t)a.G), all), 0);
   const int last = (s.end + step - 1) / step;
   s.count = last;
   if (a.window) {
-    s.open = max(p0 - a.window + 1, 0);
-    s.first = s.open / step;
+    s.open = max(base - a.window + 1, 0);
+    s.first = max(p0 - a.window + 1, 0) / step;
     s.sink = min((min(a.sinks, s.end) + step - 1) / step, s.first);
     s.count = s.sink + max(last - s.first, 0);
   }
@@ -257,7 +245,7 @@ __device__ __forceinline__ u32x4_t seen_bits(const ChunkArgs& a, const Steps& s,
   u32x4_t w;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    auto seen = [&](int k) { return page_ok & (k < s.end) & ((k >= s.open) | (k < a.sinks)); };
+    auto seen = [&](int k) { return page_ok & (k < s.close) & ((k >= s.open) | (k < a.sinks)); };
     w[q] = (seen(key + 2 * q) ? 0x0000ffffu : 0u) | (seen(key + 2 * q + 1) ? 0xffff0000u : 0u);
   }
   return w;
@@ -292,7 +280,7 @@ __device__ __forceinline__ void few_body(const ChunkArgs& a, int hk, int item, F
   if (!find_item<true, false>(a, item, it)) return;
   const int G = a.G;
   const int p0 = it.len - it.n, p1 = p0 + it.rows / G - 1;      // (one tile a sequence)
-  const Steps steps = steps_of(a, p0, p1, it.len, kStep);
+  const Steps steps = steps_of(a, it, p0, p1, kStep);
   const int lo = (int)((int64_t)steps.count * it.piece / it.pieces);
   const int hi = (int)((int64_t)steps.count * (it.piece + 1) / it.pieces);
   const int mine = hi - lo > wave ? (hi - lo - 1 - wave) / kWaves + 1 : 0;
@@ -538,7 +526,7 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
   if (!find_item<false, false>(a, item, it)) return;
   const int r0 = it.tile * kTile, rw = r0 + wave * 16 * NC;       // first row of the tile, of this wave
   const int base = it.len - it.n;                                 // position of the sequence's first row
-  const Steps steps = steps_of(a, base + r0 / a.G, base + (min(r0 + kTile, it.rows) - 1) / a.G, it.len, kKeys);
+  const Steps steps = steps_of(a, it, base + r0 / a.G, base + (min(r0 + kTile, it.rows) - 1) / a.G, kKeys);
   const int lo = (int)((int64_t)steps.count * it.piece / it.pieces);
   const int hi = (int)((int64_t)steps.count * (it.piece + 1) / it.pieces);
   // positions of this wave's rows (none: every key is behind its last one)
@@ -642,8 +630,8 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
     }
     const int key0 = steps.at(j) * kKeys;
     // V of keys that no row sees may hold anything: zero (uniform over the workgroup; the first
-    // and last steps of a tile)
-    if (bad || key0 + kKeys > steps.end || (WIN && key0 < steps.open && key0 + kKeys > a.sinks)) {
+    // and last steps of a sequence)
+    if (bad || key0 + kKeys > steps.close || (WIN && key0 < steps.open && key0 + kKeys > a.sinks)) {
 #pragma unroll 1
       for (int i = 0; i < kI; ++i) {
         const int vi = i * kWaves + wave, key = vi / (D / 32) * 16 + (lane >> 5) * 8;
@@ -688,12 +676,15 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
         const bool ok = !((bad >> ((u * 32 + grp * 8) / P)) & 1);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          const int n = ok ? min(pos[c], steps.end - 1) - tv : -1;             // last visible e
-          const int w0 = WIN ? pos[c] - a.window + 1 - tv : 0, sk = WIN ? a.sinks - tv : 0;
+          // bit e: key tv + e is visible (v_bfe spreads it over a word, v_bfi picks)
+          auto below = [](int x) { return (1u << min(max(x, 0), 8)) - 1u; };    // bits e < x
+          uint32_t see = below(min(pos[c], steps.end - 1) - tv + 1);
+          if (WIN) see &= ~below(pos[c] - a.window + 1 - tv) | below(a.sinks - tv);
+          see = ok ? see : 0u;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const bool see = (e <= n) & (!WIN | (e >= w0) | (e < sk));
-            t[u][c][e] = see ? t[u][c][e] : -INFINITY;
+            const uint32_t all = (uint32_t)__builtin_amdgcn_sbfe((int)see, e, 1);
+            t[u][c][e] = __uint_as_float((__float_as_uint(t[u][c][e]) & all) | (0xff800000u & ~all));
           }
         }
       }

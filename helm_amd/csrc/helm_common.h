@@ -164,4 +164,21 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// Sum over the lanes up to and with this one, by DPP moves (every lane active).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = dpp_add<0x111, 0xF>(v);           // row_shr 1, 2, 4, 8: within rows of 16
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);           // row_bcast 15: rows 1 and 3 take the row before
+  return dpp_add<0x143, 0xC>(v);        // row_bcast 31: rows 2 and 3 take the first half
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+
 constexpr float kLog2e = 1.4426950408889634f;

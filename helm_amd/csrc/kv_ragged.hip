@@ -145,59 +145,177 @@ __global__ __launch_bounds__(256) void rope_rows_kernel(RopeArgs a) {
   for (int j = 0; j < J; ++j) dst[lane + 64 * j] = f2h(y[j]);
 }
 
-// The same for many rows: a workgroup takes 16 rows x 8 heads.  Bound by moving qkv once; the
-// form above spends its time on a sine, a cosine and a 64-bit reduction per element of
-// every head and on a store per V element in a line of its own.  Here
-//   * the rows' sequences are counted by ballots, their angles' factors made once, into LDS
-//   * q / k heads: 8 dims of a row a lane (16-byte loads and stores), so the pair (i, i + r/2) is
-//     r/16 lanes away: r a multiple of 16, or interleaved pairs
-//   * v heads: 16 tokens of a head are turned through LDS, so that neighbouring lanes write
-//     neighbouring tokens of a dim (V pages are [D][P])
-constexpr int kPT = 16, kPH = 8;
+// Sum over the LANES (8 or 16) neighbouring lanes of a row, in all of them.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v) {
+  auto with = [&](auto ctrl) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  with(std::integral_constant<int, 0xB1>{});     // quad_perm [1,0,3,2]
+  with(std::integral_constant<int, 0x4E>{});     // quad_perm [2,3,0,1]
+  with(std::integral_constant<int, 0x141>{});    // row_half_mirror
+  if constexpr (LANES == 16) with(std::integral_constant<int, 0x140>{});   // row_mirror
+  return v;
+}
+
+// The same for many rows.  Bound by moving qkv once; the form above spends its time on a sine, a
+// cosine and a 64-bit reduction per element of every head and on a store per V element in a line of
+// its own.  Here a workgroup takes 256 / (D / 8) tokens, D / 8 lanes a token, and
+//   * of q and k kPH heads one after another: a lane holds the same four pairs of each, so their
+//     factors are made once and stay in registers and no value changes lanes.  Its 8 dims are two
+//     groups of 4: at 4 l and r/2 + 4 l of the r rotated dims (r a multiple of 8), behind them, or
+//     with interleaved pairs everywhere, 8 neighbours.
+//   * of v kVH heads of 16 tokens that lie in one page from a multiple of 16 on (whatever rows they
+//     are), turned through LDS: V pages are [D][P], and 32 bytes of a dim written by two workgroups
+//     are two partial writes of two L2s.  2000 + 129 + 1297 + 500 tokens of 40 + 8 + 8 heads (112 MB):
+//     with rows' own blocks of 16 and 2-byte stores 26.6 us
+constexpr int kPH = 16, kVH = 8;
 constexpr int kPad = 2;                  // halves between the tokens of a head's V in LDS
 
+// The want-th block of 16 positions that holds new tokens: its sequence's first row and position,
+// the positions [lo, hi) of it that are new, and the slot (-1: none); false where there are fewer.
+struct VBlock {
+  int row, slot, at, lo, hi;             // position p is row `row + p`; the block begins at `at`
+};
+__device__ __forceinline__ bool v_block(const RopeArgs& a, int want, VBlock& v) {
+  const int lane = threadIdx.x & 63;
+  uint32_t before = 0;
+  for (int i0 = 0; i0 < a.B; i0 += 64) {
+    const int i = min(i0 + lane, a.B - 1);
+    int s0 = i, e = i + 1;
+    const int len = a.seq_lens[i];
+    if (a.q_starts) {
+      s0 = a.q_starts[i];
+      e = a.q_starts[i + 1];
+    }
+    const int first = len - (e - s0);    // position of row s0
+    // (rows outside qkv and positions outside the table are none)
+    const int lo = max(first + max(-s0, 0), 0), hi = (int)min((int64_t)(len - max(e - a.N, 0)), (int64_t)a.max_pages * a.P);
+    const uint32_t n = i0 + lane < a.B && e > s0 && hi > lo ? (uint32_t)((hi - 1) / 16 - lo / 16 + 1) : 0u;
+    const uint32_t upto = before + wave_scan(n);
+    const uint64_t hit = __ballot(upto > (uint32_t)want);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      v.lo = (int)lane_of((uint32_t)lo, l);
+      v.hi = (int)lane_of((uint32_t)hi, l);
+      v.row = (int)lane_of((uint32_t)(s0 - first), l);
+      v.at = (v.lo / 16 + want - (int)(lane_of(upto, l) - lane_of(n, l))) * 16;
+      const int s = a.page_table[(int64_t)(i0 + l) * a.pt_stride + v.at / a.P];
+      v.slot = s >= 0 && s < a.pool.num_slots ? s : -1;
+      v.lo = max(v.lo, v.at);
+      v.hi = min(v.hi, v.at + 16);
+      return true;
+    }
+    before = lane_of(upto, 63);
+  }
+  return false;
+}
+
 template <int D>
-__global__ __launch_bounds__(256) void rope_tile_kernel(RopeArgs a) {
-  constexpr int RL = D / 8;              // lanes of a row
-  constexpr int RW = 256 / RL;           // rows at a time
-  constexpr int kIter = kPT * kPH / RW;
-  constexpr int HALF = D / 2;
-  __shared__ __attribute__((aligned(16))) float2 s_cs[kPT][HALF];
-  __shared__ int s_cnt[4][kPT];
-  __shared__ Place s_place[kPT];
-  __shared__ uint16_t s_v[kPH][kPT][D + kPad];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int li = tid % RL, lr = tid / RL;
-  const int row0 = blockIdx.x * kPT, nt = min(kPT, a.N - row0);
-  const int groups_qk = (a.Hq + a.Hkv + kPH - 1) / kPH;
-  const bool v_heads = (int)blockIdx.y >= groups_qk;
-  const int h0 = v_heads ? (blockIdx.y - groups_qk) * kPH : blockIdx.y * kPH;   // of its kind
-  const int nh = min(kPH, (v_heads ? a.Hkv : a.Hq + a.Hkv) - h0);
-  uint4 raw[kIter];                      // row i * RW + lr of the group: token-major
+__device__ __forceinline__ void v_tile(const RopeArgs& a, int block, int h0, uint16_t* s_v) {
+  constexpr int RL = D / 8;              // lanes of a token
+  constexpr int kIter = 16 * kVH * RL / 256;
+  const int tid = threadIdx.x;
+  VBlock v;
+  if (!v_block(a, block, v) || v.slot < 0) return;
+  const int nh = min(kVH, a.Hkv - h0);
+  uint4 x[kIter];
 #pragma unroll
   for (int i = 0; i < kIter; ++i) {
-    const int r = i * RW + lr, t = min(r / kPH, nt - 1), h = min(r % kPH, nh - 1);
-    raw[i] = ld_nt16(a.qkv + (int64_t)(row0 + t) * a.qkv_st + (int64_t)((v_heads ? a.Hq + a.Hkv : 0) + h0 + h) * D + li * 8);
+    const int c = i * 256 + tid, h = min(c / (16 * RL), nh - 1), p = min(max(v.at + c / RL % 16, v.lo), v.hi - 1);
+    x[i] = ld_nt16(a.qkv + (int64_t)(v.row + p) * a.qkv_st + (int64_t)(a.Hq + a.Hkv + h0 + h) * D + c % RL * 8);
   }
-  uint4 qw{}, kw{};
-  if (!v_heads && a.q_norm_w) {
-    qw = *reinterpret_cast<const uint4*>(a.q_norm_w + li * 8);
-    kw = *reinterpret_cast<const uint4*>(a.k_norm_w + li * 8);
+#pragma unroll
+  for (int i = 0; i < kIter; ++i) {
+    const int c = i * 256 + tid;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(s_v + c / RL * (D + kPad) + c % RL * 8);
+    dst[0] = x[i].x;
+    dst[1] = x[i].y;
+    dst[2] = x[i].z;
+    dst[3] = x[i].w;
   }
-  if (a.q_starts) {
+  __syncthreads();
+  uint16_t* base = a.pool.v + (int64_t)v.slot * a.pool.v_ss + (int64_t)h0 * a.pool.v_hs + v.at % a.P;
+  // neighbouring lanes: the two halves of a dim's 16 tokens, then the next dim
+  const int t0 = (tid & 1) * 8;
+  const bool whole = v.lo <= v.at + t0 && v.hi >= v.at + t0 + 8;
+#pragma unroll 2
+  for (int i = tid >> 1; i < nh * D; i += 128) {
+    const int h = i / D, d = i % D;
+    const uint16_t* src = s_v + (h * 16 + t0) * (D + kPad) + d;
+    uint16_t* dst = base + (int64_t)h * a.pool.v_hs + (int64_t)d * a.pool.v_ds + t0;
+    uint16_t y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = src[e * (D + kPad)];
+    if (whole) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16,
+                                                  y[4] | (uint32_t)y[5] << 16, y[6] | (uint32_t)y[7] << 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (v.at + t0 + e >= v.lo && v.at + t0 + e < v.hi) dst[e] = y[e];
+    }
+  }
+}
+
+// The first v_items workgroups are those of v.
+template <int D>
+__global__ __launch_bounds__(256, 4) void rope_tile_kernel(RopeArgs a, int v_items, int qk_tiles) {
+  constexpr int RL = D / 8;
+  constexpr int PT = 256 / RL;           // tokens of a workgroup
+  __shared__ int s_cnt[4][PT];
+  __shared__ Place s_place[PT];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v[kVH * 16 * (D + kPad)];
+  if ((int)blockIdx.x < v_items) {
+    const int groups = (a.Hkv + kVH - 1) / kVH;
+    v_tile<D>(a, (int)(blockIdx.x / (unsigned)groups), (int)(blockIdx.x % (unsigned)groups) * kVH, s_v);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int li = tid % RL, lt = tid / RL;
+  const int x = (int)blockIdx.x - v_items, group = x / qk_tiles;
+  const int row0 = (x - group * qk_tiles) * PT, nt = min(PT, a.N - row0);
+  const int h0 = group * kPH, nh = min(kPH, a.Hq + a.Hkv - h0);
+  const int half = a.rot / 2;
+  int dA = li * 8, dB = dA + 4;
+  if (!a.inter && li < a.rot / 8) dA = li * 4, dB = half + li * 4;
+  const uint16_t* src = a.qkv + (int64_t)(row0 + min(lt, nt - 1)) * a.qkv_st + (int64_t)h0 * D;
+  constexpr int kAhead = 8;              // heads on the way
+  uint2 rA[kAhead], rB[kAhead];
+  auto load = [&](int i, int h) {
+    rA[i] = *reinterpret_cast<const uint2*>(src + (int64_t)min(h, nh - 1) * D + dA);
+    rB[i] = *reinterpret_cast<const uint2*>(src + (int64_t)min(h, nh - 1) * D + dB);
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) load(i, i);
+  uint2 wq[2], wk[2];
+  float freq[4];
+  bool turn[4];                          // the lane's pairs 4 li + e: (dA + e, dB + e), or neighbours
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    turn[e] = (a.inter || li < a.rot / 8) && li * 4 + e < half;
+    freq[e] = turn[e] ? a.inv_freq[li * 4 + e] : 0.f;
+  }
+  if (a.q_norm_w) {
+    wq[0] = *reinterpret_cast<const uint2*>(a.q_norm_w + dA);
+    wq[1] = *reinterpret_cast<const uint2*>(a.q_norm_w + dB);
+    wk[0] = *reinterpret_cast<const uint2*>(a.k_norm_w + dA);
+    wk[1] = *reinterpret_cast<const uint2*>(a.k_norm_w + dB);
+  }
+  if (a.q_starts) {                      // how many sequences end at or before each row
     int cnt = 0;                         // lane t: of row0 + t
     for (int i0 = wave * 64; i0 < a.B; i0 += 256) {
       const int e = i0 + lane < a.B ? a.q_starts[i0 + lane + 1] : 0x7fffffff;
-#pragma unroll
-      for (int t = 0; t < kPT; ++t) {
+#pragma unroll 8
+      for (int t = 0; t < PT; ++t) {
         const int c = __popcll(__ballot(e <= row0 + t));
         cnt += lane == t ? c : 0;
       }
     }
-    if (lane < kPT) s_cnt[wave][lane] = cnt;
+    if (lane < PT) s_cnt[wave][lane] = cnt;
+    __syncthreads();
   }
-  __syncthreads();
-  if (tid < kPT) {
+  if (tid < PT) {
     const int row = row0 + tid;
     int b = row;
     if (a.q_starts) b = s_cnt[0][tid] + s_cnt[1][tid] + s_cnt[2][tid] + s_cnt[3][tid];
@@ -209,88 +327,59 @@ __global__ __launch_bounds__(256) void rope_tile_kernel(RopeArgs a) {
     s_place[tid] = p;
   }
   __syncthreads();
-  if (v_heads) {
+  const Place p = s_place[lt];
+  float2 cs[4];
 #pragma unroll
-    for (int i = 0; i < kIter; ++i) {
-      const int r = i * RW + lr;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(&s_v[r % kPH][r / kPH][li * 8]);
-      dst[0] = raw[i].x;
-      dst[1] = raw[i].y;
-      dst[2] = raw[i].z;
-      dst[3] = raw[i].w;
-    }
-    __syncthreads();
-    const int t = tid % kPT;             // neighbouring lanes: neighbouring tokens
-    const Place p = s_place[t];
-    if (p.slot < 0) return;
-    uint16_t* base = a.pool.v + (int64_t)p.slot * a.pool.v_ss + (int64_t)h0 * a.pool.v_hs + p.off;
-    for (int h = 0; h < nh; ++h)
-#pragma unroll 4
-      for (int d = tid / kPT; d < D; d += 256 / kPT)
-        base[(int64_t)h * a.pool.v_hs + (int64_t)d * a.pool.v_ds] = s_v[h][t][d];
-    return;
-  }
-  const int half = a.rot / 2;
-  for (int i = tid; i < kPT * half; i += 256) {
-    const int t = i / half, f = i - t * half;
-    s_cs[t][f] = rope_factors(s_place[t].pos, a.inv_freq[f], a.rope_scale);
-  }
-  __syncthreads();
+  for (int e = 0; e < 4; ++e) cs[e] = rope_factors(p.pos, freq[e], a.rope_scale);
+  uint16_t* kdst = a.pool.k + (int64_t)max(p.slot, 0) * a.pool.k_ss + p.off * D;
+  uint16_t* qdst = a.q_out + (int64_t)(row0 + lt) * a.Hq * D;
+#pragma unroll 1
+  for (int h8 = 0; h8 < nh; h8 += kAhead) {
 #pragma unroll
-  for (int i = 0; i < kIter; ++i) {
-    const int r = i * RW + lr, t = r / kPH, h = h0 + r % kPH;
-    const bool live = t < nt && r % kPH < nh;
-    const bool is_q = h < a.Hq;
-    const uint32_t rw[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-    float x[8];
+    for (int i = 0; i < kAhead; ++i) {
+      const int h = h0 + h8 + i;
+      const bool is_q = h < a.Hq;
+      float x[8] = {lo_h(rA[i].x), hi_h(rA[i].x), lo_h(rA[i].y), hi_h(rA[i].y),
+                    lo_h(rB[i].x), hi_h(rB[i].x), lo_h(rB[i].y), hi_h(rB[i].y)};
+      if (h8 + kAhead < nh) load(i, h8 + kAhead + i);
+      if (a.q_norm_w) {
+        float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[2 * e] = lo_h(rw[e]);
-      x[2 * e + 1] = hi_h(rw[e]);
-    }
-    if (a.q_norm_w) {
-      float ss = 0.f;
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+        const float rstd = rsqrtf(row_sum<RL>(ss) / (float)D + a.eps);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-      for (int off = RL / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
-      const float rstd = rsqrtf(ss / (float)D + a.eps);
-      const uint32_t ww[4] = {is_q ? qw.x : kw.x, is_q ? qw.y : kw.y, is_q ? qw.z : kw.z, is_q ? qw.w : kw.w};
+        for (int g = 0; g < 2; ++g) {
+          const uint32_t w0 = is_q ? wq[g].x : wk[g].x, w1 = is_q ? wq[g].y : wk[g].y;
+          x[4 * g] = x[4 * g] * rstd * lo_h(w0);
+          x[4 * g + 1] = x[4 * g + 1] * rstd * hi_h(w0);
+          x[4 * g + 2] = x[4 * g + 2] * rstd * lo_h(w1);
+          x[4 * g + 3] = x[4 * g + 3] * rstd * hi_h(w1);
+        }
+      }
+      float y[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[2 * e] = x[2 * e] * rstd * lo_h(ww[e]);
-        x[2 * e + 1] = x[2 * e + 1] * rstd * hi_h(ww[e]);
+        const float u = a.inter ? x[2 * e] : x[e], v = a.inter ? x[2 * e + 1] : x[4 + e];
+        const float yu = turn[e] ? fmaf(u, cs[e].x, -v * cs[e].y) : u, yv = turn[e] ? fmaf(v, cs[e].x, u * cs[e].y) : v;
+        if (a.inter) {
+          y[2 * e] = yu;
+          y[2 * e + 1] = yv;
+        } else {
+          y[e] = yu;
+          y[4 + e] = yv;
+        }
       }
-    }
-    float y[8];
-    const int d0 = li * 8;
-    if (a.inter) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool turn = d0 + 2 * e < a.rot;
-        const float2 cs = turn ? s_cs[t][d0 / 2 + e] : make_float2(1.f, 0.f);
-        y[2 * e] = turn ? fmaf(x[2 * e], cs.x, -x[2 * e + 1] * cs.y) : x[2 * e];
-        y[2 * e + 1] = turn ? fmaf(x[2 * e + 1], cs.x, x[2 * e] * cs.y) : x[2 * e + 1];
+      const uint2 oA = make_uint2(pack_h2(y[0], y[1]), pack_h2(y[2], y[3]));
+      const uint2 oB = make_uint2(pack_h2(y[4], y[5]), pack_h2(y[6], y[7]));
+      if (lt >= nt || h8 + i >= nh) continue;
+      if (is_q) {
+        if (p.seq < 0) continue;
+        *reinterpret_cast<uint2*>(qdst + h * D + dA) = oA;
+        *reinterpret_cast<uint2*>(qdst + h * D + dB) = oB;
+      } else if (p.slot >= 0) {
+        *reinterpret_cast<uint2*>(kdst + (int64_t)(h - a.Hq) * a.pool.k_hs + dA) = oA;
+        *reinterpret_cast<uint2*>(kdst + (int64_t)(h - a.Hq) * a.pool.k_hs + dB) = oB;
       }
-    } else {
-      const bool turn = d0 < a.rot, first = d0 < half;     // (whole lanes: half is a multiple of 8)
-      const int f0 = first ? d0 : d0 - half;
-      const int from = lane + (first ? half / 8 : -(half / 8));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float partner = __shfl(x[e], from & 63, 64);
-        const float2 cs = turn ? s_cs[t][f0 + e] : make_float2(1.f, 0.f);
-        y[e] = turn ? fmaf(x[e], cs.x, (first ? -partner : partner) * cs.y) : x[e];
-      }
-    }
-    if (!live) continue;
-    const Place p = s_place[t];
-    const uint4 out = make_uint4(pack_h2(y[0], y[1]), pack_h2(y[2], y[3]), pack_h2(y[4], y[5]), pack_h2(y[6], y[7]));
-    if (is_q) {
-      if (p.seq >= 0) *reinterpret_cast<uint4*>(a.q_out + ((int64_t)(row0 + t) * a.Hq + h) * D + d0) = out;
-    } else if (p.slot >= 0) {
-      *reinterpret_cast<uint4*>(a.pool.k + (int64_t)p.slot * a.pool.k_ss + (int64_t)(h - a.Hq) * a.pool.k_hs +
-                                p.off * D + d0) = out;
     }
   }
 }
@@ -512,12 +601,16 @@ extern "C" int helm_rope_append(const void* qkv, int64_t qkv_stride_t, const voi
   a.inter = interleaved != 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t rows = (int64_t)N * (Hq + 2 * Hkv);
-  const bool tiles = rows >= kTileRows && (a.inter || rotary_dim % 16 == 0);
+  const bool tiles = rows >= kTileRows && (a.inter || rotary_dim % 8 == 0);
   auto go = [&](auto d_tag) {
     constexpr int Dc = decltype(d_tag)::value;
     if (tiles) {
-      const dim3 grid((unsigned)((N + kPT - 1) / kPT), (unsigned)((Hq + Hkv + kPH - 1) / kPH + (Hkv + kPH - 1) / kPH));
-      hipLaunchKernelGGL((rope_tile_kernel<Dc>), grid, dim3(256), 0, s, a);
+      constexpr int pt = 256 / (Dc / 8);
+      const int qk_tiles = (N + pt - 1) / pt, groups = (Hq + Hkv + kPH - 1) / kPH;
+      // a sequence's n tokens lie in at most n / 16 + 2 blocks
+      const int64_t v_items = ((int64_t)N / 16 + 2 * (int64_t)std::min(B, N)) * ((Hkv + kVH - 1) / kVH);
+      hipLaunchKernelGGL((rope_tile_kernel<Dc>), dim3((unsigned)(v_items + (int64_t)qk_tiles * groups)), dim3(256), 0, s, a,
+                         (int)v_items, qk_tiles);
     } else {
       hipLaunchKernelGGL((rope_rows_kernel<Dc>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
     }
