@@ -778,6 +778,16 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
   __shared__ __attribute__((aligned(16))) TileLds<D> lds;
   tile_body<D, P, WIN>(a, (int)(blockIdx.x % (unsigned)a.Hkv), (int)(blockIdx.x / (unsigned)a.Hkv), lds);
 }
+// Both forms in one launch, the many rows' workgroups first: those of few rows wait for memory and
+// fill the places that are left.
+template <int D, int P, bool WIN>
+__global__ __launch_bounds__(kThreads, 2) void both_attn_kernel(ChunkArgs a) {
+  __shared__ __attribute__((aligned(16))) union { FewLds<D, 1> few; TileLds<D> tile; } lds;
+  const int hk = (int)(blockIdx.x % (unsigned)a.Hkv), x = (int)(blockIdx.x / (unsigned)a.Hkv);
+  if (x < a.f[kMany].items) tile_body<D, P, WIN>(a, hk, x, lds.tile);
+  else few_body<D, P, 1>(a, hk, x - a.f[kMany].items, lds.few);
+}
+
 // out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over a tile's pieces.  Bound by latency: the
 // plan, the maxima, the partials.  A workgroup takes R rows (grid.y of them a tile, the tiles of
 // few rows first); its threads are 4 dims of a row each, and where those are fewer than 256, groups
@@ -917,11 +927,14 @@ void launch(ChunkArgs a, const Plan& p, float* ws, hipStream_t s) {
   auto run = [&](auto kernel, int items) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)items * (unsigned)a.Hkv), dim3(kThreads), 0, s, a);
   };
-  if (many.items) {
+  if (many.items && few.items && p.few_nc == 1) {
+    if (a.window) run(both_attn_kernel<D, P, true>, many.items + few.items);
+    else run(both_attn_kernel<D, P, false>, many.items + few.items);
+  } else if (many.items) {
     if (a.window) run(tile_attn_kernel<D, P, true>, many.items);
     else run(tile_attn_kernel<D, P, false>, many.items);
   }
-  if (few.items) {
+  if (few.items && !(many.items && p.few_nc == 1)) {
     if (p.few_nc == 1) run(few_attn_kernel<D, P, 1>, few.items);
     else run(few_attn_kernel<D, P, 2>, few.items);
   }
