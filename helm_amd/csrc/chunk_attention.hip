@@ -70,11 +70,17 @@ struct ChunkArgs {
   const int32_t* q_starts;              // null: one row per sequence
   int N, B, Hq, Hkv, G, P, max_pages, max_new;
   int window, sinks;                    // window 0: none
+  uint32_t mul_g;                       // 2^32 / G + 1 (G = 1: 0)
   int covered;                          // tokens that the table has room for
   float qk_scale_log2;
   Form f[2];                            // few rows, many rows
 };
 constexpr int kFew = 0, kMany = 1;
+
+// Token of a row (token, head): x / G as one high product, exact while x G < 2^32.
+__device__ __forceinline__ int token_of(const ChunkArgs& a, int row) {
+  return a.mul_g ? (int)__umulhi((uint32_t)row, a.mul_g) : row;
+}
 
 struct Seq {
   int start, n, rows, len;              // first row, new tokens, rows (token, head) to do, tokens
@@ -220,7 +226,7 @@ __device__ __forceinline__ Steps steps_of(const ChunkArgs& a, const Item& it, in
   const int base = it.len - it.n;       // position of the sequence's first row
   const int all = min(it.len, a.covered);
   s.end = max(min(p1 + 1, all), 0);
-  s.close = max(min(base + (int)((uint32_t)it.rows / (uint32_t)a.G), all), 0);
+  s.close = max(min(base + token_of(a, it.rows), all), 0);
   const int last = (s.end + step - 1) / step;
   s.count = last;
   if (a.window) {
@@ -279,7 +285,7 @@ __device__ __forceinline__ void few_body(const ChunkArgs& a, int hk, int item, F
   Item it;
   if (!find_item<true, false>(a, item, it)) return;
   const int G = a.G;
-  const int p0 = it.len - it.n, p1 = p0 + it.rows / G - 1;      // (one tile a sequence)
+  const int p0 = it.len - it.n, p1 = p0 + token_of(a, it.rows) - 1;      // (one tile a sequence)
   const Steps steps = steps_of(a, it, p0, p1, kStep);
   const int lo = (int)((int64_t)steps.count * it.piece / it.pieces);
   const int hi = (int)((int64_t)steps.count * (it.piece + 1) / it.pieces);
@@ -302,7 +308,7 @@ __device__ __forceinline__ void few_body(const ChunkArgs& a, int hk, int item, F
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int row = min(c * 16 + col, it.rows - 1);
-    const int t = row / G;
+    const int t = token_of(a, row);
     pos[c] = p0 + t;
     const uint16_t* qp = a.q + (int64_t)(it.start + t) * a.q_st + (int64_t)(hk * G + row - t * G) * a.q_sh + grp * 8;
 #pragma unroll
@@ -454,7 +460,7 @@ __device__ __forceinline__ void few_body(const ChunkArgs& a, int hk, int item, F
       if (d == 0) *reinterpret_cast<float2*>(f.part_ml + at * 2) = make_float2(m, l);
     } else {
       const float inv = l == 0.f ? 0.f : 1.f / l;       // (a row that sees nothing: zeros; NaN stays)
-      const int t = row / G;
+      const int t = token_of(a, row);
       *reinterpret_cast<uint2*>(a.out + (int64_t)(it.start + t) * a.o_st + (int64_t)(hk * G + row - t * G) * a.o_sh + d) =
           make_uint2(pack_h2(n[0] * inv, n[1] * inv), pack_h2(n[2] * inv, n[3] * inv));
     }
@@ -526,24 +532,11 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
   if (!find_item<false, false>(a, item, it)) return;
   const int r0 = it.tile * kTile, rw = r0 + wave * 16 * NC;       // first row of the tile, of this wave
   const int base = it.len - it.n;                                 // position of the sequence's first row
-  const Steps steps = steps_of(a, it, base + r0 / a.G, base + (min(r0 + kTile, it.rows) - 1) / a.G, kKeys);
+  const Steps steps = steps_of(a, it, base + token_of(a, r0), base + token_of(a, min(r0 + kTile, it.rows) - 1), kKeys);
   const int lo = (int)((int64_t)steps.count * it.piece / it.pieces);
   const int hi = (int)((int64_t)steps.count * (it.piece + 1) / it.pieces);
   // positions of this wave's rows (none: every key is behind its last one)
-  const int pw0 = base + rw / a.G, pw1 = rw < it.rows ? base + (min(rw + 16 * NC, it.rows) - 1) / a.G : -1;
-
-  int pos[NC];
-  h8_t qb[NC][KT];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int row = min(rw + c * 16 + col, it.rows - 1);
-    const int t = row / a.G;
-    pos[c] = base + t;
-    const uint16_t* qp =
-        a.q + (int64_t)(it.start + t) * a.q_st + (int64_t)(hk * a.G + row - t * a.G) * a.q_sh + grp * 8;
-#pragma unroll
-    for (int kk = 0; kk < KT; ++kk) qb[c][kk] = ld_h8(qp + kk * 32);
-  }
+  const int pw0 = base + token_of(a, rw), pw1 = rw < it.rows ? base + token_of(a, min(rw + 16 * NC, it.rows) - 1) : -1;
 
   // The table is read through scalar loads: a step's slots are the same for all lanes
   typedef const __attribute__((address_space(4))) int32_t cint_t;
@@ -554,6 +547,20 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
 #pragma unroll
     for (int u = 0; u < UPP; ++u) slot[u] = ptab[min(pg + u, a.max_pages - 1)];
   };
+  if (lo < hi) look_up(lo);
+  int pos[NC];
+  h8_t qb[NC][KT];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int row = min(rw + c * 16 + col, it.rows - 1);
+    const int t = token_of(a, row);
+    pos[c] = base + t;
+    const uint16_t* qp =
+        a.q + (int64_t)(it.start + t) * a.q_st + (int64_t)(hk * a.G + row - t * a.G) * a.q_sh + grp * 8;
+#pragma unroll
+    for (int kk = 0; kk < KT; ++kk) qb[c][kk] = ld_h8(qp + kk * 32);
+  }
+
   // bytes of this thread's chunks from their page's start
   uint32_t k_off[kI], v_off[kI];
 #pragma unroll
@@ -616,7 +623,6 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
 
   uint32_t bad_next = 0, stage = 0;
   if (lo < hi) {
-    look_up(lo);
     bad_next = issue(lds0);
     look_up(lo + 1);
   }
@@ -756,7 +762,7 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
       if (grp == 0) *reinterpret_cast<float2*>(f.part_ml + at * 2) = make_float2(thr[c] == kLazy ? m_run[c] : -INFINITY, l);
     } else {
       const float inv = l == 0.f ? 0.f : 1.f / l;       // (a row that sees nothing: zeros; NaN stays)
-      const int tt = row / a.G;
+      const int tt = pos[c] - base;
       uint16_t* dst = a.out + (int64_t)(it.start + tt) * a.o_st + (int64_t)(hk * a.G + row - tt * a.G) * a.o_sh + grp * 4;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -868,7 +874,7 @@ __global__ __launch_bounds__(kThreads) void chunk_merge_kernel(ChunkArgs a, int 
     const int r = at[u] / (D / 4), d = at[u] % (D / 4) * 4;
     if (r >= rows) break;
     const float inv = s_inv[r];
-    const int row = r0 + y0 + r, t = row / a.G;
+    const int row = r0 + y0 + r, t = token_of(a, row);
     *reinterpret_cast<uint2*>(a.out + (int64_t)(it.start + t) * a.o_st + (int64_t)(hk * a.G + row - t * a.G) * a.o_sh + d) =
         make_uint2(pack_h2(n[u][0] * inv, n[u][1] * inv), pack_h2(n[u][2] * inv, n[u][3] * inv));
   }
@@ -974,7 +980,8 @@ extern "C" int helm_chunk_attn(const void* q, int64_t q_stride_t, int64_t q_stri
   HELM_CHECK_ARG(scale > 0.f && scale < INFINITY, f + ": scale must be positive and finite");
   HELM_CHECK_SUPPORTED(D == 64 || D == 128, f + ": head_dim must be 64 or 128");
   HELM_CHECK_SUPPORTED(P == 16 || P == 32 || P == 64, f + ": page size must be 16, 32 or 64");
-  HELM_CHECK_SUPPORTED((int64_t)N * (Hq / Hkv) < (1 << 30) && Hq <= 65535, f + ": too many rows or heads");
+  HELM_CHECK_SUPPORTED((int64_t)N * (Hq / Hkv) < (1 << 30) && (int64_t)N * (Hq / Hkv) * (Hq / Hkv) < (1ll << 32) && Hq <= 65535,
+                       f + ": too many rows or heads");
   HELM_CHECK_SUPPORTED((int64_t)max_pages * P <= (int64_t)1 << 30 && window <= 1 << 30 && sinks <= 1 << 30,
                        f + ": more than 2^30 keys");
   HELM_CHECK_ARG(B == 1 || pt_stride >= max_pages, f + ": page-table stride < max_pages");
@@ -1005,7 +1012,8 @@ extern "C" int helm_chunk_attn(const void* q, int64_t q_stride_t, int64_t q_stri
   a.v_ss = pool->v_slot_stride; a.v_hs = pool->v_head_stride; a.v_ds = pool->v_dim_stride;
   a.num_slots = (int32_t)std::min<int64_t>(pool->num_slots, 0x7fffffff);   // (slots are int32)
   a.page_table = page_table; a.pt_stride = pt_stride; a.seq_lens = seq_lens; a.q_starts = q_starts;
-  a.N = N; a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.P = P; a.max_pages = max_pages;
+  a.N = N; a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.P = P;
+  a.mul_g = a.G > 1 ? (uint32_t)((1ull << 32) / (uint32_t)a.G + 1) : 0; a.max_pages = max_pages;
   a.max_new = std::min(max_new, N);
   a.window = window; a.sinks = window ? sinks : 0;
   a.covered = max_pages * P;
