@@ -895,7 +895,7 @@ Form form_of(int lo, int hi, int tile, int step, int min_steps, int want, int64_
   f.most_keys = (int)keys;
   const int64_t steps = (keys + (1 << step) - 1) >> step;
   f.items = (int)std::min<int64_t>(tiles + (steps > min_steps ? want + 1 : 0), 1 << 28);
-  f.parts = steps > min_steps ? (int)std::min<int64_t>(want + 2, tiles * kMaxPieces) : 0;
+  f.parts = steps > min_steps ? want + 2 : 0;            // (also where q_starts is no ascending list)
   f.cut_tiles = (int)std::min<int64_t>(f.parts / 2, tiles);
   return f;
 }
@@ -977,7 +977,7 @@ extern "C" int helm_chunk_attn(const void* q, int64_t q_stride_t, int64_t q_stri
   HELM_CHECK_ARG(window >= 0 && sinks >= 0, f + ": window and sinks must not be negative");
   HELM_CHECK_ARG(q_starts || N == B, f + ": without q_starts there is one row per sequence");
   HELM_CHECK_ARG(Hq % Hkv == 0, f + ": Hq must be a multiple of Hkv");
-  HELM_CHECK_ARG(scale > 0.f && scale < INFINITY, f + ": scale must be positive and finite");
+  HELM_CHECK_ARG(scale > 0.f && scale * kLog2e < INFINITY, f + ": scale must be positive and finite");
   HELM_CHECK_SUPPORTED(D == 64 || D == 128, f + ": head_dim must be 64 or 128");
   HELM_CHECK_SUPPORTED(P == 16 || P == 32 || P == 64, f + ": page size must be 16, 32 or 64");
   HELM_CHECK_SUPPORTED((int64_t)N * (Hq / Hkv) < (1 << 30) && (int64_t)N * (Hq / Hkv) * (Hq / Hkv) < (1ll << 32) && Hq <= 65535,

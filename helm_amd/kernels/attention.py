@@ -751,6 +751,7 @@ def fork_pages(pool, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: 
         if t.dtype != torch.int32 or t.dim() != 1 or t.shape != parents.shape or not t.is_contiguous():
             raise RuntimeError(f"{what}: parents and fresh must be contiguous int32 vectors of one length")
     n = parents.shape[0]
+    given = table_out is not None or lens_out is not None
     if table_out is None:
         table_out = page_table.new_empty((n, cols))
     if lens_out is None:
@@ -758,10 +759,18 @@ def fork_pages(pool, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: 
     if table_out.shape != (n, cols):
         raise RuntimeError(f"{what}: table_out must be int32 [{n}, {cols}], row-major")
     _, ots = _check_table(what, table_out, lens_out, n)
-    for a, b in ((table_out, page_table), (lens_out, seq_lens), (table_out, seq_lens), (lens_out, page_table),
-                 (table_out, parents), (table_out, fresh), (lens_out, parents), (lens_out, fresh)):
-        if _overlap(a, b):
-            raise RuntimeError(f"{what}: the outputs must not overlap the inputs")
+    if given:
+        # [first, past the last) byte of each
+        t0, l0 = table_out.data_ptr(), lens_out.data_ptr()
+        t1, l1 = t0 + 4 * (max(n - 1, 0) * ots + cols), l0 + 4 * n
+        i0 = page_table.data_ptr()
+        p0, f0, s0 = parents.data_ptr(), fresh.data_ptr(), seq_lens.data_ptr()
+        for x0, x1 in ((i0, i0 + 4 * (max(page_table.shape[0] - 1, 0) * pts + cols)), (p0, p0 + 4 * n),
+                       (f0, f0 + 4 * n), (s0, s0 + 4 * page_table.shape[0])):
+            if t0 < x1 and x0 < t1 or l0 < x1 and x0 < l1:
+                raise RuntimeError(f"{what}: the outputs must not overlap the inputs")
+        if t0 < l1 and l0 < t1:
+            raise RuntimeError(f"{what}: table_out and lens_out overlap")
     if n == 0:
         return table_out, lens_out
     if cols == 0:
@@ -771,15 +780,6 @@ def fork_pages(pool, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: 
                     fresh.data_ptr(), table_out.data_ptr(), ots, lens_out.data_ptr(), n, cols, pool.num_kv_heads,
                     pool.k.shape[-1], P, _native.raw_stream(index))
     return table_out, lens_out
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """True when the bytes from a's first to its last element meet those of b."""
-    def span(t):
-        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1 if t.numel() else 0
-        return t.data_ptr(), t.data_ptr() + n * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
 
 
 def stage_pages_h2d(host_pool: torch.Tensor, dev_staging: torch.Tensor, host_slots,

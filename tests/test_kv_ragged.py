@@ -477,3 +477,39 @@ def test_moves_replayed_from_a_graph():
         assert to[0, n // 16] == 40 and lo.tolist() == [n, 33]
         if n == 20:
             assert all(torch.equal(raw(t), w) for t, w in zip(ts, want))
+
+
+@pytest.mark.gpu
+def test_pools_past_32_bits():
+    """Pages whose first element lies behind 2^32 of the pool: written, read, copied, forked."""
+    hkv, p, d = 8, 64, 128
+    slots = (1 << 32) // (hkv * p * d) + 40              # 65576 pages of 128 KiB each for K and V
+    k = torch.empty(slots, hkv, p, d, dtype=torch.float16, device="cuda")
+    v = torch.empty(slots, hkv, d, p, dtype=torch.float16, device="cuda")
+    pool = ka.PoolView.of_pool(k, v.transpose(2, 3))
+    hi = slots - 40
+    r = Rope((8, hkv, d), p, [(0, 150), (0, 40)], d, False, seed=5)
+    low = torch.where(r.table >= 0, r.table, -1)
+    small = r.run()
+    r.check(small)
+    table = torch.where(low >= 0, low + hi, -1).cuda()
+    for i in range(len(r.k0)):                           # the same bits before, behind the border
+        k[hi + i].copy_(r.k0[i]), v[hi + i].copy_(r.v0[i])
+    q = torch.empty(190, 8, d, dtype=torch.float16, device="cuda")
+    lens, starts = r.lens.cuda(), r.starts.cuda()
+    fused.rope_append(r.qkv.cuda(), pool, table, lens, starts, p, r.inv.cuda(), 8, hkv, d, q_out=q)
+    n = len(r.k0)
+    assert torch.equal(q.cpu(), small[0]) and torch.equal(k[hi:hi + n].cpu(), small[1]) and torch.equal(v[hi:hi + n].cpu(), small[2])
+    near = ka.PoolView.of_pool(small[1].cuda(), small[2].cuda().transpose(2, 3))
+    for kw in ({}, {"window": 30, "sinks": 2}):
+        far = ka.chunk_attention(q, pool, table, lens, starts, p, **kw)
+        assert torch.equal(far, ka.chunk_attention(q, near, low.int().cuda(), lens, starts, p, **kw))
+    last = q[torch.tensor([149, 189])].contiguous()
+    assert torch.equal(ka.window_decode_attention(last, pool, table, lens, p, 70),
+                       ka.window_decode_attention(last, near, low.int().cuda(), lens, p, 70))
+    one = torch.tensor([hi + 20], dtype=torch.int32, device="cuda")
+    ka.copy_pages(pool, table[0, :1].contiguous(), one, p)
+    assert torch.equal(k[hi + 20], k[table[0, 0]]) and torch.equal(v[hi + 20], v[table[0, 0]])
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    rows, _ = ka.fork_pages(pool, table, lens, zero, one + 1, p)
+    assert rows[0, 2] == hi + 21 and torch.equal(k[hi + 21], k[table[0, 2]]) and torch.equal(v[hi + 21], v[table[0, 2]])
