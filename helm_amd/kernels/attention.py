@@ -153,8 +153,13 @@ class PoolView:
                             self.v_dim_stride, self.num_slots)
 
     def c_ref(self):
-        """A pointer to a helm_kv_pool for one call (kept alive by the caller's frame)."""
-        return ctypes.byref(self.c_struct())
+        """A pointer to a helm_kv_pool (made again only when the view's fields have changed)."""
+        key = (self.k.data_ptr(), self.v.data_ptr(), self.k_slot_stride, self.k_head_stride, self.v_slot_stride,
+               self.v_head_stride, self.v_dim_stride, self.num_slots)
+        held = self.__dict__.get("_held")
+        if held is None or held[0] != key:
+            held = self.__dict__["_held"] = (key, ctypes.byref(KvPoolStruct(*key)))
+        return held[1]
 
     @staticmethod
     def _check(k: torch.Tensor, v: torch.Tensor) -> None:
@@ -576,47 +581,60 @@ def chunk_workspace_bytes(N: int, B: int, Hq: int, Hkv: int, D: int, P: int, max
     return int(_native.lib().helm_chunk_attn_workspace_bytes(N, B, Hq, Hkv, D, P, max_pages, max_new, window, sinks))
 
 
-def _check_table(what: str, page_table: torch.Tensor, seq_lens: torch.Tensor, B: Optional[int] = None) -> Tuple[int, int]:
-    """(columns, row stride) of an int32 page table [B, max_pages] with its lengths [B]."""
-    if (page_table.dtype != torch.int32 or page_table.dim() != 2 or (B is not None and page_table.shape[0] != B)
-            or (page_table.stride(1) != 1 and page_table.shape[1] > 1)):
+def _check_table(what: str, page_table: torch.Tensor, seq_lens: torch.Tensor) -> Tuple[int, int, int]:
+    """(sequences, columns, row stride) of an int32 page table [B, max_pages] with its lengths [B]."""
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2:
         raise RuntimeError(f"{what}: page_table must be int32 [B, max_pages], row-major")
-    if seq_lens.dtype != torch.int32 or seq_lens.shape != page_table.shape[:1] or not seq_lens.is_contiguous():
-        raise RuntimeError(f"{what}: seq_lens must be int32 [B], contiguous")
     rows, cols = page_table.shape
-    if rows > 1 and page_table.stride(0) < cols:
+    stride, unit = page_table.stride()
+    if unit != 1 and cols > 1:
+        raise RuntimeError(f"{what}: page_table must be int32 [B, max_pages], row-major")
+    if seq_lens.dtype is not torch.int32 or seq_lens.shape != (rows,) or not seq_lens.is_contiguous():
+        raise RuntimeError(f"{what}: seq_lens must be int32 [B], contiguous")
+    if rows <= 1:
+        return rows, cols, cols
+    if stride < cols:
         raise RuntimeError(f"{what}: the rows of page_table overlap")
-    return cols, page_table.stride(0) if rows > 1 else cols
+    return rows, cols, stride
+
+
+def _check_starts(what: str, q_starts: Optional[torch.Tensor], N: int, B: int) -> None:
+    if q_starts is None:
+        if N != B:
+            raise RuntimeError(f"{what}: {N} rows for {B} sequences (without q_starts each has one)")
+    elif q_starts.dtype is not torch.int32 or q_starts.shape != (B + 1,) or not q_starts.is_contiguous():
+        raise RuntimeError(f"{what}: q_starts must be int32 [B + 1] = [{B + 1}], contiguous")
 
 
 def _check_fp16_pool(what: str, pool: PoolView, page_size: int) -> Tuple[int, int]:
     """(kv heads, head_dim) of an fp16 pool whose pages hold page_size tokens."""
-    if not isinstance(pool, PoolView) or pool.k.dtype != torch.float16 or pool.v.dtype != torch.float16:
+    if not isinstance(pool, PoolView) or pool.k.dtype is not torch.float16 or pool.v.dtype is not torch.float16:
         raise RuntimeError(f"{what}: the pool must be a PoolView of fp16 pages")
     if page_size not in (16, 32, 64):
         raise RuntimeError(f"{what}: the page size must be 16, 32 or 64")
-    if pool.k_head_stride < page_size * pool.k.shape[-1] or pool.v_dim_stride < page_size:
+    D = pool.k.size(-1)
+    if pool.k_head_stride < page_size * D or pool.v_dim_stride < page_size:
         raise RuntimeError(f"{what}: the pool's pages do not hold {page_size} tokens")
-    return pool.num_kv_heads, pool.k.shape[-1]
+    return pool.num_kv_heads, D
 
 
 def _chunk(what: str, q: torch.Tensor, pool: PoolView, page_table: torch.Tensor, seq_lens: torch.Tensor,
            q_starts: Optional[torch.Tensor], page_size: int, window: int, sinks: int, scale: Optional[float],
            max_new: Optional[int], workspace: Optional[AttnWorkspace], out: Optional[torch.Tensor]) -> torch.Tensor:
     index = _native.gpu_of(what, q, pool.k, pool.v, page_table, seq_lens, q_starts, out)
-    if q.dtype != torch.float16 or q.dim() != 3 or (q.stride(2) != 1 and q.shape[2] > 1):
+    if q.dtype is not torch.float16 or q.dim() != 3:
         raise RuntimeError(f"{what}: q must be fp16 [N, Hq, D] with unit stride on D")
-    N, Hq, D = q.shape
+    N, Hq, D = shape = q.shape
+    st, sh, sd = q.stride()
+    if sd != 1:
+        raise RuntimeError(f"{what}: q must be fp16 [N, Hq, D] with unit stride on D")
     Hkv, Dp = _check_fp16_pool(what, pool, page_size)
     if D != Dp or D not in (64, 128):
         raise RuntimeError(f"{what}: q has head_dim {D}, the pool {Dp} (64 or 128 are supported)")
     if Hq % Hkv:
         raise RuntimeError(f"{what}: {Hq} query heads are no multiple of the pool's {Hkv}")
-    max_pages, pts = _check_table(what, page_table, seq_lens, N if q_starts is None else None)
-    B = page_table.shape[0]
-    if q_starts is not None and (q_starts.dtype != torch.int32 or q_starts.shape != (B + 1,)
-                                 or not q_starts.is_contiguous()):
-        raise RuntimeError(f"{what}: q_starts must be int32 [B + 1] = [{B + 1}], contiguous")
+    B, max_pages, pts = _check_table(what, page_table, seq_lens)
+    _check_starts(what, q_starts, N, B)
     if window < 0 or sinks < 0:
         raise RuntimeError(f"{what}: window and sinks must not be negative")
     if max_new is None:
@@ -629,17 +647,22 @@ def _chunk(what: str, q: torch.Tensor, pool: PoolView, page_table: torch.Tensor,
         raise RuntimeError(f"{what}: scale must be positive and finite")
     if out is None:
         out = q.new_empty((N, Hq, D))
-    elif (out.dtype != torch.float16 or out.shape != (N, Hq, D) or out.stride(2) != 1 or out.stride(0) % 4
-          or out.stride(1) % 4 or out.data_ptr() % 8):
-        raise RuntimeError(f"{what}: out must be fp16 [N, Hq, D], unit stride on D, rows 8-byte aligned")
+        ot, oh = Hq * D, D
+    else:
+        if out.dtype is not torch.float16 or out.shape != shape:
+            raise RuntimeError(f"{what}: out must be fp16 [N, Hq, D], unit stride on D, rows 8-byte aligned")
+        ot, oh, od = out.stride()
+        if od != 1 or ot % 4 or oh % 4 or out.data_ptr() % 8:
+            raise RuntimeError(f"{what}: out must be fp16 [N, Hq, D], unit stride on D, rows 8-byte aligned")
     if N == 0 or B == 0:
         return out
     if max_pages == 0:
         raise RuntimeError(f"{what}: the page table has no columns")
-    st, sh, _ = q.stride()
-    if st % 8 or sh % 8 or q.data_ptr() % 16:
+    qp = q.data_ptr()
+    if st % 8 or sh % 8 or qp % 16:
         q = q.clone(memory_format=torch.contiguous_format)
         st, sh, _ = q.stride()
+        qp = q.data_ptr()
     max_new = min(int(max_new), N)
     # (what no key reaches is no window)
     window = 0 if window >= max_pages * page_size else int(window)
@@ -650,9 +673,9 @@ def _chunk(what: str, q: torch.Tensor, pool: PoolView, page_table: torch.Tensor,
         if workspace is None:
             workspace = AttnWorkspace(q.device)
         ws = workspace.reserve(index, need)
-    _native.call_on(index, "helm_chunk_attn", q.data_ptr(), st, sh, pool.c_ref(), page_table.data_ptr(), pts,
-                    seq_lens.data_ptr(), _native.ptr(q_starts), N, B, Hq, Hkv, D, page_size, max_pages, max_new,
-                    window, sinks, scale, out.data_ptr(), out.stride(0), out.stride(1), ws, need,
+    _native.call_on(index, "helm_chunk_attn", qp, st, sh, pool.c_ref(), page_table.data_ptr(), pts,
+                    seq_lens.data_ptr(), None if q_starts is None else q_starts.data_ptr(), N, B, Hq, Hkv, D, page_size,
+                    max_pages, max_new, window, sinks, scale, out.data_ptr(), ot, oh, ws, need,
                     _native.raw_stream(index))
     return out
 
@@ -746,7 +769,7 @@ def fork_pages(pool, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: 
     what = "fork_pages"
     P = _page_layout(what, pool, page_size)
     index = _native.gpu_of(what, pool.k, pool.v, page_table, seq_lens, parents, fresh, table_out, lens_out)
-    cols, pts = _check_table(what, page_table, seq_lens)
+    B, cols, pts = _check_table(what, page_table, seq_lens)
     for t in (parents, fresh):
         if t.dtype != torch.int32 or t.dim() != 1 or t.shape != parents.shape or not t.is_contiguous():
             raise RuntimeError(f"{what}: parents and fresh must be contiguous int32 vectors of one length")
@@ -758,15 +781,15 @@ def fork_pages(pool, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: 
         lens_out = seq_lens.new_empty((n,))
     if table_out.shape != (n, cols):
         raise RuntimeError(f"{what}: table_out must be int32 [{n}, {cols}], row-major")
-    _, ots = _check_table(what, table_out, lens_out, n)
+    _, _, ots = _check_table(what, table_out, lens_out)
     if given:
         # [first, past the last) byte of each
         t0, l0 = table_out.data_ptr(), lens_out.data_ptr()
         t1, l1 = t0 + 4 * (max(n - 1, 0) * ots + cols), l0 + 4 * n
         i0 = page_table.data_ptr()
         p0, f0, s0 = parents.data_ptr(), fresh.data_ptr(), seq_lens.data_ptr()
-        for x0, x1 in ((i0, i0 + 4 * (max(page_table.shape[0] - 1, 0) * pts + cols)), (p0, p0 + 4 * n),
-                       (f0, f0 + 4 * n), (s0, s0 + 4 * page_table.shape[0])):
+        for x0, x1 in ((i0, i0 + 4 * (max(B - 1, 0) * pts + cols)), (p0, p0 + 4 * n),
+                       (f0, f0 + 4 * n), (s0, s0 + 4 * B)):
             if t0 < x1 and x0 < t1 or l0 < x1 and x0 < l1:
                 raise RuntimeError(f"{what}: the outputs must not overlap the inputs")
         if t0 < l1 and l0 < t1:
@@ -776,7 +799,7 @@ def fork_pages(pool, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: 
     if cols == 0:
         raise RuntimeError(f"{what}: the page table has no columns")
     _native.call_on(index, "helm_fork_pages_q8" if isinstance(pool, Q8PoolView) else "helm_fork_pages", pool.c_ref(),
-                    page_table.data_ptr(), pts, seq_lens.data_ptr(), page_table.shape[0], parents.data_ptr(),
+                    page_table.data_ptr(), pts, seq_lens.data_ptr(), B, parents.data_ptr(),
                     fresh.data_ptr(), table_out.data_ptr(), ots, lens_out.data_ptr(), n, cols, pool.num_kv_heads,
                     pool.k.shape[-1], P, _native.raw_stream(index))
     return table_out, lens_out

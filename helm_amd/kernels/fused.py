@@ -15,7 +15,7 @@ import torch
 
 from .. import _native
 from . import gemv_split_bytes
-from .attention import _check_fp16_pool, _check_places, _check_table
+from .attention import _check_fp16_pool, _check_places, _check_starts, _check_table
 
 
 def _check_fp16(*ts):
@@ -265,11 +265,8 @@ def rope_append(qkv: torch.Tensor, pool, page_table: torch.Tensor, seq_lens: tor
     if _check_fp16_pool(what, pool, page_size) != (Hkv, D):
         raise RuntimeError(f"{what}: {Hkv} heads of {D} do not fit the pool's {pool.num_kv_heads} of {pool.k.shape[-1]}")
     N, width = qkv.shape
-    cols, pts = _check_table(what, page_table, seq_lens, N if q_starts is None else None)
-    B = page_table.shape[0]
-    if q_starts is not None and (q_starts.dtype != torch.int32 or q_starts.shape != (B + 1,)
-                                 or not q_starts.is_contiguous()):
-        raise RuntimeError(f"{what}: q_starts must be int32 [B + 1] = [{B + 1}], contiguous")
+    B, cols, pts = _check_table(what, page_table, seq_lens)
+    _check_starts(what, q_starts, N, B)
     if (inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous()
             or 2 * inv_freq.shape[0] > D):
         raise RuntimeError(f"{what}: inv_freq must be fp32 [r / 2], contiguous, with r <= {D} rotated dims")
