@@ -44,6 +44,7 @@ struct Form {
   int lo, hi;          // it takes sequences of lo < rows <= hi
   int tile, step;      // log2 of the rows of a tile, of the keys of a step
   int min_steps;       // least steps of a piece
+  float per_piece;     // most pieces of a step
   int want;            // pieces of a kv head that fill the chip
   float per_want;      // 1 / want and a little, so that work * per_want is not below work / want
   int most_keys;       // that a tile can see
@@ -135,9 +136,10 @@ __device__ __forceinline__ float dpp_max(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
-// Pieces of a tile of so many steps, at most m each.
-__device__ __forceinline__ int pieces_of(int steps, float inv_m) {
-  return min(max((int)ceilf((float)steps * inv_m), 1), kMaxPieces);
+// Pieces of a tile of so many steps: of m each at most, and of 1 / per_piece at least.
+__device__ __forceinline__ int pieces_of(const Form& f, int steps, float inv_m) {
+  const int most = min(max((int)((float)steps * f.per_piece), 1), kMaxPieces);
+  return min(max((int)ceilf((float)steps * inv_m), 1), most);
 }
 
 // Most steps of a piece, 1 / m returned: with W the sum of tiles x steps of a kv head, the least m
@@ -159,10 +161,10 @@ __device__ __forceinline__ float inv_steps(const ChunkArgs& a, const Form& f, co
 #pragma unroll 1
     for (float by = 1.f; by < 2.f; by += 0.25f) {
       const float inv = 1.f / fmaxf(mean * by, (float)f.min_steps);
-      float n = (float)(first.tiles * pieces_of(first.steps, inv));
+      float n = (float)(first.tiles * pieces_of(f, first.steps, inv));
       for (int i = 64; i < a.B; i += 64) {
         const Seq s = seq_of(a, f, i + lane);
-        n += (float)(s.tiles * pieces_of(s.steps, inv));
+        n += (float)(s.tiles * pieces_of(f, s.steps, inv));
       }
       if (dpp_sum(n) <= (float)f.want) {
         m = mean * by;
@@ -184,7 +186,7 @@ __device__ __forceinline__ bool find_item(const ChunkArgs& a, int want, Item& it
   uint32_t items = 0, parts = 0;        // of the sequences before
   for (int i0 = 0; i0 < a.B; i0 += 64) {
     const Seq s = i0 == 0 ? first : seq_of(a, f, i0 + lane);
-    const int pieces = pieces_of(s.steps, inv);
+    const int pieces = pieces_of(f, s.steps, inv);
     const uint32_t own_parts = pieces > 1 ? (uint32_t)(s.tiles * pieces) : 0u;
     const uint32_t mine = MERGE ? (pieces > 1 ? (uint32_t)s.tiles : 0u) : (uint32_t)(s.tiles * pieces);
     const uint32_t upto = items + wave_scan(mine), parts_upto = parts + wave_scan(own_parts);
@@ -888,14 +890,17 @@ struct Plan {
   int few_nc;                           // 16-row tiles of the few-row kernel
 };
 
-Form form_of(int lo, int hi, int tile, int step, int min_steps, int want, int64_t tiles, int64_t keys) {
+Form form_of(int lo, int hi, int tile, int step, int min_steps, float per_piece, int want, int64_t tiles,
+             int64_t keys) {
   Form f{};
   f.lo = lo; f.hi = hi; f.tile = tile; f.step = step; f.min_steps = min_steps; f.want = want;
   f.per_want = 1.00002f / (float)want;
+  f.per_piece = per_piece;
   f.most_keys = (int)keys;
   const int64_t steps = (keys + (1 << step) - 1) >> step;
-  f.items = (int)std::min<int64_t>(tiles + (steps > min_steps ? want + 1 : 0), 1 << 28);
-  f.parts = steps > min_steps ? want + 2 : 0;            // (also where q_starts is no ascending list)
+  const bool cut = steps > min_steps && (float)steps * per_piece >= 2.f;
+  f.items = (int)std::min<int64_t>(tiles + (cut ? want + 1 : 0), 1 << 28);
+  f.parts = cut ? want + 2 : 0;         // (also where q_starts is no ascending list)
   f.cut_tiles = (int)std::min<int64_t>(f.parts / 2, tiles);
   return f;
 }
@@ -914,9 +919,11 @@ Plan plan_of(int N, int B, int Hq, int Hkv, int P, int max_pages, int max_new, i
     return window ? std::min<int64_t>(all, (int64_t)window + sinks + rows / G + 2 * step) : all;
   };
   const int want = std::max(1, 512 / Hkv);
-  if (few) p.f[kFew] = form_of(0, few, few == 16 ? 4 : 5, 5, 4, want, seqs, keys(few, 32));
+  if (few) p.f[kFew] = form_of(0, few, few == 16 ? 4 : 5, 5, 4, 1.f, want, seqs, keys(few, 32));
   if (most > few)
-    p.f[kMany] = form_of(few, 1 << 30, 7, 6, 4, want, (int64_t)N * G / kTile + seqs, keys(kTile, kKeys));
+    // a piece of fewer than 8 steps costs more in partials than it saves (700 rows after 100 of 40 heads in
+    // two pieces of 7 steps 32.4 us, whole 26.2)
+    p.f[kMany] = form_of(few, 1 << 30, 7, 6, 8, 0.125f, want, (int64_t)N * G / kTile + seqs, keys(kTile, kKeys));
   return p;
 }
 int64_t part_floats(const Form& f, int Hkv, int D) { return ((int64_t)Hkv * f.parts << f.tile) * (D + 2); }
