@@ -748,6 +748,23 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
         for (int c = 0; c < NC; ++c) o[c][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[c], o[c][d], 0, 0, 0);
       }
     }
+    // The order of this block: the first half's probabilities, its products with the second half's
+    // probabilities between them (two vector instructions and an operand read a product), the second
+    // half's products.  chunk of 4096 after 12288, 40 heads 1099 -> 1066 us, the compiler's own order
+    // before; raised wave priority around the products 1132-1170.
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);      // operand reads
+    __builtin_amdgcn_sched_group_barrier(0x002, 28, 0);     // vector instructions
+#pragma unroll
+    for (int i = 0; i < NC * (1 + DT); ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);    // a product
+      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NC * (1 + DT); ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
   }
 
   // o[c][d][r] = O^T[dim d*16 + grp*4 + r][row col of tile c]
