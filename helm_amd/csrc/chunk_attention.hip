@@ -6,19 +6,28 @@
 // or j > p - window, or j < sinks).  out = softmax(scale q . K^T) V over those keys.
 //
 // All lengths are on the device, so what a workgroup does is found on the device too (the
-// plan): each sequence's rows (token, head of the kv head's group; token-major) are cut into
-// row tiles, each tile's keys into the sequence's number of pieces, and workgroup x of a
-// kv head takes the x-th (sequence, tile, piece).  Pieces are sized so that a launch has a
-// few more workgroups than the chip has places, whatever the lengths are; sequences of one
-// piece write their output, the others fp32 partials that a second kernel merges.  The
-// grid and the workspace depend on bounds that the host knows (plan_of).
+// plan, 1.4 us of a workgroup's start): each sequence's rows (token, head of the kv head's
+// group; token-major) are cut into row tiles, each tile's keys into the sequence's number of
+// pieces, and workgroup x of a kv head takes the x-th (sequence, tile, piece).  Pieces are
+// sized so that all of them find places on the chip at once, whatever the lengths are;
+// sequences of one piece write their output, the others fp32 partials that a second kernel
+// merges.  The grid and the workspace depend on bounds that the host knows (plan_of).  The kv
+// head is the fastest-varying workgroup index: with 8 of them each XCD serves one, and its
+// K/V stays in that XCD's L2.
 //
-// Two kernels share the sequences by their number of rows:
-//   few_attn_kernel   up to 16 or 32 rows (decode, drafts): bound by streaming K and V
-//                     once; the four waves of a workgroup take key steps in turn
-//   tile_attn_kernel  more (prompts): bound by the matrix cores; the waves take rows and
-//                     share K and V through LDS
-// Both run S^T = K . Q^T and O^T += V^T . P^T on v_mfma_f32_16x16x32_f16 with the keys of the
+// Two forms share the sequences by their number of rows:
+//   few_body   up to 16 or 32 rows (decode, drafts): bound by streaming K and V once; the four
+//              waves of a workgroup take key steps in turn.  16 items of up to 12000 tokens
+//              under a window of 2048, 40 heads over 8 (117 MB): 24 us and 4.5 for the merge;
+//              one item of 16384 under 4096 (17 MB): 7.8 and 3.9, a chain of round trips (kernel
+//              arguments, lengths, table, K / V) on either side of one step
+//   tile_body  more (prompts): bound by the matrix cores; the waves take rows and share K and V
+//              through LDS.  4096 tokens after 12288, 40 heads over 8: 1066 us, 1.13 PFLOP/s, 0.98 of
+//              what an 8192^3 fp16 product reaches on this card (1.16).  A workgroup's start and end
+//              cost 8 us beside 1.9 a step of 64 keys (two workgroups a CU): prompts under a window of
+//              1024, 18 steps a tile, run at 0.79 PFLOP/s
+// A batch with sequences of both kinds runs them in one launch (both_attn_kernel).
+// Both forms run S^T = K . Q^T and O^T += V^T . P^T on v_mfma_f32_16x16x32_f16 with the keys of the
 // score tiles permuted so that each lane holds the probabilities of the 8 consecutive keys
 // whose V^T it feeds to the second product, and an online softmax in the log2 domain whose
 // maximum is raised only when it is passed by kLazy.
@@ -262,8 +271,9 @@ __device__ __forceinline__ u32x4_t seen_bits(const ChunkArgs& a, const Steps& s,
 // ── few rows ─────────────────────────────────────────────────────────────────
 
 // NC tiles of 16 rows.  Steps of 32 keys, one wave each, round robin; K's and V's registers
-// are filled again as soon as they have been read.  P is split into fp16 hi + lo parts, so
-// that the product keeps fp32's accuracy (the matrix cores wait for memory anyway).
+// are filled again as soon as they have been read (157 registers at NC = 1, 215 at 2: three and two
+// workgroups a CU).  P is split into fp16 hi + lo parts, so that the product keeps fp32's
+// accuracy (the matrix cores wait for memory anyway).
 template <int D, int NC>
 struct FewLds {
   float o[kWaves][16 * NC][D];
@@ -507,6 +517,14 @@ __device__ __forceinline__ int kswz(int r) {
   return ((r & 3) | (((r >> 3) & 3) << 2)) & (CPR - 1);
 }
 
+// A wave takes kNC x 16 rows, a workgroup kTile.  Per step of 64 keys a wave runs 68 products a
+// 1088 cycles of the matrix core at D = 128, and on the vector unit per score a multiply-add, half
+// a maximum, an exponential and half a conversion; the two halves of a step share one check of
+// the maximum, so that the second half's products can run beside the first half's softmax.
+// What the step does not compute: page slots come by scalar loads a step ahead (a copy
+// instruction reads one page), operand addresses are constants and one toggled stage bit, sums
+// are products with ones.  (Steps of 32 keys with three workgroups a CU in 168 registers: long
+// prompts 1% faster, mixed batches 4%, prompts under a window 5% and short ones 15% slower.)
 template <int D>
 struct TileLds {
   u32x4_t kv[2][2 * kKeys * D / 8];
@@ -804,7 +822,8 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
   tile_body<D, P, WIN>(a, (int)(blockIdx.x % (unsigned)a.Hkv), (int)(blockIdx.x / (unsigned)a.Hkv), lds);
 }
 // Both forms in one launch, the many rows' workgroups first: those of few rows wait for memory and
-// fill the places that are left.
+// fill the places that are left.  700 rows after 8000 beside 24 single rows, 40 heads: 204 us, in two
+// launches 214, the two kinds in turn 260.
 template <int D, int P, bool WIN>
 __global__ __launch_bounds__(kThreads, 2) void both_attn_kernel(ChunkArgs a) {
   __shared__ __attribute__((aligned(16))) union { FewLds<D, 1> few; TileLds<D> tile; } lds;
@@ -813,8 +832,9 @@ __global__ __launch_bounds__(kThreads, 2) void both_attn_kernel(ChunkArgs a) {
   else few_body<D, P, 1>(a, hk, x - a.f[kMany].items, lds.few);
 }
 
-// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over a tile's pieces.  Bound by latency: the
-// plan, the maxima, the partials.  A workgroup takes R rows (grid.y of them a tile, the tiles of
+// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over a tile's pieces.  Bound by latency (the
+// plan, the maxima, the partials: 3.5-4.5 us, with nothing to merge too), beside many rows by
+// reading their partials (30 MB: 13 us).  A workgroup takes R rows (grid.y of them a tile, the tiles of
 // few rows first); its threads are 4 dims of a row each, and where those are fewer than 256, groups
 // that take the pieces in turn.
 template <int D, int R>

@@ -65,7 +65,8 @@ __device__ __forceinline__ Place place_of(const RopeArgs& a, int row, int b) {
 }
 
 // One wave per (row, head).  Bound by latency: the row's sequence (how many of q_starts[1 ..] are
-// not above it, 64 at a time), its length, its slot, and then the write.
+// not above it, 64 at a time), its length, its slot, and then the write: 16 rows of 32 + 8 + 8 heads 3.2
+// us.
 template <int D>
 __global__ __launch_bounds__(256) void rope_rows_kernel(RopeArgs a) {
   constexpr int J = D / 64;
@@ -158,18 +159,18 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// The same for many rows.  Bound by moving qkv once; the form above spends its time on a sine, a
+// The same for many rows.  Bound by moving qkv once: 3926 rows of 40 + 8 + 8 heads (112 MB) 25 us with
+// inputs in the last-level cache and 31 without, 22 at the rate of a large copy.  The form above spends its time on a sine, a
 // cosine and a 64-bit reduction per element of every head and on a store per V element in a line of
 // its own.  Here a workgroup takes 256 / (D / 8) tokens, D / 8 lanes a token, and
-//   * of q and k kPH heads one after another: a lane holds the same four pairs of each, so their
+//   * of q and k PH heads one after another: a lane holds the same four pairs of each, so their
 //     factors are made once and stay in registers and no value changes lanes.  Its 8 dims are two
 //     groups of 4: at 4 l and r/2 + 4 l of the r rotated dims (r a multiple of 8), behind them, or
 //     with interleaved pairs everywhere, 8 neighbours.
 //   * of v kVH heads of 16 tokens that lie in one page from a multiple of 16 on (whatever rows they
 //     are), turned through LDS: V pages are [D][P], and 32 bytes of a dim written by two workgroups
-//     are two partial writes of two L2s.  2000 + 129 + 1297 + 500 tokens of 40 + 8 + 8 heads (112 MB):
-//     with rows' own blocks of 16 and 2-byte stores 26.6 us
-constexpr int kPH = 16, kVH = 8;
+//     are two partial writes of two L2s (the rows' own blocks of 16, in 2-byte stores, take 1 us more)
+constexpr int kVH = 8;
 constexpr int kPad = 2;                  // halves between the tokens of a head's V in LDS
 
 // The want-th block of 16 positions that holds new tokens: its sequence's first row and position,
@@ -259,7 +260,7 @@ __device__ __forceinline__ void v_tile(const RopeArgs& a, int block, int h0, uin
 }
 
 // The first v_items workgroups are those of v.
-template <int D>
+template <int D, int PH>
 __global__ __launch_bounds__(256, 4) void rope_tile_kernel(RopeArgs a, int v_items, int qk_tiles) {
   constexpr int RL = D / 8;
   constexpr int PT = 256 / RL;           // tokens of a workgroup
@@ -275,12 +276,12 @@ __global__ __launch_bounds__(256, 4) void rope_tile_kernel(RopeArgs a, int v_ite
   const int li = tid % RL, lt = tid / RL;
   const int x = (int)blockIdx.x - v_items, group = x / qk_tiles;
   const int row0 = (x - group * qk_tiles) * PT, nt = min(PT, a.N - row0);
-  const int h0 = group * kPH, nh = min(kPH, a.Hq + a.Hkv - h0);
+  const int h0 = group * PH, nh = min(PH, a.Hq + a.Hkv - h0);
   const int half = a.rot / 2;
   int dA = li * 8, dB = dA + 4;
   if (!a.inter && li < a.rot / 8) dA = li * 4, dB = half + li * 4;
   const uint16_t* src = a.qkv + (int64_t)(row0 + min(lt, nt - 1)) * a.qkv_st + (int64_t)h0 * D;
-  constexpr int kAhead = 8;              // heads on the way
+  constexpr int kAhead = PH < 8 ? PH : 8;  // heads on the way
   uint2 rA[kAhead], rB[kAhead];
   auto load = [&](int i, int h) {
     rA[i] = *reinterpret_cast<const uint2*>(src + (int64_t)min(h, nh - 1) * D + dA);
@@ -384,8 +385,10 @@ __global__ __launch_bounds__(256, 4) void rope_tile_kernel(RopeArgs a, int v_ite
   }
 }
 
-// (row, head) rows from which the tile form is the faster one.
-constexpr int64_t kTileRows = 8192;
+// (row, head) rows from which the tile form is the faster one: 40 + 8 + 8 heads of 128 5600 rows 6.2 us
+// against 6.0, 8176 rows 6.1 against 7.0; 16 + 1 + 1 of 128 5400 rows 6.0 against 5.8; 16 + 8 + 8 of 64 6400 rows
+// 6.2 against 5.3, 9600 rows 6.2 against 6.4.
+constexpr int64_t tile_rows(int D) { return D == 128 ? 6000 : 9000; }
 
 // ── pages moved inside a pool ────────────────────────────────────────────────
 
@@ -482,7 +485,8 @@ __global__ __launch_bounds__(256) void fork_pages_kernel(PageArgs a) {
   copy_part<U>(a, s, f, part - 1);
 }
 
-// Chunks of a thread: one while all its workgroups are in flight at once (latency), four for more.
+// Chunks of a thread: one while all its workgroups are in flight at once (5 pages of 64 KiB 2.4 us), four
+// for more (2048 pages: 47 us, 5.7 TB/s; 58 with nothing in the last-level cache).
 template <typename Go>
 void by_width(int64_t chunks, Go go) {
   if (chunks <= 256 * 1024) go(std::integral_constant<int, 1>{});
@@ -601,16 +605,27 @@ extern "C" int helm_rope_append(const void* qkv, int64_t qkv_stride_t, const voi
   a.inter = interleaved != 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t rows = (int64_t)N * (Hq + 2 * Hkv);
-  const bool tiles = rows >= kTileRows && (a.inter || rotary_dim % 8 == 0);
+  const bool tiles = rows >= tile_rows(D) && (a.inter || rotary_dim % 8 == 0);
   auto go = [&](auto d_tag) {
     constexpr int Dc = decltype(d_tag)::value;
     if (tiles) {
       constexpr int pt = 256 / (Dc / 8);
-      const int qk_tiles = (N + pt - 1) / pt, groups = (Hq + Hkv + kPH - 1) / kPH;
+      const int qk_tiles = (N + pt - 1) / pt;
       // a sequence's n tokens lie in at most n / 16 + 2 blocks
       const int64_t v_items = ((int64_t)N / 16 + 2 * (int64_t)std::min(B, N)) * ((Hkv + kVH - 1) / kVH);
-      hipLaunchKernelGGL((rope_tile_kernel<Dc>), dim3((unsigned)(v_items + (int64_t)qk_tiles * groups)), dim3(256), 0, s, a,
-                         (int)v_items, qk_tiles);
+      auto run = [&](auto ph_tag) {
+        constexpr int PH = decltype(ph_tag)::value;
+        const int groups = (Hq + Hkv + PH - 1) / PH;
+        hipLaunchKernelGGL((rope_tile_kernel<Dc, PH>), dim3((unsigned)(v_items + (int64_t)qk_tiles * groups)), dim3(256), 0,
+                           s, a, (int)v_items, qk_tiles);
+      };
+      // Heads of a workgroup: 16 make the factors least often, but are a chain; fewer where the chip has
+      // places left.  us with 4 / 8 / 16, 40 + 8 + 8 heads of 128: 300 rows (57 workgroups of 16) 6.4 / 8.1 / 12.2,
+      // 1024 (192) 11.5 / 11.2 / 14.3, 2048 (384) 18.5 / 17.0 / 19.4, 3926 (738) 28.7 / 27.6 / 25.6
+      const int64_t wide = (int64_t)qk_tiles * ((Hq + Hkv + 15) / 16);
+      if (wide >= 512) run(std::integral_constant<int, 16>{});
+      else if (wide >= 192) run(std::integral_constant<int, 8>{});
+      else run(std::integral_constant<int, 4>{});
     } else {
       hipLaunchKernelGGL((rope_rows_kernel<Dc>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
     }

@@ -220,7 +220,16 @@ def test_rope_many_rows(heads, inter):
     for i, rot in enumerate([d, d // 2, 16, 0, 26]):
         r = Rope(heads, (16, 32, 64)[i % 3], LONG, rot, inter, norm=bool(i & 1), scale=1.0 if i else 1.14, first=i % 2,
                  pad=i % 3, seed=i)
-        assert r.rows * (heads[0] + 2 * heads[1]) >= 8192
+        assert r.rows * (heads[0] + 2 * heads[1]) >= 9000
+        r.check(r.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(40, 8, 128), (72, 8, 128), (61, 9, 64), (150, 10, 64)])
+def test_rope_heads_of_a_workgroup(heads):
+    """Enough rows for 8 and for 16 heads a workgroup, and heads that fill no last one."""
+    for inter in (False, True):
+        r = Rope(heads, 16, LONG, heads[2] // 2 if inter else heads[2], inter, norm=not inter, seed=int(inter))
         r.check(r.run())
 
 
