@@ -692,7 +692,7 @@ def chunk_attention(q: torch.Tensor, pool: PoolView, page_table: torch.Tensor, s
     tokens; seq_lens[b] counts them and its cached ones, page_table [B, max_pages] holds its
     slots (all int32).  The token at position p sees keys j <= p; with a `window` of w > 0 only
     j > p - w, and the first `sinks` tokens: pages that no new token sees may be freed (-1 in
-    the table).  A token that sees no key gives zeros.  Rows before q_starts[0] and from
+    the table), places that none sees may hold anything.  A token that sees no key gives zeros.  Rows before q_starts[0] and from
     q_starts[B] on are not written, so a batch may be padded.
 
     max_new bounds the new tokens of a sequence (any longer one has its first max_new rows

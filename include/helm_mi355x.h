@@ -321,7 +321,8 @@ int helm_prefill_attn_mask(const void* q, int64_t q_stride_t, int64_t q_stride_h
  *     before q_starts[0] or from q_starts[B] on are not written.
  *   - Table entries outside [0, num_slots) contribute no keys, and are not needed for pages
  *     that no row sees (those behind the window may be freed); keys past max_pages * P do
- *     not exist.  K and V of places that no row sees may hold anything.
+ *     not exist.  K and V of places that no row sees may hold anything, and K of any place
+ *     that a row does not see (a V that is not finite may reach the rows beside those that see it).
  *   - max_new: the most new tokens of a sequence that the call is prepared for (N: any);
  *     a sequence with more has only its first max_new rows written.
  *   - workspace (16-byte aligned, contents on entry do not matter) of at least

@@ -453,3 +453,50 @@ def test_python_refusals():
         ka.window_decode_attention(b.d_q, b.pool, b.d_table, b.d_lens, 16, 4)      # three rows, two sequences
     empty = ka.chunk_attention(b.d_q[:0], b.pool, b.d_table, b.d_lens, b.d_starts, 16)
     assert empty.shape == (0, 4, 64)
+
+
+def flat_pool(L, hkv, d, page, seed):
+    """Keys of zeros and values of +-1 of one sequence of L tokens in shuffled pages, its table, and the
+    sums of values up to each token [L + 1, hkv, d]."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n = -(-L // page)
+    v = torch.randint(0, 2, (n * page, hkv, d), generator=g, device="cuda", dtype=torch.int8) * 2 - 1
+    order = torch.randperm(n, generator=g, device="cuda")
+    vp = torch.empty(n, hkv, d, page, dtype=torch.float16, device="cuda")
+    vp[order] = v.view(n, page, hkv, d).permute(0, 2, 3, 1).half()
+    kp = torch.zeros(n, hkv, page, d, dtype=torch.float16, device="cuda")
+    sums = torch.cat([torch.zeros(1, hkv, d, dtype=torch.int32, device="cuda"), v.int().cumsum(0, dtype=torch.int32)])
+    return ka.PoolView.of_pool(kp, vp.transpose(2, 3)), order.int()[None].contiguous(), sums
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d,page", [(16, 1, 64, 16), (8, 2, 128, 64)])
+@pytest.mark.parametrize("window", [0, 100, 20000])
+def test_long_prompts(hq, hkv, d, page, window):
+    """Tens of thousands of rows after tens of thousands of keys, every row against exact sums."""
+    n, L = 30000, 41003
+    pool, table, sums = flat_pool(L, hkv, d, page, 1)
+    q = torch.randn(n, hq, d, dtype=torch.float16, device="cuda")
+    out = ka.chunk_attention(q, pool, table, torch.tensor([L], dtype=torch.int32, device="cuda"),
+                             torch.tensor([0, n], dtype=torch.int32, device="cuda"), page, window, 3 if window else 0)
+    p = torch.arange(L - n, L, device="cuda")
+    lo = (p - window + 1).clamp(min=0) if window else torch.zeros_like(p)
+    total, count = sums[p + 1] - sums[lo], p + 1 - lo
+    if window:
+        more = lo.clamp(max=3)                           # sinks before the window
+        total, count = total + sums[more], count + more
+    want = (total.double() / count.double()[:, None, None]).repeat_interleave(hq // hkv, 1)
+    assert ((out.double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -22).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [0, 1000, 200000])
+def test_decode_after_hundreds_of_thousands_of_tokens(window):
+    L = 300017
+    pool, table, sums = flat_pool(L, 2, 64, 16, 2)
+    q = torch.randn(1, 8, 64, dtype=torch.float16, device="cuda")
+    out = ka.window_decode_attention(q, pool, table, torch.tensor([L], dtype=torch.int32, device="cuda"), 16, window, 7)
+    lo = L - window if window else 0
+    more = 7 if window else 0
+    want = ((sums[L] - sums[lo] + sums[more]).double() / (L - lo + more)).repeat_interleave(4, 0)
+    assert ((out[0].double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -22).all()
