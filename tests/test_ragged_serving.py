@@ -2,12 +2,12 @@
 decoding sequences, forks that share pages, windows that free them, compaction, captured steps.
 
 Each sequence's projections are kept on the side; what a step attends is checked against fp64
-from them: q and k turned in fp64 and rounded to fp16 as the cache holds them (a rounding may fall
-the other way: 2^-11 of a key, which moves a score by up to 2^-11 |q| |k| scale, 0.04 for |q| = |k| =
-sqrt(128) * 1.5, so a probability by 4% where one key's rounding differs in all its dims the same
-way; of 128 dims' independent halves of a step next to a border less than one in 2^8 falls the other
-way, 2^-11 * 1.5 * 1.5 * 2^-3 of a score), plus the bounds of the kernels' own: 2^-9 of the largest |v|
-with the output's rounding.
+from them, q and k turned in fp64 and rounded to fp16 as the cache holds them.  A value within the
+kernel's 2^-19 of a border between two fp16 numbers may be rounded to the other one, a step of 2^-10 of
+it, in one of 2^8 dims: that moves a score by 2^-10 |q_d k_d| D^-0.5, at most 1.4e-3 for |q_d k_d| <= 16, and
+the output by p (1 - p) 2 max |v| times as much, 0.7e-3 max |v|.  With the probabilities' rounding (2^-11
+of sum p |v - o|, at most 2^-10 max |v|) and the output's (2^-11 |o|) that is below 2^-9 max |v| + 2^-11 |o|;
+2^-9 max |v| is asked for.
 """
 import math
 
