@@ -91,6 +91,15 @@ __device__ __forceinline__ uint4 ld_nt16(const void* p) {
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 
+// Streaming stores (non-temporal): of much data that the kernel does not read again.
+__device__ __forceinline__ void st_nt8(void* p, uint32_t x, uint32_t y) {
+  __builtin_nontemporal_store((uint64_t)y << 32 | x, reinterpret_cast<uint64_t*>(p));
+}
+__device__ __forceinline__ void st_nt16(void* p, uint4 v) {
+  const u32x4_t x = {v.x, v.y, v.z, v.w};
+  __builtin_nontemporal_store(x, reinterpret_cast<u32x4_t*>(p));
+}
+
 __device__ __forceinline__ float h2f(uint16_t b) {
   return (float)__builtin_bit_cast(_Float16, b);
 }

@@ -159,8 +159,8 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// The same for many rows.  Bound by moving qkv once: 3926 rows of 40 + 8 + 8 heads (112 MB) 25 us with
-// inputs in the last-level cache and 31 without, 22 at the rate of a large copy.  The form above spends its time on a sine, a
+// The same for many rows.  Bound by moving qkv once: 3926 rows of 40 + 8 + 8 heads (112 MB) 22 us, with
+// inputs in the last-level cache or without, and 22 at the rate of a large copy.  The form above spends its time on a sine, a
 // cosine and a 64-bit reduction per element of every head and on a store per V element in a line of
 // its own.  Here a workgroup takes 256 / (D / 8) tokens, D / 8 lanes a token, and
 //   * of q and k PH heads one after another: a lane holds the same four pairs of each, so their
@@ -170,6 +170,9 @@ __device__ __forceinline__ float row_sum(float v) {
 //   * of v kVH heads of 16 tokens that lie in one page from a multiple of 16 on (whatever rows they
 //     are), turned through LDS: V pages are [D][P], and 32 bytes of a dim written by two workgroups
 //     are two partial writes of two L2s (the rows' own blocks of 16, in 2-byte stores, take 1 us more)
+// q, K and V are stored non-temporally: the 3926 rows 25 us warm and 32 cold with plain stores.  An
+// attention over them right after takes about as much back at up to 4000 rows (append and attention of
+// 4 x 256 rows after 200 39.6 -> 38.9 us, 4 x 1000 99 -> 101), but not at 8000 (16 x 500 after 300 203 -> 194).
 constexpr int kVH = 8;
 constexpr int kPad = 2;                  // halves between the tokens of a head's V in LDS
 
@@ -249,8 +252,8 @@ __device__ __forceinline__ void v_tile(const RopeArgs& a, int block, int h0, uin
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = src[e * (D + kPad)];
     if (whole) {
-      *reinterpret_cast<uint4*>(dst) = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16,
-                                                  y[4] | (uint32_t)y[5] << 16, y[6] | (uint32_t)y[7] << 16);
+      st_nt16(dst, make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16,
+                              y[4] | (uint32_t)y[5] << 16, y[6] | (uint32_t)y[7] << 16));
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -375,11 +378,11 @@ __global__ __launch_bounds__(256, 4) void rope_tile_kernel(RopeArgs a, int v_ite
       if (lt >= nt || h8 + i >= nh) continue;
       if (is_q) {
         if (p.seq < 0) continue;
-        *reinterpret_cast<uint2*>(qdst + h * D + dA) = oA;
-        *reinterpret_cast<uint2*>(qdst + h * D + dB) = oB;
+        st_nt8(qdst + h * D + dA, oA.x, oA.y);
+        st_nt8(qdst + h * D + dB, oB.x, oB.y);
       } else if (p.slot >= 0) {
-        *reinterpret_cast<uint2*>(kdst + (int64_t)(h - a.Hq) * a.pool.k_hs + dA) = oA;
-        *reinterpret_cast<uint2*>(kdst + (int64_t)(h - a.Hq) * a.pool.k_hs + dB) = oB;
+        st_nt8(kdst + (int64_t)(h - a.Hq) * a.pool.k_hs + dA, oA.x, oA.y);
+        st_nt8(kdst + (int64_t)(h - a.Hq) * a.pool.k_hs + dB, oB.x, oB.y);
       }
     }
   }
@@ -447,7 +450,9 @@ __device__ __forceinline__ void copy_part(const PageArgs& a, int64_t from, int64
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int c = (part * U + u) * 256 + threadIdx.x;
-    if (c < all) *reinterpret_cast<uint4*>(chunk_at(a, to, c)) = x[u];
+    if (c >= all) continue;
+    if (U > 1) st_nt16(chunk_at(a, to, c), x[u]);
+    else *reinterpret_cast<uint4*>(chunk_at(a, to, c)) = x[u];
   }
 }
 
@@ -486,7 +491,8 @@ __global__ __launch_bounds__(256) void fork_pages_kernel(PageArgs a) {
 }
 
 // Chunks of a thread: one while all its workgroups are in flight at once (5 pages of 64 KiB 2.4 us), four
-// for more (2048 pages: 47 us, 5.7 TB/s; 58 with nothing in the last-level cache).
+// for more, stored non-temporally: 2048 pages with nothing in the last-level cache 55 us, with plain stores 58;
+// where it holds both sides 53 against 45, but 512 pages 13.4 against 14.8.
 template <typename Go>
 void by_width(int64_t chunks, Go go) {
   if (chunks <= 256 * 1024) go(std::integral_constant<int, 1>{});
@@ -620,8 +626,8 @@ extern "C" int helm_rope_append(const void* qkv, int64_t qkv_stride_t, const voi
                            s, a, (int)v_items, qk_tiles);
       };
       // Heads of a workgroup: 16 make the factors least often, but are a chain; fewer where the chip has
-      // places left.  us with 4 / 8 / 16, 40 + 8 + 8 heads of 128: 300 rows (57 workgroups of 16) 6.4 / 8.1 / 12.2,
-      // 1024 (192) 11.5 / 11.2 / 14.3, 2048 (384) 18.5 / 17.0 / 19.4, 3926 (738) 28.7 / 27.6 / 25.6
+      // places left.  us with 4 / 8 / 16, 40 + 8 + 8 heads of 128: 300 rows (57 workgroups of 16) 6.5 / 8.4 / 11.5,
+      // 1024 (192) 10.4 / 10.0 / 12.8, 2048 (384) 15.8 / 14.1 / 15.3, 3000 (564) 21.7 / 20.6 / 18.8
       const int64_t wide = (int64_t)qk_tiles * ((Hq + Hkv + 15) / 16);
       if (wide >= 512) run(std::integral_constant<int, 16>{});
       else if (wide >= 192) run(std::integral_constant<int, 8>{});
