@@ -664,8 +664,9 @@ def _chunk(what: str, q: torch.Tensor, pool: PoolView, page_table: torch.Tensor,
         st, sh, _ = q.stride()
         qp = q.data_ptr()
     max_new = min(int(max_new), N)
-    # (what no key reaches is no window)
-    window = 0 if window >= max_pages * page_size else int(window)
+    # A window as long as the largest position hides nothing; one as long as the table does: lengths
+    # may pass the table.
+    window = 0 if window >= 2 ** 31 - 1 else int(window)
     sinks = min(int(sinks), max_pages * page_size) if window else 0
     need = chunk_workspace_bytes(N, B, Hq, Hkv, D, page_size, max_pages, max_new, window, sinks)
     ws = None
@@ -691,9 +692,10 @@ def chunk_attention(q: torch.Tensor, pool: PoolView, page_table: torch.Tensor, s
     Sequence b has rows q_starts[b] .. q_starts[b + 1] - 1 of q [N, Hq, D] fp16, its newest
     tokens; seq_lens[b] counts them and its cached ones, page_table [B, max_pages] holds its
     slots (all int32).  The token at position p sees keys j <= p; with a `window` of w > 0 only
-    j > p - w, and the first `sinks` tokens: pages that no new token sees may be freed (-1 in
-    the table), places that none sees may hold anything.  A token that sees no key gives zeros.  Rows before q_starts[0] and from
-    q_starts[B] on are not written, so a batch may be padded.
+    j > p - w (w up to 2^30), and the first `sinks` tokens: pages that no new token sees may be freed
+    (-1 in the table), places that none sees may hold anything.  A length may pass the table: its
+    keys end there, its positions do not.  A token that sees no key gives zeros.  Rows before
+    q_starts[0] and from q_starts[B] on are not written, so a batch may be padded.
 
     max_new bounds the new tokens of a sequence (any longer one has its first max_new rows
     written): the smaller, the fewer kernels run.  Lengths are read on the device: a captured
