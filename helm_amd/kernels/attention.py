@@ -161,6 +161,10 @@ class PoolView:
             held = self.__dict__["_held"] = (key, ctypes.byref(KvPoolStruct(*key)))
         return held[1]
 
+    def __getstate__(self):
+        # (a pointer can be neither copied nor pickled; c_ref makes the copy's own)
+        return {name: x for name, x in self.__dict__.items() if name != "_held"}
+
     @staticmethod
     def _check(k: torch.Tensor, v: torch.Tensor) -> None:
         d = k.shape[-1]
