@@ -41,6 +41,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr float kLazy = 8.f;            // lazy-rescale slack of the running maximum (log2)
+// What a probability is carried times 2^: the largest, 2^(kLazy + kLift), stays in fp16's range, and a
+// small one keeps 2^-11 of itself down to 2^-21 of the maximum's and 2^-32 of the maximum's below (at
+// 2^0, 131072 keys of 2^-25 beside one of 1 would vanish, 0.4% of the weight).
+constexpr float kLift = 7.f;
 constexpr int kMaxPieces = 64;          // of a tile's keys
 
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
@@ -625,8 +629,9 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
   v_at = (uint32_t)(kKC + (grp >> 1) * (D / 32) * 64 + (grp & 1) * 32 + col) * 16;
   auto lds_h8 = [&](uint32_t at) { return *reinterpret_cast<const h8_t*>(reinterpret_cast<const char*>(&s_kv[0][0]) + at); };
 
-  // m_run: what a column's scores are relative to (0 until it has met a key), thr: how far a
-  // score may pass it (a column that has met no key takes any)
+  // m_run: what a column's scores are relative to, kLift below the maximum it was last set to (0 until it
+  // has met a key), thr: how far a score may pass it (a column that has met no key takes any)
+  constexpr float kTop = kLazy + kLift;
   float m_run[NC], thr[NC];
   f4_t o[NC][DT], l_acc[NC];
 #pragma unroll
@@ -735,10 +740,10 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
         float m = fmaxf(mx[c], __shfl_xor(mx[c], 16, 64));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
         const bool up = m > thr[c];
-        const float by = up ? m : 0.f;
-        const float alpha = up ? (thr[c] == kLazy ? __builtin_amdgcn_exp2f(-by) : 0.f) : 1.f;
+        const float by = up ? m - kLift : 0.f;
+        const float alpha = up ? (thr[c] == kTop ? __builtin_amdgcn_exp2f(-by) : 0.f) : 1.f;
         m_run[c] += by;
-        thr[c] = up ? kLazy : thr[c];
+        thr[c] = up ? kTop : thr[c];
         l_acc[c] *= alpha;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[c][d] *= alpha;
@@ -796,7 +801,7 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
       float* dst = f.part_o + at * D + grp * 4;
 #pragma unroll
       for (int d = 0; d < DT; ++d) *reinterpret_cast<f4_t*>(dst + d * 16) = o[c][d];
-      if (grp == 0) *reinterpret_cast<float2*>(f.part_ml + at * 2) = make_float2(thr[c] == kLazy ? m_run[c] : -INFINITY, l);
+      if (grp == 0) *reinterpret_cast<float2*>(f.part_ml + at * 2) = make_float2(thr[c] == kTop ? m_run[c] : -INFINITY, l);
     } else {
       const float inv = l == 0.f ? 0.f : 1.f / l;       // (a row that sees nothing: zeros; NaN stays)
       const int tt = pos[c] - base;

@@ -1,5 +1,7 @@
 """chunk_attention where its definition is easy to miss: windows of sequences that are longer than
-their table."""
+their table, one key far above very many others."""
+import math
+
 import pytest
 import torch
 
@@ -37,3 +39,50 @@ def test_windows_past_2_to_the_30():
         b.window = window
         with pytest.raises(RuntimeError, match="2\\^30"):
             b.run()
+
+
+# ── one key far above very many others ───────────────────────────────────────
+
+def peaked(heads, batch, new, n, nats, at, page=64):
+    """`batch` sequences of n + 1 tokens over two slots: the key at `at` scores `nats` (a whole number of
+    2^-6) and has values of -1, all others score 0 and have values of +1.  The calls' arguments, and
+    what each of the `new` rows gives."""
+    hq, hkv, d = heads
+    k = torch.zeros(2, hkv, page, d, dtype=torch.float16, device="cuda")
+    v = ka.alloc_v((2, hkv, page, d), device="cuda")
+    v.fill_(1.0)
+    k[0, :, at % page, 0] = nats
+    v[0, :, at % page] = -1.0
+    table = torch.ones(batch, -(-(n + 1) // page), dtype=torch.int32, device="cuda")
+    table[:, at // page] = 0
+    q = torch.randn(batch * new, hq, d, generator=torch.Generator().manual_seed(0)).half().cuda()
+    q[..., 0] = 1.0
+    lens = torch.full((batch,), n + 1, dtype=torch.int32, device="cuda")
+    starts = torch.arange(batch + 1, dtype=torch.int32, device="cuda") * new
+    p = torch.arange(n + 1 - new, n + 1, dtype=torch.float64)          # others that a row sees
+    tail = p * math.exp(-nats)
+    return (q, ka.PoolView.of_pool(k, v), table, lens, starts, page), (tail - 1) / (tail + 1), tail / (tail + 1)
+
+
+# (n, nats): the others' share of the weight, their single weights from 2^-21 to 2^-25.2
+PEAKS = [(16384, 14.5), (131072, 15.0), (131072, 17.5), (262144, 16.265625)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(8, 8, 64), (8, 8, 128)])
+@pytest.mark.parametrize("n,nats", PEAKS)
+def test_many_rows_with_one_key_far_above_the_others(heads, n, nats):
+    """A weight w of the largest is off by 2^-11 w or, where it is small, by 2^-32 (fp16 at 2^7 of it), in
+    numerator and denominator alike: the output by 2^-11 sum w |v - o| <= 2^-11 4 tail, by 2 n 2^-32, by its
+    own rounding and by 2^-16 of the exponents'.  And the sums are fp32: a matrix instruction adds eight products
+    to a sum with one rounding to nearest, n keys are n / 8 of them, which one weight above all others
+    makes alike.  With that weight as 1 a numerator within (-1, 0) is off by 2^-25 each time, a denominator
+    within [1, 2) by 2^-24, the quotient by n (2^-28 + 2^-27) in all."""
+    for batch, at in ((64, 0), (64, 20000), (64, n // 2 + 5), (1, 0)):   # whole, and in pieces
+        at = min(at, n // 3)
+        args, want, tail = peaked(heads, batch, 40, n, nats, at)
+        got = ka.chunk_attention(*args, scale=1.0, max_new=40).cpu().double().view(batch, 40, -1)
+        want, tail = want.view(1, 40, 1), tail.view(1, 40, 1)
+        err = (got - want).abs()
+        tol = 2.0 ** -11 * want.abs() + 2.0 ** -9 * tail + n * (2.0 ** -31 + 2.0 ** -28 + 2.0 ** -27) + 2.0 ** -16
+        assert (err <= tol).all(), f"{batch} sequences, at {at}: off by {err.max().item():.2e}, {tol.min().item():.2e} allowed"
