@@ -276,8 +276,9 @@ __device__ __forceinline__ u32x4_t seen_bits(const ChunkArgs& a, const Steps& s,
 
 // NC tiles of 16 rows.  Steps of 32 keys, one wave each, round robin; K's and V's registers
 // are filled again as soon as they have been read (157 registers at NC = 1, 215 at 2: three and two
-// workgroups a CU).  P is split into fp16 hi + lo parts, so that the product keeps fp32's
-// accuracy (the matrix cores wait for memory anyway).
+// workgroups a CU).  P is split into fp16 hi + lo parts (the matrix cores wait for memory anyway): at
+// 2^kLift it enters the product to 2^-22 of itself, below 2^-21 of the maximum's to 2^-32 of that, where lo
+// has no bits left.  Its sum is that of the fp32 values.
 template <int D, int NC>
 struct FewLds {
   float o[kWaves][16 * NC][D];
@@ -411,7 +412,7 @@ __device__ __forceinline__ void few_body(const ChunkArgs& a, int hk, int item, F
         for (int d = 0; d < DT; ++d) o[c][d] *= alpha;
         m_run[c] = m_new;
       }
-      const float ref = m_run[c] == -INFINITY ? 0.f : -m_run[c];
+      const float ref = m_run[c] == -INFINITY ? 0.f : kLift - m_run[c];
       h8_t ph, pl;
       float sum = 0.f;
 #pragma unroll

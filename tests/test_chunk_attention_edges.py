@@ -86,3 +86,21 @@ def test_many_rows_with_one_key_far_above_the_others(heads, n, nats):
         err = (got - want).abs()
         tol = 2.0 ** -11 * want.abs() + 2.0 ** -9 * tail + n * (2.0 ** -31 + 2.0 ** -28 + 2.0 ** -27) + 2.0 ** -16
         assert (err <= tol).all(), f"{batch} sequences, at {at}: off by {err.max().item():.2e}, {tol.min().item():.2e} allowed"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(8, 8, 64), (8, 8, 128), (160, 8, 64)])
+@pytest.mark.parametrize("n,nats", PEAKS)
+def test_few_rows_with_one_key_far_above_the_others(heads, n, nats):
+    """In the product a weight w of the largest is off by 2^-22 w or, where it is small, by 2^-32 (two
+    fp16 parts at 2^7 of it), in the sum of the weights by nothing: the output by n 2^-32, by 2^-22, by its own
+    rounding and by 2^-16 of the exponents'.  And the sums are fp32: a wave adds a quarter of the keys, eight at a
+    time in two parts, n / 16 roundings of 2^-25 of the largest weight as above; its denominators, a lane's 8
+    keys of 32 at a time, n / 128 of 2^-24."""
+    for batch, at in ((64, 0), (64, 20000), (1, 0)):
+        at = min(at, n // 3)
+        args, want, _ = peaked(heads, batch, 1, n, nats, at)
+        got = ka.window_decode_attention(*args[:4], args[5], 0, scale=1.0).cpu().double().view(batch, -1)
+        err = (got - want).abs()
+        tol = 2.0 ** -11 * want.abs() + n * (2.0 ** -32 + 2.0 ** -29 + 2.0 ** -31) + 2.0 ** -22 + 2.0 ** -16
+        assert (err <= tol).all(), f"{batch} sequences, at {at}: off by {err.max().item():.2e}, {tol.min().item():.2e} allowed"
