@@ -1,10 +1,11 @@
 """chunk_attention where its definition is easy to miss: windows of sequences that are longer than
-their table, one key far above very many others."""
+their table, one key far above very many others, the bound of the workspace."""
 import math
 
 import pytest
 import torch
 
+from helm_amd import _native
 from helm_amd.kernels import attention as ka
 from test_chunk_attention import Batch
 
@@ -104,3 +105,23 @@ def test_few_rows_with_one_key_far_above_the_others(heads, n, nats):
         err = (got - want).abs()
         tol = 2.0 ** -11 * want.abs() + n * (2.0 ** -32 + 2.0 ** -29 + 2.0 ** -31) + 2.0 ** -22 + 2.0 ** -16
         assert (err <= tol).all(), f"{batch} sequences, at {at}: off by {err.max().item():.2e}, {tol.min().item():.2e} allowed"
+
+
+# ── workspace ────────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows,N,B,hq,hkv,pages,new,window,sinks", [
+    # (rows of a partial in each form that the call can run)
+    ((16,), 1, 1, 32, 8, 1024, 1, 4096, 4), ((16,), 300, 300, 16, 1, 900, 1, 0, 0), ((16,), 64, 64, 8, 8, 4096, 1, 0, 0),
+    ((16,), 9, 3, 5, 1, 77, 3, 0, 0), ((32,), 20, 4, 32, 8, 200, 5, 0, 0), ((32,), 40, 40, 40, 2, 333, 1, 2000, 0),
+    ((128,), 4096, 1, 40, 8, 1024, 4096, 0, 0), ((128,), 64, 2, 64, 1, 100, 60, 0, 0), ((128,), 7, 7, 34, 1, 640, 1, 0, 0),
+    ((16, 128), 700, 25, 40, 8, 512, 700, 0, 0), ((32, 128), 600, 9, 40, 2, 512, 300, 0, 0),
+    ((16, 128), 9000, 3, 32, 32, 990, 9000, 3000, 9), ((16, 128), 800, 3, 2048, 1024, 100, 700, 0, 0)])
+def test_workspace_of_each_form(rows, N, B, hq, hkv, pages, new, window, sinks, d):
+    """Partials of at most 512 / Hkv pieces a kv head and two more, of as many rows as the form's tiles,
+    D values and two numbers each, whatever the lengths; nothing where no sequence can have two pieces."""
+    f = _native.lib().helm_chunk_attn_workspace_bytes
+    pieces = hkv * (max(512 // hkv, 1) + 2)
+    bound = sum(pieces * r * (d + 2) * 4 for r in rows)
+    assert 0 < f(N, B, hq, hkv, d, 16, pages, new, window, sinks) <= bound
+    assert f(N, B, hq, hkv, d, 16, 8, new, window, sinks) == 0              # 128 tokens
