@@ -6,7 +6,9 @@
 // or j > p - window, or j < sinks).  out = softmax(scale q . K^T) V over those keys.
 //
 // All lengths are on the device, so what a workgroup does is found on the device too (the
-// plan, 1.4 us of a workgroup's start): each sequence's rows (token, head of the kv head's
+// plan, 1.4 us of a workgroup's start with up to 64 sequences; every wave reads all of them, 64 at a time,
+// so it grows with their number: one token after 100 of 32 heads takes 33 us with 256 sequences, 70 with 512, 165
+// with 1024): each sequence's rows (token, head of the kv head's
 // group; token-major) are cut into row tiles, each tile's keys into the sequence's number of
 // pieces, and workgroup x of a kv head takes the x-th (sequence, tile, piece).  Pieces are
 // sized so that all of them find places on the chip at once, whatever the lengths are;
@@ -19,13 +21,13 @@
 //   few_body   up to 16 or 32 rows (decode, drafts): bound by streaming K and V once; the four
 //              waves of a workgroup take key steps in turn.  16 items of up to 12000 tokens
 //              under a window of 2048, 40 heads over 8 (117 MB): 24 us and 4.5 for the merge;
-//              one item of 16384 under 4096 (17 MB): 7.8 and 3.9, a chain of round trips (kernel
+//              one item of 16384 under 4096 (17 MB): 7.3 and 4.5, a chain of round trips (kernel
 //              arguments, lengths, table, K / V) on either side of one step
 //   tile_body  more (prompts): bound by the matrix cores; the waves take rows and share K and V
-//              through LDS.  4096 tokens after 12288, 40 heads over 8: 1066 us, 1.13 PFLOP/s, 0.98 of
-//              what an 8192^3 fp16 product reaches on this card (1.16).  A workgroup's start and end
+//              through LDS.  4096 tokens after 12288, 40 heads over 8: 1075-1105 us, 1.09-1.12 PFLOP/s,
+//              0.95-0.98 of what an 8192^3 fp16 product reaches on this card (1.15).  A workgroup's start and end
 //              cost 8 us beside 1.9 a step of 64 keys (two workgroups a CU): prompts under a window of
-//              1024, 18 steps a tile, run at 0.79 PFLOP/s
+//              1024, 18 steps a tile, run at 0.80 PFLOP/s
 // A batch with sequences of both kinds runs them in one launch (both_attn_kernel).
 // Both forms run S^T = K . Q^T and O^T += V^T . P^T on v_mfma_f32_16x16x32_f16 with the keys of the
 // score tiles permuted so that each lane holds the probabilities of the 8 consecutive keys
@@ -755,7 +757,9 @@ __device__ __forceinline__ void tile_body(const ChunkArgs& a, int hk, int item, 
       }
     }
     // P enters the product rounded to fp16, and so do the sums (a product with ones): the
-    // rounding of a probability then moves numerator and denominator alike
+    // rounding of a probability then moves numerator and denominator alike, an output by 2^-11 sum p |v - o|
+    // at most (random data: 2.9e-4 of the output's size from the exact one, its own rounding is 2.1e-4 of
+    // that).  A second product of a low part, as few rows have, would be 32 more of a step's 68.
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       h8_t ph[NC];
@@ -828,8 +832,8 @@ __global__ __launch_bounds__(kThreads, 2) void tile_attn_kernel(ChunkArgs a) {
   tile_body<D, P, WIN>(a, (int)(blockIdx.x % (unsigned)a.Hkv), (int)(blockIdx.x / (unsigned)a.Hkv), lds);
 }
 // Both forms in one launch, the many rows' workgroups first: those of few rows wait for memory and
-// fill the places that are left.  700 rows after 8000 beside 24 single rows, 40 heads: 204 us, in two
-// launches 214, the two kinds in turn 260.
+// fill the places that are left.  700 rows after 8000 beside 24 single rows, 40 heads: 190 us.  Before the
+// products and exponentials were put in turn 204, in two launches 214, with the two kinds in turn 260.
 template <int D, int P, bool WIN>
 __global__ __launch_bounds__(kThreads, 2) void both_attn_kernel(ChunkArgs a) {
   __shared__ __attribute__((aligned(16))) union { FewLds<D, 1> few; TileLds<D> tile; } lds;

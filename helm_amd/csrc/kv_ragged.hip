@@ -388,9 +388,11 @@ __global__ __launch_bounds__(256, 4) void rope_tile_kernel(RopeArgs a, int v_ite
   }
 }
 
-// (row, head) rows from which the tile form is the faster one: 40 + 8 + 8 heads of 128 5600 rows 6.2 us
-// against 6.0, 8176 rows 6.1 against 7.0; 16 + 1 + 1 of 128 5400 rows 6.0 against 5.8; 16 + 8 + 8 of 64 6400 rows
-// 6.2 against 5.3, 9600 rows 6.2 against 6.4.
+// (row, head) rows from which the tile form is the faster one (us against the form above): 40 + 8 + 8 heads of
+// 128 5600 rows 5.5 / 5.3, 6384 5.6 / 5.6, 8176 5.7 / 6.2; 16 + 1 + 1 of 128 5598 5.5 / 5.3, 6390 5.5 / 5.7; 16 + 8
+// + 8 of 64 8160 5.7 / 5.1, 9600 5.8 / 5.7, 12000 5.8 / 6.4.  Half pairs of r dims that are no multiple of 8 stay
+// in the form above at any size: 4000 rows of 40 + 8 + 8 heads 90 us at r = 26 or 36 and 99 at 100, where r = 32
+// takes 27, 128 21 and interleaved pairs of any r 27.
 constexpr int64_t tile_rows(int D) { return D == 128 ? 6000 : 9000; }
 
 // ── pages moved inside a pool ────────────────────────────────────────────────

@@ -701,6 +701,11 @@ def chunk_attention(q: torch.Tensor, pool: PoolView, page_table: torch.Tensor, s
     keys end there, its positions do not.  A token that sees no key gives zeros.  Rows before
     q_starts[0] and from q_starts[B] on are not written, so a batch may be padded.
 
+    Sums and softmax are fp32.  Probabilities enter the product with 22 bits for sequences of few
+    rows (new tokens x query heads per kv head, up to 16 or 32: helm_chunk_attn) and rounded to fp16
+    for longer ones; in both, one below 2^-21 of the largest is off by up to 2^-32 of that.  K that a
+    row does not see may be anything; V that is not finite may reach the other rows of its sequence.
+
     max_new bounds the new tokens of a sequence (any longer one has its first max_new rows
     written): the smaller, the fewer kernels run.  Lengths are read on the device: a captured
     call takes other lengths of the same tensors at each replay.  How a sequence's keys are
@@ -769,8 +774,8 @@ def fork_pages(pool, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: 
       fresh[i] < 0    p's row as it is (the one child that goes on in p's own last page)
 
     parents and fresh are int32 [n]; a parent outside [0, B) gives a row of -1 and length 0.  A
-    length past the table counts as the table's.  Slots in `fresh` are in the pool, in use
-    nowhere, and named once.  The rows of several layers go in one call as rows of one table.
+    length past the table counts as the table's, and where the table is full there is no column for
+    `fresh`.  Slots in `fresh` are in the pool, in use nowhere, and named once.  The rows of several layers go in one call as rows of one table.
     The outputs must not overlap the inputs."""
     what = "fork_pages"
     P = _page_layout(what, pool, page_size)

@@ -138,7 +138,10 @@ def rope_scaled_inv_freq(rotary_dim: int, theta: float, kind: str, factor: float
                  them its turns weigh the two linearly
       "yarn"     the same two ends with weights linear in the dim's index between those of
                  beta_fast (rounded down) and beta_slow (rounded up) turns, and q and k both times
-                 0.1 ln(factor) + 1 (arXiv 2309.00071)"""
+                 0.1 ln(factor) + 1: the ends and the factor of arXiv 2309.00071, whose weights are
+                 linear in the turns ("bands"); weights by index, with the last one at most
+                 rotary_dim - 1 and a width of at least 1e-3, are the convention of the models that
+                 name this kind"""
     if rotary_dim < 2 or rotary_dim % 2:
         raise RuntimeError(f"rope_scaled_inv_freq: rotary_dim must be even and positive (got {rotary_dim})")
     if not factor >= 1.0:
@@ -247,7 +250,7 @@ def rope_append(qkv: torch.Tensor, pool, page_table: torch.Tensor, seq_lens: tor
     Sequence b has rows q_starts[b] .. q_starts[b + 1] - 1 of the fused projection qkv [N,
     (Hq + 2 Hkv) * D] fp16, the last of its seq_lens[b] tokens (None: one row each); the token
     at position p goes to slot page_table[b, p // P] at p % P (a place outside the table or the
-    pool is not written).  Per q and k head: RMSNorm where the norm weights are given, then the
+    pool is not written; two tokens must not name one place).  Per q and k head: RMSNorm where the norm weights are given, then the
     first 2 len(inv_freq) dims turn by the angle p * inv_freq[i] (in 64 bits), pairs (i, i + r/2)
     of the r rotated dims, or with `interleaved` (2 i, 2 i + 1), times rope_scale; the other
     dims pass.  All in fp32, q and k rounded once; v's bits are copied.  `positions` (int32 [N])

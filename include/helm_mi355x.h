@@ -323,10 +323,19 @@ int helm_prefill_attn_mask(const void* q, int64_t q_stride_t, int64_t q_stride_h
  *     that no row sees (those behind the window may be freed); keys past max_pages * P do
  *     not exist.  K and V of places that no row sees may hold anything, and K of any place
  *     that a row does not see (a V that is not finite may reach the rows beside those that see it).
+ *     A row whose scores are all -inf counts as one that sees no key.
+ *   - Sums and softmax are fp32.  Probabilities enter the product in two fp16 parts (22 bits) for
+ *     sequences of few rows (tokens times G = Hq / Hkv): up to 32 where max_new * G is at most 32
+ *     or G is 17 to 32, else up to 16; none where G is above 32, or max_new * G with B == 1.  For the
+ *     others they are rounded to fp16, in numerator and denominator alike: an output is off by up
+ *     to 2^-11 sum p |v - out| beside its own rounding.  In both, one below 2^-21 of the largest is off
+ *     by up to 2^-32 of that.
  *   - max_new: the most new tokens of a sequence that the call is prepared for (N: any);
  *     a sequence with more has only its first max_new rows written.
  *   - workspace (16-byte aligned, contents on entry do not matter) of at least
  *     helm_chunk_attn_workspace_bytes for the same numbers; 0: may be NULL.
+ *   - window and sinks up to 2^30.  A length may pass the table: the keys end there, positions and
+ *     windows go by the length.
  * The keys of sequences are cut by what else is in the batch, so a row's last bits can
  * depend on it; a call's bits do not change from run to run.  scale > 0; D 64 or 128; P 16,
  * 32 or 64; any Hq / Hkv.  The prefill SDPA of kv_offload.py:253-265 and the decode one of
@@ -429,8 +438,8 @@ int helm_copy_pages_q8(const struct helm_kv_pool_q8* pool, const int32_t* src, c
  *   fresh[i] <  0: p's row as it is
  *   fresh[i] >= 0: p's full pages, then fresh[i], then -1; where p's last page is not full it is
  *                  copied to slot fresh[i] (K and V whole)
- * Slots in fresh are in use nowhere and named once; outputs do not overlap inputs; tables of
- * at most 2^30 tokens.  Follows the page lists of helm/runtime/kv_cache.py:30-113, of which the
+ * (A full table has no column for fresh[i].)  Slots in fresh are in use nowhere and named once;
+ * outputs do not overlap inputs; tables of at most 2^30 tokens.  Follows the page lists of helm/runtime/kv_cache.py:30-113, of which the
  * reference keeps one per sequence and shares none. */
 int helm_fork_pages(const helm_kv_pool* pool, const int32_t* page_table, int64_t pt_stride,
                     const int32_t* seq_lens, int B, const int32_t* parents, const int32_t* fresh,
