@@ -775,8 +775,8 @@ def fork_pages(pool, page_table: torch.Tensor, seq_lens: torch.Tensor, parents: 
 
     parents and fresh are int32 [n]; a parent outside [0, B) gives a row of -1 and length 0.  A
     length past the table counts as the table's, and where the table is full there is no column for
-    `fresh`.  Slots in `fresh` are in the pool, in use nowhere, and named once.  The rows of several layers go in one call as rows of one table.
-    The outputs must not overlap the inputs."""
+    `fresh`.  Slots in `fresh` are in the pool, in use nowhere, and named once.  The rows of several
+    layers go in one call as rows of one table.  The outputs must not overlap the inputs."""
     what = "fork_pages"
     P = _page_layout(what, pool, page_size)
     index = _native.gpu_of(what, pool.k, pool.v, page_table, seq_lens, parents, fresh, table_out, lens_out)

@@ -250,9 +250,9 @@ def rope_append(qkv: torch.Tensor, pool, page_table: torch.Tensor, seq_lens: tor
     Sequence b has rows q_starts[b] .. q_starts[b + 1] - 1 of the fused projection qkv [N,
     (Hq + 2 Hkv) * D] fp16, the last of its seq_lens[b] tokens (None: one row each); the token
     at position p goes to slot page_table[b, p // P] at p % P (a place outside the table or the
-    pool is not written; two tokens must not name one place).  Per q and k head: RMSNorm where the norm weights are given, then the
-    first 2 len(inv_freq) dims turn by the angle p * inv_freq[i] (in 64 bits), pairs (i, i + r/2)
-    of the r rotated dims, or with `interleaved` (2 i, 2 i + 1), times rope_scale; the other
+    pool is not written; two tokens must not name one place).  Per q and k head: RMSNorm where the
+    norm weights are given, then the first 2 len(inv_freq) dims turn by the angle p * inv_freq[i] (in
+    64 bits), pairs (i, i + r/2) of the r rotated dims, or with `interleaved` (2 i, 2 i + 1), times rope_scale; the other
     dims pass.  All in fp32, q and k rounded once; v's bits are copied.  `positions` (int32 [N])
     gives angles of their own, places stay those of the cache.  inv_freq is fp32:
     rope_inv_freq, or rope_scaled_inv_freq for long contexts.

@@ -439,8 +439,9 @@ int helm_copy_pages_q8(const struct helm_kv_pool_q8* pool, const int32_t* src, c
  *   fresh[i] >= 0: p's full pages, then fresh[i], then -1; where p's last page is not full it is
  *                  copied to slot fresh[i] (K and V whole)
  * (A full table has no column for fresh[i].)  Slots in fresh are in use nowhere and named once;
- * outputs do not overlap inputs; tables of at most 2^30 tokens.  Follows the page lists of helm/runtime/kv_cache.py:30-113, of which the
- * reference keeps one per sequence and shares none. */
+ * outputs do not overlap inputs; tables of at most 2^30 tokens.  Follows the page lists of
+ * helm/runtime/kv_cache.py:30-113, of which the reference keeps one per sequence and shares
+ * none. */
 int helm_fork_pages(const helm_kv_pool* pool, const int32_t* page_table, int64_t pt_stride,
                     const int32_t* seq_lens, int B, const int32_t* parents, const int32_t* fresh,
                     int32_t* table_out, int64_t out_stride, int32_t* lens_out, int n, int max_pages,
