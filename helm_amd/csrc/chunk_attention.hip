@@ -8,8 +8,8 @@
 // All lengths are on the device, so what a workgroup does is found on the device too (the
 // plan, 1.4 us of a workgroup's start with up to 64 sequences; every wave reads all of them, 64 at a time,
 // so it grows with their number: one token after 100 of 32 heads takes 33 us with 256 sequences, 70 with 512, 165
-// with 1024): each sequence's rows (token, head of the kv head's group; token-major) are cut into row tiles, each tile's keys into the sequence's number of
-// pieces, and workgroup x of a kv head takes the x-th (sequence, tile, piece).  Pieces are
+// with 1024): each sequence's rows (token, head of the kv head's group; token-major) are cut into
+// row tiles, each tile's keys into the sequence's number of pieces, and workgroup x of a kv head takes the x-th (sequence, tile, piece).  Pieces are
 // sized so that all of them find places on the chip at once, whatever the lengths are;
 // sequences of one piece write their output, the others fp32 partials that a second kernel
 // merges.  The grid and the workspace depend on bounds that the host knows (plan_of).  The kv
